@@ -16,10 +16,12 @@ LIB_PATH = os.path.join(_HERE, "libenn_b200.so")
 
 try:
     from .abi_types import *          # noqa: F401,F403  (constants, descriptors, conv_desc)
-    from .abi_types import ConvDesc, FcDesc, AddDesc, PoolDesc, OpInfo, MeanDesc, ConcatDesc, SoftmaxDesc, ResizeDesc
+    from .abi_types import ConvDesc, FcDesc, AddDesc, PoolDesc, OpInfo, MeanDesc, ConcatDesc, SoftmaxDesc, ResizeDesc, \
+        TokenFcDesc, TokenNormDesc, TokenGateDesc, LogProbsDesc
 except ImportError:                   # loaded as a plain module
     from abi_types import *           # noqa: F401,F403
-    from abi_types import ConvDesc, FcDesc, AddDesc, PoolDesc, OpInfo, MeanDesc, ConcatDesc, SoftmaxDesc, ResizeDesc
+    from abi_types import ConvDesc, FcDesc, AddDesc, PoolDesc, OpInfo, MeanDesc, ConcatDesc, SoftmaxDesc, ResizeDesc, \
+        TokenFcDesc, TokenNormDesc, TokenGateDesc, LogProbsDesc
 
 # Every symbol include/enn_b200.h declares, with its prototype: (restype, argtypes).
 _P = C.c_void_p
@@ -48,6 +50,12 @@ PROTOTYPES = {
     "enn_b200_concat_prepare": (C.c_int32, [_P, C.POINTER(ConcatDesc), C.POINTER(_P)]),
     "enn_b200_softmax_prepare": (C.c_int32, [_P, C.POINTER(SoftmaxDesc), C.POINTER(_P)]),
     "enn_b200_resize_bilinear_prepare": (C.c_int32, [_P, C.POINTER(ResizeDesc), C.POINTER(_P)]),
+    "enn_b200_token_fc_prepare": (C.c_int32, [_P, C.POINTER(TokenFcDesc), _P, _P, _P, C.POINTER(_P)]),
+    "enn_b200_token_norm_prepare": (C.c_int32, [_P, C.POINTER(TokenNormDesc), _P, _P, _P, _P, C.POINTER(_P)]),
+    "enn_b200_token_gate_prepare": (C.c_int32, [_P, C.POINTER(TokenGateDesc), C.POINTER(_P)]),
+    "enn_b200_log_probs_prepare": (C.c_int32, [_P, C.POINTER(LogProbsDesc), C.POINTER(_P)]),
+    "enn_b200_token_pitch": (C.c_int64, [C.c_int32]),
+    "enn_b200_op_execute_rows": (C.c_int32, [_P, C.c_int32, C.POINTER(_P), C.c_int32, C.POINTER(_P), C.c_int32]),
     "enn_b200_op_set_impl": (C.c_int32, [_P, C.c_int32]),
     "enn_b200_op_execute": (C.c_int32, [_P, _P, _P]),
     "enn_b200_op_execute2": (C.c_int32, [_P, _P, _P, _P]),
@@ -62,6 +70,7 @@ PROTOTYPES = {
     "enn_b200_oplist_create": (C.c_int32, [_P, C.POINTER(_P)]),
     "enn_b200_oplist_add_tensor": (C.c_int32, [_P, C.c_int64, C.POINTER(C.c_int32)]),
     "enn_b200_oplist_add_op": (C.c_int32, [_P, _P, C.POINTER(C.c_int32), C.c_int32, C.c_int32]),
+    "enn_b200_oplist_add_op_n": (C.c_int32, [_P, _P, C.POINTER(C.c_int32), C.c_int32, C.POINTER(C.c_int32), C.c_int32]),
     "enn_b200_oplist_set_io": (C.c_int32, [_P, C.POINTER(C.c_int32), C.c_int32, C.POINTER(C.c_int32), C.c_int32]),
     "enn_b200_oplist_finalize": (C.c_int32, [_P]),
     "enn_b200_oplist_execute": (C.c_int32, [_P, C.POINTER(_P), C.POINTER(_P)]),
@@ -234,6 +243,14 @@ class Op:
         arr = (C.c_void_p * len(in_devs))(*[p.value if hasattr(p, "value") else p for p in in_devs])
         self.ctx.check(lib.enn_b200_op_execute_n(self.h, arr, len(in_devs), out_dev))
 
+    def execute_rows(self, rows, in_devs, out_devs):
+        """Token operators: the first `rows` rows, device addresses of the inputs and outputs in the descriptor's order."""
+        ins = (C.c_void_p * len(in_devs))(*[p.value if hasattr(p, "value") else p for p in in_devs])
+        outs = (C.c_void_p * len(out_devs))(*[p.value if hasattr(p, "value") else p for p in out_devs])
+        st = lib.enn_b200_op_execute_rows(self.h, rows, ins, len(in_devs), outs, len(out_devs))
+        if st != SUCCESS:
+            self.ctx.check(st)
+
     def run_n(self, xs):
         """Upload several host arrays, execute the n-input form, download."""
         devs = [self.ctx.to_device(x) for x in xs]
@@ -344,6 +361,44 @@ def resize_bilinear(ctx, desc):
     return _prepare_simple(ctx, lib.enn_b200_resize_bilinear_prepare, desc)
 
 
+def token_pitch(c):
+    """Bytes from row to row of byte rows of c channels."""
+    return lib.enn_b200_token_pitch(c)
+
+
+def _vector(v, dtype, size=None):
+    """A constant of a token operator: None, a host array, or the address of host or device memory."""
+    if v is None or isinstance(v, int) or hasattr(v, "value"):
+        return v, v
+    a = np.ascontiguousarray(v, dtype=dtype)
+    if size is not None and a.size != size:
+        raise ValueError(f"a constant of {a.size} values where {size} are needed")
+    return _np_ptr(a), a
+
+
+def _prepare_token(ctx, fn, desc, *constants):
+    h = C.c_void_p()
+    ctx.check(fn(ctx.h, C.byref(desc), *[p for p, _ in constants], C.byref(h)))      # `constants` keeps the arrays alive
+    return Op(ctx, h)
+
+
+def token_fc(ctx, desc, w, channel_scales, bias=None):
+    return _prepare_token(ctx, lib.enn_b200_token_fc_prepare, desc, _vector(w, np.int8, desc.n * desc.k),
+                          _vector(channel_scales, np.float32, desc.n), _vector(bias, np.float32, desc.n))
+
+
+def token_norm(ctx, desc, weight=None, bias=None, post_weight=None, post_bias=None):
+    return _prepare_token(ctx, lib.enn_b200_token_norm_prepare, desc, *[_vector(v, np.float32, desc.c) for v in (weight, bias, post_weight, post_bias)])
+
+
+def token_gate(ctx, desc):
+    return _prepare_simple(ctx, lib.enn_b200_token_gate_prepare, desc)
+
+
+def log_probs(ctx, desc):
+    return _prepare_simple(ctx, lib.enn_b200_log_probs_prepare, desc)
+
+
 class OpList:
     """Operator list with BufferTable-style tensor ids (GpuUserDriver Open/Execute/CloseSubGraph)."""
 
@@ -363,6 +418,12 @@ class OpList:
     def add(self, op, in_ids, out_id):
         ids = (C.c_int32 * len(in_ids))(*in_ids)
         self.ctx.check(lib.enn_b200_oplist_add_op(self.h, op.h, ids, len(in_ids), out_id))
+        op.h = None        # owned by the list now
+
+    def add_n(self, op, in_ids, out_ids):
+        """An operator with several outputs."""
+        ins, outs = (C.c_int32 * len(in_ids))(*in_ids), (C.c_int32 * len(out_ids))(*out_ids)
+        self.ctx.check(lib.enn_b200_oplist_add_op_n(self.h, op.h, ins, len(in_ids), outs, len(out_ids)))
         op.h = None        # owned by the list now
 
     def set_io(self, inputs, outputs, out_bytes):

@@ -10,6 +10,10 @@ import numpy as np
 SUCCESS, FAILURE, CUDA_FAILURE, INVALID_PARAMS = 0, 1, 2, 3
 ACT_NONE, ACT_RELU, ACT_RELU1, ACT_RELU6 = 0, 1, 2, 3
 U8, S8 = 0, 1
+F32, F16, BF16 = 16, 17, 18                       # token operators only
+NORM_NONE, NORM_RMS, NORM_LAYER = 0, 1, 2
+GATE_SILU, GATE_GELU, GATE_GELU_TANH, GATE_RELU, GATE_SIGMOID = 0, 1, 2, 3, 4
+LOG_PROBS_MAX_TOP = 32
 W_OIHW, W_OHWI, W_IOHW = 0, 1, 2
 IMPL_DIRECT, IMPL_TCGEN05, IMPL_GEMV, IMPL_DEPTHWISE, IMPL_ELTWISE = 0, 1, 2, 3, 4
 
@@ -63,6 +67,23 @@ class SoftmaxDesc(C.Structure):
 
 class ResizeDesc(C.Structure):
     _fields_ = [(n, C.c_int32) for n in ("n", "h", "w", "c", "out_h", "out_w", "align_corners", "half_pixel_centers", "act_dtype")]
+
+
+class TokenFcDesc(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("m", "k", "n", "out_dtype")] + [("in_pitch", C.c_int64)]
+
+
+class TokenNormDesc(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("m", "c", "norm", "post_norm", "residual", "gate_tokens", "io_dtype", "out_dtype")] + [
+        ("eps", C.c_float), ("post_eps", C.c_float), ("residual_scale", C.c_float)]
+
+
+class TokenGateDesc(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("m", "c", "act", "packed", "in_dtype", "out_dtype")]
+
+
+class LogProbsDesc(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("m", "vocab", "in_dtype", "given", "top")] + [("scale", C.c_float), ("in_pitch", C.c_int64)]
 
 
 def mean_desc(dims, axes, act_dtype=U8):

@@ -37,7 +37,8 @@ struct enn_b200_context {
 
 namespace enn_b200 {
 
-enum OpKind { OP_CONV = 0, OP_DEPTHWISE = 1, OP_DECONV = 2, OP_FC = 3, OP_ADD = 4, OP_AVGPOOL = 5, OP_MAXPOOL = 6, OP_MEAN = 7, OP_CONCAT = 8, OP_SOFTMAX = 9, OP_RESIZE = 10 };
+enum OpKind { OP_CONV = 0, OP_DEPTHWISE = 1, OP_DECONV = 2, OP_FC = 3, OP_ADD = 4, OP_AVGPOOL = 5, OP_MAXPOOL = 6, OP_MEAN = 7, OP_CONCAT = 8, OP_SOFTMAX = 9, OP_RESIZE = 10,
+              OP_TOKEN_FC = 11, OP_TOKEN_NORM = 12, OP_TOKEN_GATE = 13, OP_LOG_PROBS = 14 };
 
 // Geometry + quantisation handed to kernels by value.
 struct ConvGeom {
@@ -79,6 +80,8 @@ __host__ __device__ inline uint32_t add_lut2_index(uint32_t a, uint32_t b) {
     return idx ^ ((idx >> 6) & 0x7cu);
 }
 
+struct TokenState;     // token_ops.h
+
 struct PoolGeom {
     int32_t n, h, w, c, kh, kw, sh, sw, pt, pl, oh, ow;
     int32_t act_min, act_max, is_signed;
@@ -115,6 +118,7 @@ struct enn_b200_op {
     void *dw_ring = nullptr;           // depthwise row-ring plan (depthwise.cu), owned
     void *tc = nullptr;                // tensor-core plan (gemm_tc.cu), owned
     void *graph_state = nullptr;       // state of Mean / Concat / Softmax / Resize (graph_ops.cu), owned
+    enn_b200::TokenState *token = nullptr;   // token operators (token_ops.h), owned
     std::unique_ptr<RuntimeConstants> dyn;   // set when the descriptor said weights_as_input / bias_as_input
     enn_b200_op *fused_add = nullptr;  // convolution + quantized add: the add operator whose table the epilogue uses (owned)
 };
@@ -146,6 +150,7 @@ cudaError_t launch_avgpool(const PoolGeom &p, const void *in, void *out, cudaStr
 cudaError_t launch_maxpool(const PoolGeom &p, const void *in, void *out, cudaStream_t s);
 cudaError_t launch_graph_op(enn_b200_op *op, const void *const *ins, int n_in, void *out);     // Mean, Concat, Softmax, Resize
 void graph_op_release(enn_b200_op *op);
+void token_release(enn_b200_op *op);                                                           // token_abi.cu
 cudaError_t launch_transpose_nchw_nhwc(const void *src, void *dst, int n, int c, int h, int w, bool to_nhwc,
                                        cudaStream_t s);
 

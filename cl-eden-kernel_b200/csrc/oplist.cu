@@ -16,6 +16,9 @@
 #include <new>
 
 #include "internal.h"
+#include "token_ops.h"
+
+using enn_b200::TokenCall;
 
 struct enn_b200_oplist {
     enn_b200_context *ctx = nullptr;
@@ -30,7 +33,9 @@ struct enn_b200_oplist {
     struct Node {
         enn_b200_op *op = nullptr;
         std::vector<int> ins;
-        int out = -1;
+        int out = -1;                  // the first output
+        std::vector<int> more_outs;    // the others of an operator with several
+        bool writes(int t) const { return out == t || std::find(more_outs.begin(), more_outs.end(), t) != more_outs.end(); }
     };
     std::vector<Tensor> tensors;
     std::vector<Node> nodes;
@@ -59,15 +64,25 @@ int32_t lfail(enn_b200_oplist *l, int32_t st, const char *msg) {
     if (l && l->ctx) l->ctx->last_error = msg;
     return st;
 }
+// Enqueues one node; ptr(tensor id) is the device memory of a tensor.
+template <typename F>
+int32_t run_node(const enn_b200_oplist::Node &n, F ptr) {
+    const void *ins[ENN_B200_CONCAT_MAX_INPUTS];
+    const int32_t n_in = static_cast<int32_t>(n.ins.size());
+    for (int32_t i = 0; i < n_in; ++i) ins[i] = ptr(n.ins[i]);
+    if (!n.op->token) return enn_b200_op_execute_n(n.op, ins, n_in, ptr(n.out));
+    void *outs[TokenCall::kMaxOuts] = {ptr(n.out)};
+    int32_t n_out = 1;
+    for (int t : n.more_outs) outs[n_out++] = ptr(t);
+    return enn_b200_op_execute_rows(n.op, n.op->token->call.m, ins, n_in, outs, n_out);
+}
 int32_t run_nodes(enn_b200_oplist *l, int slot = 0) {
     auto ptr = [&](int t) {
         auto &T = l->tensors[t];
         return (slot == 1 && T.dev_alt) ? T.dev_alt : T.dev;
     };
     for (auto &n : l->nodes) {
-        const void *ins[ENN_B200_CONCAT_MAX_INPUTS];
-        for (size_t i = 0; i < n.ins.size(); ++i) ins[i] = ptr(n.ins[i]);
-        const int32_t st = enn_b200_op_execute_n(n.op, ins, static_cast<int32_t>(n.ins.size()), ptr(n.out));
+        const int32_t st = run_node(n, ptr);
         if (st != ENN_B200_SUCCESS) return st;
     }
     return ENN_B200_SUCCESS;
@@ -97,6 +112,7 @@ int32_t enn_b200_oplist_add_tensor(enn_b200_oplist *l, int64_t bytes, int32_t *t
 
 int32_t enn_b200_oplist_add_op(enn_b200_oplist *l, enn_b200_op *op, const int32_t *in_ids, int32_t n_in, int32_t out_id) {
     if (!l || !op || !in_ids || n_in < 1 || n_in > ENN_B200_CONCAT_MAX_INPUTS) return lfail(l, ENN_B200_INVALID_PARAMS, "oplist_add_op: bad argument");
+    if (op->token) return enn_b200_oplist_add_op_n(l, op, in_ids, n_in, &out_id, 1);
     if (l->finalized) return lfail(l, ENN_B200_FAILURE, "oplist already finalized");
     if (op->dyn) return lfail(l, ENN_B200_INVALID_PARAMS, "oplist_add_op: operators with runtime filter / bias run outside operator lists");
     const int nt = static_cast<int>(l->tensors.size());
@@ -119,6 +135,32 @@ int32_t enn_b200_oplist_add_op(enn_b200_oplist *l, enn_b200_op *op, const int32_
     n.op = op;
     n.ins.assign(in_ids, in_ids + n_in);
     n.out = out_id;
+    l->nodes.push_back(n);
+    return ENN_B200_SUCCESS;
+}
+
+int32_t enn_b200_oplist_add_op_n(enn_b200_oplist *l, enn_b200_op *op, const int32_t *in_ids, int32_t n_in, const int32_t *out_ids, int32_t n_out) {
+    if (!l || !op || !in_ids || !out_ids) return lfail(l, ENN_B200_INVALID_PARAMS, "oplist_add_op_n: bad argument");
+    if (!op->token) return n_out == 1 ? enn_b200_oplist_add_op(l, op, in_ids, n_in, out_ids[0]) : lfail(l, ENN_B200_INVALID_PARAMS, "oplist_add_op_n: this operator has one output");
+    if (l->finalized) return lfail(l, ENN_B200_FAILURE, "oplist already finalized");
+    if (op->ctx != l->ctx) return lfail(l, ENN_B200_INVALID_PARAMS, "oplist_add_op_n: the operator belongs to another context");
+    const TokenCall &c = op->token->call;
+    if (n_in != c.n_in || n_out != c.n_out) return lfail(l, ENN_B200_INVALID_PARAMS, "oplist_add_op_n: wrong input or output count for this operator");
+    const int nt = static_cast<int>(l->tensors.size());
+    for (int i = 0; i < n_in; ++i)
+        if (in_ids[i] < 0 || in_ids[i] >= nt || l->tensors[in_ids[i]].bytes < c.in_bytes[i]) return lfail(l, ENN_B200_INVALID_PARAMS, "oplist_add_op_n: bad input tensor id, or the tensor is too small");
+    for (int o = 0; o < n_out; ++o) {
+        if (out_ids[o] < 0 || out_ids[o] >= nt || l->tensors[out_ids[o]].bytes < c.out_bytes[o]) return lfail(l, ENN_B200_INVALID_PARAMS, "oplist_add_op_n: bad output tensor id, or the tensor is too small");
+        for (int i = 0; i < n_in; ++i)
+            if (out_ids[o] == in_ids[i] && !(c.in_place && o == 0 && i == 1)) return lfail(l, ENN_B200_INVALID_PARAMS, "oplist_add_op_n: an output must not be an input");
+        for (int p = 0; p < o; ++p)
+            if (out_ids[o] == out_ids[p]) return lfail(l, ENN_B200_INVALID_PARAMS, "oplist_add_op_n: an output named twice");
+    }
+    enn_b200_oplist::Node n;
+    n.op = op;
+    n.ins.assign(in_ids, in_ids + n_in);
+    n.out = out_ids[0];
+    n.more_outs.assign(out_ids + 1, out_ids + n_out);
     l->nodes.push_back(n);
     return ENN_B200_SUCCESS;
 }
@@ -165,19 +207,19 @@ int32_t enn_b200_oplist_finalize(enn_b200_oplist *l) {
                 if (M.is_input || M.is_output || readers[mid] != 1) continue;
                 int prod = -1;
                 for (size_t c = 0; c < a; ++c)
-                    if (l->nodes[c].out == mid) prod = static_cast<int>(c);      // the last writer before the add
+                    if (l->nodes[c].writes(mid)) prod = static_cast<int>(c);      // the last writer before the add
                 if (prod < 0 || l->nodes[prod].op->kind != enn_b200::OP_CONV || l->nodes[prod].ins.size() != 1) continue;
                 // The other addend must exist before the convolution runs.
                 const int other = add.ins[1 - side];
                 bool other_ready = l->tensors[other].is_input;
                 for (int c = 0; c < prod; ++c)
-                    if (l->nodes[c].out == other) other_ready = true;
+                    if (l->nodes[c].writes(other)) other_ready = true;
                 for (size_t c = prod; c < a; ++c)
-                    if (l->nodes[c].out == other) other_ready = false;            // rewritten in between
+                    if (l->nodes[c].writes(other)) other_ready = false;            // rewritten in between
                 if (!other_ready) continue;
                 bool touched = false;      // nothing between the two may read or write the add's output tensor
                 for (size_t c = prod; c < a && !touched; ++c) {
-                    touched = l->nodes[c].out == add.out;
+                    touched = l->nodes[c].writes(add.out);
                     for (int t : l->nodes[c].ins) touched = touched || t == add.out;
                 }
                 if (touched) continue;
@@ -200,9 +242,13 @@ int32_t enn_b200_oplist_finalize(enn_b200_oplist *l) {
             if (T.first_def < 0 && !T.is_input) return lfail(l, ENN_B200_INVALID_PARAMS, "oplist: tensor read before it is written");
             T.last_use = i;
         }
-        auto &O = l->tensors[n.out];
-        if (O.first_def < 0) O.first_def = i;
-        O.last_use = std::max(O.last_use, i);
+        auto written = [&](int t) {
+            auto &O = l->tensors[t];
+            if (O.first_def < 0) O.first_def = i;
+            O.last_use = std::max(O.last_use, i);
+        };
+        written(n.out);
+        for (int t : n.more_outs) written(t);
     }
     // Liveness-based assignment: graph inputs/outputs get dedicated buffers (the caller's copies land there);
     // an intermediate takes the smallest free pool buffer that fits, and returns it after its last reader.
@@ -216,8 +262,9 @@ int32_t enn_b200_oplist_finalize(enn_b200_oplist *l) {
     for (auto &T : l->tensors)
         if (T.is_input || T.is_output || T.first_def < 0) T.pool_slot = new_slot(T.bytes);
     for (int i = 0; i < n_nodes; ++i) {
-        auto &T = l->tensors[l->nodes[i].out];
-        if (T.pool_slot < 0) {
+        auto place = [&](int t) {
+            auto &T = l->tensors[t];
+            if (T.pool_slot >= 0) return;
             int best = -1;
             for (size_t k = 0; k < free_slots.size(); ++k) {
                 const int s = free_slots[k];
@@ -230,7 +277,9 @@ int32_t enn_b200_oplist_finalize(enn_b200_oplist *l) {
                 T.pool_slot = new_slot(T.bytes);
             }
             expiring[T.last_use].push_back(T.pool_slot);
-        }
+        };
+        place(l->nodes[i].out);
+        for (int t : l->nodes[i].more_outs) place(t);
         // Buffers whose last reader is this node become free for the NEXT node (never for this node's output).
         for (int s : expiring[i]) free_slots.push_back(s);
     }
@@ -471,9 +520,7 @@ int32_t enn_b200_oplist_profile(enn_b200_oplist *l, int32_t repeats, float *node
         cudaEventRecord(ev[0], ctx->stream);
         for (int i = 0; i < n && st == ENN_B200_SUCCESS; ++i) {
             const auto &nd = l->nodes[i];
-            const void *ins[ENN_B200_CONCAT_MAX_INPUTS];
-            for (size_t k = 0; k < nd.ins.size(); ++k) ins[k] = l->tensors[nd.ins[k]].dev;
-            st = enn_b200_op_execute_n(nd.op, ins, static_cast<int32_t>(nd.ins.size()), l->tensors[nd.out].dev);
+            st = run_node(nd, [&](int t) { return l->tensors[t].dev; });
             cudaEventRecord(ev[i + 1], ctx->stream);
         }
         if (st == ENN_B200_SUCCESS && cudaStreamSynchronize(ctx->stream) != cudaSuccess) st = lfail(l, ENN_B200_CUDA_FAILURE, "oplist_profile: execution failed");

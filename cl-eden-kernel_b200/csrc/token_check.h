@@ -1,0 +1,139 @@
+// Checks of the token operators' descriptors and calls, and the sizes that follow from them.  Host code without CUDA, so that the
+// refusals are tested without a device.
+#pragma once
+#include <stdint.h>
+
+#include <cmath>
+
+#include "../../include/enn_b200.h"
+
+namespace enn_b200 {
+
+// What a call of a prepared token operator is checked against.
+struct TokenCall {
+    static constexpr int kMaxIns = 3, kMaxOuts = 4;
+    int32_t m = 0;
+    int32_t n_in = 0, n_out = 0;
+    int64_t in_bytes[kMaxIns] = {}, out_bytes[kMaxOuts] = {};      // of all m rows
+    int32_t in_align[kMaxIns] = {}, out_align[kMaxOuts] = {};      // element sizes
+    bool in_place = false;                                          // out 0 may be the memory of in 1 (token_norm's stream)
+
+    void add_in(int64_t bytes, int32_t align) {
+        in_align[n_in] = align;
+        in_bytes[n_in++] = bytes;
+    }
+    void add_out(int64_t bytes, int32_t align) {
+        out_align[n_out] = align;
+        out_bytes[n_out++] = bytes;
+    }
+};
+
+inline int32_t float_size(int32_t dtype) {
+    return dtype == ENN_B200_F32 ? 4 : (dtype == ENN_B200_F16 || dtype == ENN_B200_BF16 ? 2 : 0);
+}
+
+inline int64_t token_pitch(int32_t c) { return (static_cast<int64_t>(c) + 15) & ~int64_t{15}; }
+
+// The check_* return null and fill `call`, or what is wrong with the descriptor.
+inline const char *check_token_fc(const enn_b200_token_fc_desc &d, TokenCall *call) {
+    if (d.m < 0 || d.k <= 0 || d.n <= 0 || d.n > (1 << 21)) return "token_fc: bad shape (n is 1 .. 2^21)";
+    if (d.k >= 131072) return "token_fc: k must be below 131072 (sums of products are 32-bit)";
+    const int32_t e = float_size(d.out_dtype);
+    if (!e) return "token_fc: out_dtype must be F32, F16 or BF16";
+    if (d.in_pitch != 0 && d.in_pitch < d.k) return "token_fc: rows overlap (in_pitch < k)";
+    if (d.in_pitch > (int64_t{1} << 38)) return "token_fc: in_pitch is too large";
+    const int64_t pitch = d.in_pitch ? d.in_pitch : token_pitch(d.k);
+    call->m = d.m;
+    call->add_in(d.m ? (d.m - 1) * pitch + d.k : 0, 1);
+    call->add_in(int64_t{4} * d.m, 4);
+    call->add_out(static_cast<int64_t>(d.m) * d.n * e, e);
+    return nullptr;
+}
+
+inline bool token_out(TokenCall *call, int32_t m, int32_t c, int32_t dtype) {
+    if (dtype == ENN_B200_S8) {
+        call->add_out(m * token_pitch(c), 1);
+        call->add_out(int64_t{4} * m, 4);
+        return true;
+    }
+    const int32_t e = float_size(dtype);
+    call->add_out(static_cast<int64_t>(m) * c * e, e);
+    return e != 0;
+}
+
+inline const char *check_token_norm(const enn_b200_token_norm_desc &d, TokenCall *call) {
+    if (d.m < 0 || d.c <= 0) return "token_norm: bad shape";
+    if (d.c > 32768) return "token_norm: c must be at most 32768";
+    if (d.norm < ENN_B200_NORM_NONE || d.norm > ENN_B200_NORM_LAYER || d.post_norm < ENN_B200_NORM_NONE || d.post_norm > ENN_B200_NORM_LAYER)
+        return "token_norm: unknown norm";
+    const int32_t e = float_size(d.io_dtype);
+    if (!e) return "token_norm: io_dtype must be F32, F16 or BF16";
+    if (d.gate_tokens < 0) return "token_norm: gate_tokens must not be negative";
+    if (!(d.eps >= 0.f) || !(d.post_eps >= 0.f) || std::isinf(d.eps) || std::isinf(d.post_eps)) return "token_norm: eps must be finite and not negative";
+    if (!std::isfinite(d.residual_scale)) return "token_norm: residual_scale must be finite";
+    const int64_t row = static_cast<int64_t>(d.c) * e;
+    call->m = d.m;
+    call->add_in(d.m * row, e);
+    if (d.residual) call->add_in(d.m * row, e);
+    if (d.gate_tokens) call->add_in((d.m / d.gate_tokens + (d.m % d.gate_tokens ? 1 : 0)) * row, e);
+    if (d.residual) call->add_out(d.m * row, e);
+    call->in_place = d.residual != 0;
+    return token_out(call, d.m, d.c, d.out_dtype) ? nullptr : "token_norm: out_dtype must be F32, F16, BF16 or S8";
+}
+
+inline const char *check_token_gate(const enn_b200_token_gate_desc &d, TokenCall *call) {
+    if (d.m < 0 || d.c <= 0) return "token_gate: bad shape";
+    if (d.c > 65536) return "token_gate: c must be at most 65536";
+    if (d.act < ENN_B200_GATE_SILU || d.act > ENN_B200_GATE_SIGMOID) return "token_gate: unknown activation";
+    const int32_t e = float_size(d.in_dtype);
+    if (!e) return "token_gate: in_dtype must be F32, F16 or BF16";
+    const int64_t row = static_cast<int64_t>(d.c) * e;
+    call->m = d.m;
+    call->add_in(d.m * row * (d.packed ? 2 : 1), e);
+    if (!d.packed) call->add_in(d.m * row, e);
+    return token_out(call, d.m, d.c, d.out_dtype) ? nullptr : "token_gate: out_dtype must be F32, F16, BF16 or S8";
+}
+
+inline const char *check_log_probs(const enn_b200_log_probs_desc &d, TokenCall *call) {
+    if (d.m < 0 || d.vocab <= 0 || d.vocab > (1 << 24)) return "log_probs: bad shape (vocab is 1 .. 2^24)";
+    const int32_t e = float_size(d.in_dtype);
+    if (!e) return "log_probs: in_dtype must be F32, F16 or BF16";
+    if (d.given < 0 || d.given > 1024) return "log_probs: given must be within 0 .. 1024";
+    if (d.top < 0 || d.top > ENN_B200_LOG_PROBS_MAX_TOP || d.top > d.vocab) return "log_probs: top must be within 0 .. min(vocab, 32)";
+    if (!(d.scale > 0.f) || std::isinf(d.scale)) return "log_probs: scale must be positive and finite";
+    if (d.in_pitch != 0 && d.in_pitch < d.vocab) return "log_probs: rows overlap (in_pitch < vocab)";
+    if (d.in_pitch > (int64_t{1} << 38)) return "log_probs: in_pitch is too large";
+    const int64_t pitch = d.in_pitch ? d.in_pitch : d.vocab;
+    call->m = d.m;
+    call->add_in(d.m ? ((d.m - 1) * pitch + d.vocab) * e : 0, e);
+    if (d.given) call->add_in(int64_t{4} * d.m * d.given, 4);
+    if (d.given) call->add_out(int64_t{4} * d.m * d.given, 4);
+    call->add_out(int64_t{4} * d.m, 4);
+    if (d.top) {
+        call->add_out(int64_t{4} * d.m * d.top, 4);
+        call->add_out(int64_t{4} * d.m * d.top, 4);
+    }
+    return nullptr;
+}
+
+// A call of enn_b200_op_execute_rows: null, or what is wrong with it.
+inline const char *check_rows_call(const TokenCall &c, int32_t rows, const void *const *ins, int32_t n_in, void *const *outs, int32_t n_out) {
+    if (rows < 0 || rows > c.m) return "rows must be within 0 and the prepared m";
+    if (n_in != c.n_in || n_out != c.n_out || !ins || !outs) return "wrong number of inputs or outputs for this operator";
+    if (rows == 0) return nullptr;      // nothing is touched: empty tensors have no address
+    for (int i = 0; i < n_in; ++i) {
+        if (!ins[i]) return "null device pointer";
+        if (reinterpret_cast<uintptr_t>(ins[i]) % c.in_align[i]) return "an input is not aligned to its element type";
+    }
+    for (int o = 0; o < n_out; ++o) {
+        if (!outs[o]) return "null device pointer";
+        if (reinterpret_cast<uintptr_t>(outs[o]) % c.out_align[o]) return "an output is not aligned to its element type";
+        for (int i = 0; i < n_in; ++i)
+            if (outs[o] == ins[i] && !(c.in_place && o == 0 && i == 1)) return "an output must not be an input's memory";
+        for (int p = 0; p < o; ++p)
+            if (outs[o] == outs[p]) return "two outputs must not be the same memory";
+    }
+    return nullptr;
+}
+
+}  // namespace enn_b200

@@ -1,0 +1,99 @@
+// State and device helpers of the token operators (token_fc, token_norm, token_gate, log_probs).
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "internal.h"
+#include "token_check.h"
+
+namespace enn_b200 {
+
+struct NormParams {
+    int32_t c;
+    int32_t norm, post_norm;
+    int32_t gate_tokens;
+    float eps, post_eps, residual_scale;
+    const float *weight, *bias, *post_weight, *post_bias;      // null: ones / zeros
+    int64_t pitch;                                              // bytes from row to row of byte rows
+};
+
+struct GateParams {
+    int32_t c, act;
+    int64_t in_stride;      // elements from row to row of the gates and of the values
+    int64_t pitch;
+};
+
+struct LogProbsParams {
+    int32_t vocab, given, top;
+    float scale;
+    int64_t pitch;          // logits from row to row
+};
+
+struct TokenFcParams {
+    int32_t k, n;
+    int64_t in_pitch;
+    int64_t w_pitch;
+    const int8_t *w;        // [n][w_pitch], zero beyond k
+    const float *channel_scale, *bias;
+};
+
+// Everything a prepared token operator holds; deleted by the operator's release.
+struct TokenState {
+    TokenCall call;
+    int32_t in_dtype = 0, out_dtype = 0;
+    bool residual = false, packed = false;
+    NormParams norm{};
+    GateParams gate{};
+    LogProbsParams log_probs{};
+    TokenFcParams fc{};
+};
+
+// One launch sequence for `rows` > 0 rows on `stream`; pointers in the descriptor's order.
+cudaError_t token_norm_launch(const TokenState &t, int32_t rows, const void *const *ins, void *const *outs, cudaStream_t stream);
+cudaError_t token_gate_launch(const TokenState &t, int32_t rows, const void *const *ins, void *const *outs, cudaStream_t stream);
+cudaError_t log_probs_launch(const TokenState &t, int32_t rows, const void *const *ins, void *const *outs, cudaStream_t stream);
+cudaError_t token_fc_launch(const TokenState &t, int32_t rows, const void *const *ins, void *const *outs, cudaStream_t stream);
+
+#ifdef __CUDACC__
+namespace {
+
+__device__ __forceinline__ float to_float(float v) { return v; }
+__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+
+// Rounded once, to nearest even.
+template <typename T> __device__ __forceinline__ T from_float(float v);
+template <> __device__ __forceinline__ float from_float<float>(float v) { return v; }
+template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// Scale of a quantised row and what its values are multiplied with, from the bits of the largest magnitude.  Magnitudes compare as
+// integers, with infinities above all numbers and NaN above those: a maximum over the bits does not lose a NaN as fmaxf does.
+struct RowScale {
+    float scale, inv;
+};
+__device__ __forceinline__ RowScale row_scale(uint32_t largest_bits) {
+    const float largest = __uint_as_float(largest_bits);
+    RowScale r;
+    if (largest_bits >= 0x7f800000u) {               // a NaN or an infinity in the row
+        r.scale = __uint_as_float(0x7fffffffu);
+        r.inv = 0.f;
+    } else if (largest_bits < 0x0d800000u) {         // 2^-100: 127 / largest would overflow further down
+        r.scale = 0.f;
+        r.inv = 0.f;
+    } else {
+        r.scale = __fdiv_rn(largest, 127.f);
+        r.inv = __fdiv_rn(127.f, largest);
+    }
+    return r;
+}
+// Both factors are at most a rounding off, so |v * inv| <= 127 (1 + 2^-23) and rounds to 127 at most.
+__device__ __forceinline__ int32_t quantise(float v, float inv) {
+    return inv == 0.f ? 0 : __float2int_rn(__fmul_rn(v, inv));      // 0 and not NaN or infinity times 0
+}
+__device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+
+}  // namespace
+#endif
+
+}  // namespace enn_b200

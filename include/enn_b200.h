@@ -39,6 +39,8 @@ enum { ENN_B200_ACT_NONE = 0, ENN_B200_ACT_RELU = 1, ENN_B200_ACT_RELU1 = 2, ENN
 
 /* Element types of activations / weights (PrecisionType::UINT8 / INT8, Common.hpp:96-104). */
 enum { ENN_B200_U8 = 0, ENN_B200_S8 = 1 };
+/* Floating element types: the token operators take them, the others refuse them. */
+enum { ENN_B200_F32 = 16, ENN_B200_F16 = 17, ENN_B200_BF16 = 18 };
 
 /* Weight memory layouts accepted at prepare time (they are re-packed once on the device):
  *   OIHW  [Cout][Cin/g][Kh][Kw]   reference NCHW models (CLConvolution.cpp:97-98)
@@ -161,6 +163,74 @@ typedef struct enn_b200_resize_desc {
     int32_t act_dtype;
 } enn_b200_resize_desc;
 
+/* ---- token operators: what runs around an 8-bit product whose activations are quantised row by row at run time, as in
+ *      the blocks of a language model served in 8-bit integers.  No counterpart in the reference.  A row is a token; an
+ *      operator is prepared once for up to `m` rows and enn_b200_op_execute_rows runs it on 0 .. m of them (1 for a decode
+ *      step, more for a prompt).  Rows past the given number are neither read nor written.
+ *
+ * Quantised rows ("byte rows"): row t is c int8 values q[t][i] in [-127, 127], enn_b200_token_pitch(c) bytes from row to
+ * row, and a float scale s[t]; they stand for q * s.  Rows are quantised as s = max_i |y_i| / 127,
+ * q_i = round(y_i * (127 / max_i |y_i|)), halves to even.  A row whose largest magnitude is below 2^-100 has s = 0 and
+ * q = 0; a row that holds a NaN or an infinity has s = NaN and q = 0, so that what is computed from it is NaN.  The bytes
+ * between c and the pitch are zero.
+ *
+ * token_fc: out[t][n] = (float(sum_k q[t][k] w[n][k]) * s[t]) * channel_scale[n] + bias[n], the sum exact in 32-bit
+ * integers, the rest in float, rounded once to out_dtype.  Inputs {q, s}, output {out [m][n]}. */
+typedef struct enn_b200_token_fc_desc {
+    int32_t m, k, n;                /* n <= 2^21; k < 131072: the largest sum of products that fits 32 bits */
+    int32_t out_dtype;              /* ENN_B200_F32 | F16 | BF16 */
+    int64_t in_pitch;               /* bytes from row to row of q; 0: enn_b200_token_pitch(k).  Multiples of 16 are fast */
+} enn_b200_token_fc_desc;
+
+/* token_norm: around a block of the residual stream.  With x the block's output, r the stream:
+ *   b = post(x) * gate * residual_scale;  h = r + b;  y = norm(h)
+ * post and norm are NORM_NONE (identity), NORM_RMS x / sqrt(mean x^2 + eps) * weight + bias, or
+ * NORM_LAYER (x - mean) / sqrt(mean (x - mean)^2 + eps) * weight + bias; a weight or bias that is not given is 1 or 0.
+ * residual == 0: h = b and it is not written.  gate_tokens > 0: rows t with the same t / gate_tokens share row
+ * t / gate_tokens of the gate tensor (1: a row of gates per token).  Computed in float; y is taken from h before h is
+ * rounded to io_dtype.  out_dtype ENN_B200_S8: y leaves as byte rows.
+ * Inputs {x, r if residual, gate if gate_tokens} [m][c], outputs {h if residual, y, s if out_dtype is S8}; h may be r's
+ * memory, every other output is memory of its own. */
+enum { ENN_B200_NORM_NONE = 0, ENN_B200_NORM_RMS = 1, ENN_B200_NORM_LAYER = 2 };
+typedef struct enn_b200_token_norm_desc {
+    int32_t m, c;                   /* c <= 32768 */
+    int32_t norm, post_norm;        /* ENN_B200_NORM_* */
+    int32_t residual;
+    int32_t gate_tokens;
+    int32_t io_dtype;               /* type of x, r, gate and h: ENN_B200_F32 | F16 | BF16 */
+    int32_t out_dtype;              /* type of y: those or ENN_B200_S8 */
+    float eps, post_eps;            /* >= 0 */
+    float residual_scale;           /* finite */
+} enn_b200_token_norm_desc;
+
+/* token_gate: y = act(g) * u, in float.  SILU g / (1 + e^-g), GELU g * Phi(g), GELU_TANH its tanh form
+ * g / 2 * (1 + tanh(sqrt(2 / pi) (g + 0.044715 g^3))), RELU, SIGMOID.  packed != 0: one input [m][2 c], gates first; else two
+ * inputs {g, u} [m][c].  Outputs {y, s if out_dtype is S8}, memory of their own. */
+enum { ENN_B200_GATE_SILU = 0, ENN_B200_GATE_GELU = 1, ENN_B200_GATE_GELU_TANH = 2, ENN_B200_GATE_RELU = 3, ENN_B200_GATE_SIGMOID = 4 };
+typedef struct enn_b200_token_gate_desc {
+    int32_t m, c;                   /* c <= 65536 */
+    int32_t act, packed;
+    int32_t in_dtype, out_dtype;    /* as token_norm's io_dtype, out_dtype */
+} enn_b200_token_gate_desc;
+
+/* log_probs: for rows of logits l[vocab], z = scale * l, p = softmax(z):
+ *   given[t][j] = log p[ids[t][j]]  (a negative id gives 0, one past the vocabulary NaN)
+ *   entropy[t]  = - sum_i p_i log p_i, where p_i = 0 adds nothing
+ *   top_ids[t], top[t]: the `top` largest logits in descending order, the lower index first among equals, and their log p.
+ * -inf rules a logit out.  A row that is ruled out as a whole, or holds +inf or a NaN, has no distribution: NaN in place of
+ * its numbers; top_ids are then still in order, NaN above all.
+ * Inputs {logits [m][vocab], int32 ids [m][given] if given}, outputs {given if given, entropy, int32 top_ids and top if top};
+ * results are float. */
+#define ENN_B200_LOG_PROBS_MAX_TOP 32
+typedef struct enn_b200_log_probs_desc {
+    int32_t m, vocab;               /* vocab <= 2^24 */
+    int32_t in_dtype;               /* ENN_B200_F32 | F16 | BF16 */
+    int32_t given;                  /* ids per row, 0 .. 1024 */
+    int32_t top;                    /* alternatives per row, 0 .. min(vocab, ENN_B200_LOG_PROBS_MAX_TOP) */
+    float scale;                    /* 1 / temperature, > 0 */
+    int64_t in_pitch;               /* logits from row to row; 0: vocab */
+} enn_b200_log_probs_desc;
+
 /* Derived per-op facts, for callers that size buffers or report work. */
 typedef struct enn_b200_op_info_t {
     int32_t impl;                   /* ENN_B200_IMPL_* */
@@ -248,6 +318,24 @@ int32_t enn_b200_softmax_prepare(enn_b200_context *ctx, const enn_b200_softmax_d
 /* CLResizeBilinear::initialize (CLResizeBilinear.cpp:120-218). */
 int32_t enn_b200_resize_bilinear_prepare(enn_b200_context *ctx, const enn_b200_resize_desc *desc, enn_b200_op **op);
 
+/* Token operators (descriptors above).  Constant vectors and weights may be host or device memory; device memory must be
+ * complete, it is read on the context's stream before the call returns.  None of them is retained.
+ * weights [n][k] int8, channel_scales[n], bias[n] float or NULL. */
+int32_t enn_b200_token_fc_prepare(enn_b200_context *ctx, const enn_b200_token_fc_desc *desc, const int8_t *weights,
+                                  const float *channel_scales, const float *bias, enn_b200_op **op);
+/* weight, bias of `norm`, post_weight, post_bias of `post_norm`: float [c] each, or NULL. */
+int32_t enn_b200_token_norm_prepare(enn_b200_context *ctx, const enn_b200_token_norm_desc *desc, const float *weight, const float *bias,
+                                    const float *post_weight, const float *post_bias, enn_b200_op **op);
+int32_t enn_b200_token_gate_prepare(enn_b200_context *ctx, const enn_b200_token_gate_desc *desc, enn_b200_op **op);
+int32_t enn_b200_log_probs_prepare(enn_b200_context *ctx, const enn_b200_log_probs_desc *desc, enn_b200_op **op);
+/* Bytes from row to row of byte rows of c channels: c rounded up to 16. */
+int64_t enn_b200_token_pitch(int32_t c);
+/* Runs a token operator on the first `rows` (0 .. m) rows of its inputs: enqueues on the context's stream, whatever device
+ * is current, and can be captured.  The inputs and outputs the descriptor asks for, in its order, aligned to their element
+ * type (byte rows: q and out of token_fc are fast at 16-byte addresses; outputs of 16-byte alignment are written fastest). */
+int32_t enn_b200_op_execute_rows(enn_b200_op *op, int32_t rows, const void *const *ins_dev, int32_t n_in, void *const *outs_dev,
+                                 int32_t n_out);
+
 /* Force the kernel family of a prepared conv / fc / deconv handle (ENN_B200_IMPL_DIRECT or
  * ENN_B200_IMPL_TCGEN05 ...); INVALID_PARAMS if that family cannot run the geometry.  For tests and benches. */
 int32_t enn_b200_op_set_impl(enn_b200_op *op, int32_t impl);
@@ -304,6 +392,9 @@ int32_t enn_b200_oplist_create(enn_b200_context *ctx, enn_b200_oplist **list);
 int32_t enn_b200_oplist_add_tensor(enn_b200_oplist *list, int64_t bytes, int32_t *tensor_id);
 /* Appends a prepared operator reading tensors in_ids[0..n_in) and writing out_id; the list owns the op from here on. */
 int32_t enn_b200_oplist_add_op(enn_b200_oplist *list, enn_b200_op *op, const int32_t *in_ids, int32_t n_in, int32_t out_id);
+/* The same for operators with several outputs (the token operators, which run on all their m rows in a list). */
+int32_t enn_b200_oplist_add_op_n(enn_b200_oplist *list, enn_b200_op *op, const int32_t *in_ids, int32_t n_in, const int32_t *out_ids,
+                                 int32_t n_out);
 int32_t enn_b200_oplist_set_io(enn_b200_oplist *list, const int32_t *input_ids, int32_t n_inputs, const int32_t *output_ids,
                                int32_t n_outputs);
 /* assignBuffers (gpu_op_constructor.cc:1839-1843, CLRuntime.cpp:34-157): liveness-based device buffer assignment,
@@ -330,7 +421,7 @@ int32_t enn_b200_oplist_execute_device(enn_b200_oplist *list);
 int32_t enn_b200_oplist_tensor_ptr(enn_b200_oplist *list, int32_t tensor_id, void **dev_ptr);
 /* The list's nodes after finalize (a fused CONV_2D -> ADD pair is one node): count, and per node the operator's info,
  * its kind (0 conv, 1 depthwise, 2 deconvolution, 3 fully connected, 4 add, 5 average pool, 6 max pool, 7 mean,
- * 8 concat, 9 softmax, 10 resize) and its number of inputs. */
+ * 8 concat, 9 softmax, 10 resize, 11 token_fc, 12 token_norm, 13 token_gate, 14 log_probs) and its number of inputs. */
 int32_t enn_b200_oplist_node_count(const enn_b200_oplist *list, int32_t *n_nodes);
 int32_t enn_b200_oplist_node_info(const enn_b200_oplist *list, int32_t index, enn_b200_op_info_t *info, int32_t *kind, int32_t *n_inputs);
 /* Per-operator device time in microseconds (average over `repeats` eager passes over the list's own tensors, one
