@@ -7,6 +7,7 @@
 #include "internal.h"
 #include "quant_host.h"
 #include "requant.h"
+#include "token_ops.h"
 
 using namespace enn_b200;
 
@@ -695,6 +696,10 @@ int32_t enn_b200_op_set_impl(enn_b200_op *op, int32_t impl) {
         op->info.impl = op->impl;
         return ENN_B200_SUCCESS;
     }
+    if (op->kind == OP_TOKEN_FC && (impl == ENN_B200_IMPL_DIRECT || (impl == ENN_B200_IMPL_TCGEN05 && op->token->fc.err_dev))) {
+        op->impl = op->info.impl = impl;
+        return ENN_B200_SUCCESS;
+    }
     if (op->kind == OP_DEPTHWISE && (impl == ENN_B200_IMPL_DIRECT || impl == ENN_B200_IMPL_DEPTHWISE)) {
         // DIRECT selects the general kernel, DEPTHWISE the 3x3 fast path when the geometry has one.
         op->impl = impl;
@@ -799,6 +804,10 @@ int32_t enn_b200_op_info(const enn_b200_op *op, enn_b200_op_info_t *info) {
 
 int32_t enn_b200_op_test_starve_next(enn_b200_op *op) {
     if (!op) return ENN_B200_INVALID_PARAMS;
+    if (op->kind == OP_TOKEN_FC && op->impl == ENN_B200_IMPL_TCGEN05) {
+        op->token->fc.starve_next = true;
+        return ENN_B200_SUCCESS;
+    }
     if (op->impl != ENN_B200_IMPL_TCGEN05 || !op->tc) return fail(op->ctx, ENN_B200_INVALID_PARAMS, "the self-test needs an operator on the tensor-core kernel");
     return tc_test_starve_next(op) == ENN_B200_SUCCESS ? ENN_B200_SUCCESS
                                                        : fail(op->ctx, ENN_B200_INVALID_PARAMS, "this plan has no starved form (GEMV, first layer or CTA pairs)");
@@ -807,6 +816,7 @@ int32_t enn_b200_op_test_starve_next(enn_b200_op *op) {
 int32_t enn_b200_op_clear_error(enn_b200_op *op) {
     if (!op) return ENN_B200_INVALID_PARAMS;
     if (op->tc) tc_clear_error(op);
+    if (op->token && op->token->fc.err_host) *op->token->fc.err_host = 0;
     if (op->dw_ring) dw_ring_clear_error(op);
     return ENN_B200_SUCCESS;
 }

@@ -85,7 +85,9 @@ int32_t cfail(enn_b200_context *ctx, cudaError_t e) {
 }  // namespace
 
 namespace enn_b200 {
+bool tc_available(const enn_b200_context *ctx);      // gemm_tc.cu
 void token_release(enn_b200_op *op) {
+    if (op->token->fc.err_host) cudaFreeHost(op->token->fc.err_host);
     delete op->token;
     op->token = nullptr;
 }
@@ -117,7 +119,8 @@ int32_t enn_b200_token_fc_prepare(enn_b200_context *ctx, const enn_b200_token_fc
     if (e == cudaSuccess) e = b.vector(channel_scales, d->n, &t.fc.channel_scale);
     if (e == cudaSuccess) e = b.vector(bias, d->n, &t.fc.bias);
     if (e != cudaSuccess) return cfail(ctx, e);
-    b.op->impl = b.op->info.impl = ENN_B200_IMPL_DIRECT;
+    if (tc_available(ctx) && (e = token_fc_plan(b.op)) != cudaSuccess) return cfail(ctx, e);
+    b.op->impl = b.op->info.impl = t.fc.err_dev ? ENN_B200_IMPL_TCGEN05 : ENN_B200_IMPL_DIRECT;
     b.op->info.macs = static_cast<int64_t>(d->m) * d->k * d->n;
     b.op->info.algorithmic_bytes += static_cast<int64_t>(d->n) * d->k;
     b.op->info.out_c = d->n;
@@ -196,11 +199,12 @@ int32_t enn_b200_op_execute_rows(enn_b200_op *op, int32_t rows, const void *cons
     if (!dev.ok()) return tfail(ctx, ENN_B200_CUDA_FAILURE, "the context's device cannot be selected");
     cudaError_t e = cudaErrorInvalidValue;
     switch (op->kind) {
-        case OP_TOKEN_FC: e = token_fc_launch(t, rows, ins, outs, ctx->stream); break;
+        case OP_TOKEN_FC: e = token_fc_launch(op, rows, ins, outs); break;
         case OP_TOKEN_NORM: e = token_norm_launch(t, rows, ins, outs, ctx->stream); break;
         case OP_TOKEN_GATE: e = token_gate_launch(t, rows, ins, outs, ctx->stream); break;
         case OP_LOG_PROBS: e = log_probs_launch(t, rows, ins, outs, ctx->stream); break;
     }
+    if (e == cudaErrorLaunchFailure && t.fc.err_host && *t.fc.err_host) return tfail(ctx, ENN_B200_CUDA_FAILURE, "token_fc: the kernel gave up on a barrier wait earlier");
     return e == cudaSuccess ? ENN_B200_SUCCESS : cfail(ctx, e);
 }
 

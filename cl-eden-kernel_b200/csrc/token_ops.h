@@ -1,5 +1,6 @@
 // State and device helpers of the token operators (token_fc, token_norm, token_gate, log_probs).
 #pragma once
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -29,12 +30,21 @@ struct LogProbsParams {
     int64_t pitch;          // logits from row to row
 };
 
+struct TokenFcDirect {      // what the general kernel takes
+    int32_t k, n;
+    int64_t in_pitch, w_pitch;
+    const int8_t *w;
+    const float *channel_scale, *bias;
+};
 struct TokenFcParams {
     int32_t k, n;
-    int64_t in_pitch;
-    int64_t w_pitch;
+    int64_t in_pitch, w_pitch;
     const int8_t *w;        // [n][w_pitch], zero beyond k
     const float *channel_scale, *bias;
+    CUtensorMap map_w;
+    int32_t *err_host, *err_dev;      // pinned word in which a kernel that gave up on a wait leaves a code
+    bool starve_next;                 // the next call is a self-test of that
+    TokenFcDirect direct() const { return {k, n, in_pitch, w_pitch, w, channel_scale, bias}; }
 };
 
 // Everything a prepared token operator holds; deleted by the operator's release.
@@ -52,7 +62,8 @@ struct TokenState {
 cudaError_t token_norm_launch(const TokenState &t, int32_t rows, const void *const *ins, void *const *outs, cudaStream_t stream);
 cudaError_t token_gate_launch(const TokenState &t, int32_t rows, const void *const *ins, void *const *outs, cudaStream_t stream);
 cudaError_t log_probs_launch(const TokenState &t, int32_t rows, const void *const *ins, void *const *outs, cudaStream_t stream);
-cudaError_t token_fc_launch(const TokenState &t, int32_t rows, const void *const *ins, void *const *outs, cudaStream_t stream);
+cudaError_t token_fc_launch(enn_b200_op *op, int32_t rows, const void *const *ins, void *const *outs);
+cudaError_t token_fc_plan(enn_b200_op *op);
 
 #ifdef __CUDACC__
 namespace {

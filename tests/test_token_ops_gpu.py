@@ -174,6 +174,24 @@ def test_token_fc_implementations_agree(enn, ctx):
         op.release()
 
 
+def test_token_fc_that_gives_up_on_a_wait(enn, ctx):
+    """A kernel whose wait ran out leaves a code; later calls fail until it is cleared, and then run as before."""
+    for m in (3, 300):
+        q, w, s, sw, _ = fc_inputs(14, m, 4096, 256)
+        op = enn.token_fc(ctx, enn.TokenFcDesc(m=m, k=4096, n=256, out_dtype=enn.F32), w.data_ptr(), sw.data_ptr())
+        assert op.info.impl == enn.IMPL_TCGEN05
+        y = guarded(m, 256, torch.float32)
+        op.test_starve_next()
+        execute(op, m, [q, s], [y])
+        with pytest.raises(enn.EnnError) as e:
+            execute(op, m, [q, s], [y])
+        assert e.value.status == enn.CUDA_FAILURE and "gave up" in str(e.value)
+        op.clear_error()
+        execute(op, m, [q, s], [y])
+        fc_check(y[:m], q, w, s, sw, None, "f32", 4096)
+        op.release()
+
+
 # ---- token_norm -------------------------------------------------------------------------------------------------------
 
 def norm64(x, kind, eps, weight, bias):
