@@ -84,7 +84,9 @@ cudaError_t launch_typed(const TokenState &t, int32_t rows, const void *const *i
 
 }  // namespace
 
-cudaError_t log_probs_launch(const TokenState &t, int32_t rows, const void *const *ins, void *const *outs, cudaStream_t stream) {
+cudaError_t log_probs_launch(const enn_b200_op *op, int32_t rows, const void *const *ins, void *const *outs) {
+    const TokenState &t = *op->token;
+    const cudaStream_t stream = op->ctx->stream;
     switch (t.in_dtype) {
         case ENN_B200_F32: return launch_typed<float>(t, rows, ins, outs, stream);
         case ENN_B200_F16: return launch_typed<__half>(t, rows, ins, outs, stream);

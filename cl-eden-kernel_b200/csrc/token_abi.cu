@@ -200,9 +200,9 @@ int32_t enn_b200_op_execute_rows(enn_b200_op *op, int32_t rows, const void *cons
     cudaError_t e = cudaErrorInvalidValue;
     switch (op->kind) {
         case OP_TOKEN_FC: e = token_fc_launch(op, rows, ins, outs); break;
-        case OP_TOKEN_NORM: e = token_norm_launch(t, rows, ins, outs, ctx->stream); break;
-        case OP_TOKEN_GATE: e = token_gate_launch(t, rows, ins, outs, ctx->stream); break;
-        case OP_LOG_PROBS: e = log_probs_launch(t, rows, ins, outs, ctx->stream); break;
+        case OP_TOKEN_NORM: e = token_norm_launch(op, rows, ins, outs); break;
+        case OP_TOKEN_GATE: e = token_gate_launch(op, rows, ins, outs); break;
+        case OP_LOG_PROBS: e = log_probs_launch(op, rows, ins, outs); break;
     }
     if (e == cudaErrorLaunchFailure && t.fc.err_host && *t.fc.err_host) return tfail(ctx, ENN_B200_CUDA_FAILURE, "token_fc: the kernel gave up on a barrier wait earlier");
     return e == cudaSuccess ? ENN_B200_SUCCESS : cfail(ctx, e);

@@ -58,10 +58,10 @@ struct TokenState {
     TokenFcParams fc{};
 };
 
-// One launch sequence for `rows` > 0 rows on `stream`; pointers in the descriptor's order.
-cudaError_t token_norm_launch(const TokenState &t, int32_t rows, const void *const *ins, void *const *outs, cudaStream_t stream);
-cudaError_t token_gate_launch(const TokenState &t, int32_t rows, const void *const *ins, void *const *outs, cudaStream_t stream);
-cudaError_t log_probs_launch(const TokenState &t, int32_t rows, const void *const *ins, void *const *outs, cudaStream_t stream);
+// The launch for `rows` > 0 rows on the context's stream; pointers in the descriptor's order.
+cudaError_t token_norm_launch(const enn_b200_op *op, int32_t rows, const void *const *ins, void *const *outs);
+cudaError_t token_gate_launch(const enn_b200_op *op, int32_t rows, const void *const *ins, void *const *outs);
+cudaError_t log_probs_launch(const enn_b200_op *op, int32_t rows, const void *const *ins, void *const *outs);
 cudaError_t token_fc_launch(enn_b200_op *op, int32_t rows, const void *const *ins, void *const *outs);
 cudaError_t token_fc_plan(enn_b200_op *op);
 
@@ -98,10 +98,9 @@ __device__ __forceinline__ RowScale row_scale(uint32_t largest_bits) {
     }
     return r;
 }
-// Both factors are at most a rounding off, so |v * inv| <= 127 (1 + 2^-23) and rounds to 127 at most.
-__device__ __forceinline__ int32_t quantise(float v, float inv) {
-    return inv == 0.f ? 0 : __float2int_rn(__fmul_rn(v, inv));      // 0 and not NaN or infinity times 0
-}
+// The factors are a few roundings off, so |v * inv| <= 127 (1 + 2^-21) and rounds to 127 at most; where inv is 0 the product is 0 or NaN, and
+// the conversion turns NaN into 0.
+__device__ __forceinline__ int32_t quantise(float v, float inv) { return __float2int_rn(__fmul_rn(v, inv)); }
 __device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 
 }  // namespace

@@ -1,163 +1,478 @@
 // token_norm and token_gate: row-wise operators around the 8-bit products of a block.
+//
+// Both are bound by memory: a row is read once, stays in registers as floats while its statistics are reduced, and is written once.
+// A row belongs to a warp (up to 1024 channels), a CTA, or for quantised gates a cluster; a thread holds up to four groups of eight
+// neighbouring channels, 16 bytes of a 16-bit type.  Constant vectors come from L1, which they share with nothing: the rows are loaded
+// and stored past it.
+#include "tc_common.cuh"
 #include "token_ops.h"
 
 namespace enn_b200 {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kGroup = 8;           // channels a thread handles together
+constexpr int kMaxThreads = 1024;
 
-template <typename F>
-__device__ __forceinline__ float block_reduce(float v, float *scratch, F join) {
-    for (int o = 16; o > 0; o >>= 1) v = join(v, __shfl_xor_sync(0xffffffffu, v, o));
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = scratch[threadIdx.x & (kThreads / 32 - 1)];
-    for (int o = kThreads / 64; o > 0; o >>= 1) v = join(v, __shfl_xor_sync(0xffffffffu, v, o));
+__device__ __forceinline__ uint4 ld_stream(const void *p) {
+    uint4 v;
+    asm volatile("ld.global.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
     return v;
 }
-__device__ __forceinline__ float block_sum(float v, float *scratch) {
-    return block_reduce(v, scratch, [](float a, float b) { return a + b; });
+// Eight channels as they lie in memory.
+template <typename T> struct Raw { uint4 v[sizeof(T) / 2]; };
+template <typename T> __device__ __forceinline__ Raw<T> ld8(const T *p) {
+    Raw<T> r;
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) r.v[i] = ld_stream(reinterpret_cast<const uint4 *>(p) + i);
+    return r;
 }
-__device__ __forceinline__ uint32_t block_max_bits(uint32_t v, float *scratch) {
-    return __float_as_uint(block_reduce(__uint_as_float(v), scratch, [](float a, float b) { return __uint_as_float(max(__float_as_uint(a), __float_as_uint(b))); }));
-}
-
-// row[0..c) = norm(row)
-__device__ void norm_row(float *row, int c, int kind, float eps, const float *weight, const float *bias, float *scratch) {
-    if (kind == ENN_B200_NORM_NONE) return;
-    float mean = 0.f;
-    if (kind == ENN_B200_NORM_LAYER) {
-        float s = 0.f;
-        for (int i = threadIdx.x; i < c; i += kThreads) s += row[i];
-        mean = block_sum(s, scratch) / static_cast<float>(c);
+__device__ __forceinline__ void widen(const Raw<float> &r, float (&f)[8]) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        f[4 * i] = __uint_as_float(r.v[i].x); f[4 * i + 1] = __uint_as_float(r.v[i].y);
+        f[4 * i + 2] = __uint_as_float(r.v[i].z); f[4 * i + 3] = __uint_as_float(r.v[i].w);
     }
-    float s = 0.f;
-    for (int i = threadIdx.x; i < c; i += kThreads) s += (row[i] - mean) * (row[i] - mean);
-    const float r = rsqrtf(block_sum(s, scratch) / static_cast<float>(c) + eps);
-    for (int i = threadIdx.x; i < c; i += kThreads) row[i] = (row[i] - mean) * r * (weight ? weight[i] : 1.f) + (bias ? bias[i] : 0.f);
+}
+__device__ __forceinline__ float2 widen2(uint32_t w, __half) { return __half22float2(*reinterpret_cast<const __half2 *>(&w)); }
+__device__ __forceinline__ float2 widen2(uint32_t w, __nv_bfloat16) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
+template <typename T> __device__ __forceinline__ void widen(const Raw<T> &r, float (&f)[8]) {
+    const uint32_t w[4] = {r.v[0].x, r.v[0].y, r.v[0].z, r.v[0].w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 p = widen2(w[i], T{});
+        f[2 * i] = p.x;
+        f[2 * i + 1] = p.y;
+    }
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b, __half) {
+    const __half2 p = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&p);
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b, __nv_bfloat16) {
+    const __nv_bfloat162 p = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&p);
+}
+__device__ __forceinline__ void st8(float *p, const float (&f)[8]) {
+    __stcs(reinterpret_cast<float4 *>(p), make_float4(f[0], f[1], f[2], f[3]));
+    __stcs(reinterpret_cast<float4 *>(p) + 1, make_float4(f[4], f[5], f[6], f[7]));
+}
+template <typename T> __device__ __forceinline__ void st8(T *p, const float (&f)[8]) {
+    __stcs(reinterpret_cast<uint4 *>(p), make_uint4(pack2(f[0], f[1], T{}), pack2(f[2], f[3], T{}), pack2(f[4], f[5], T{}), pack2(f[6], f[7], T{})));
+}
+__device__ __forceinline__ uint32_t pack4_s8(const float *f, float inv) {
+    uint32_t hi, d;
+    asm("cvt.pack.sat.s8.s32.b32 %0, %1, %2, 0;" : "=r"(hi) : "r"(quantise(f[3], inv)), "r"(quantise(f[2], inv)));
+    asm("cvt.pack.sat.s8.s32.b32 %0, %1, %2, %3;" : "=r"(d) : "r"(quantise(f[1], inv)), "r"(quantise(f[0], inv)), "r"(hi));
+    return d;
 }
 
-template <typename T, typename O>
-__global__ void __launch_bounds__(kThreads) token_norm_kernel(NormParams p, const T *x, const T *residual, const T *gate, T *stream, O *y, float *scale) {
-    extern __shared__ float row[];
-    __shared__ float scratch[kThreads / 32];
+// The part of a row that a group of `nt` threads holds: channels [0, n) of a segment, NV groups per thread.  VEC: neighbouring channels
+// in 16-byte pieces (n, every address and every pitch allow it); else one channel at a time, neighbouring threads on neighbouring
+// channels, for rows that begin anywhere.
+template <int NV, bool VEC>
+struct Row {
+    int n, tid, nt;
+    __device__ __forceinline__ int at(int v, int j) const { return VEC ? (v * nt + tid) * kGroup + j : (v * kGroup + j) * nt + tid; }
+
+    template <typename T> __device__ __forceinline__ void load(const T *p, Raw<T> (&raw)[NV]) const {
+        if constexpr (VEC) {
+#pragma unroll
+            for (int v = 0; v < NV; ++v) {
+                raw[v] = Raw<T>{};
+                if (at(v, 0) < n) raw[v] = ld8(p + at(v, 0));
+            }
+        } else {
+#pragma unroll
+            for (int v = 0; v < NV; ++v) {
+                T e[kGroup];
+#pragma unroll
+                for (int j = 0; j < kGroup; ++j) e[j] = at(v, j) < n ? p[at(v, j)] : from_float<T>(0.f);
+                __builtin_memcpy(&raw[v], e, sizeof(e));
+            }
+        }
+    }
+    // A constant vector, or `absent` where there is none.
+    __device__ __forceinline__ void constant(const float *p, int v, float absent, float (&f)[8]) const {
+#pragma unroll
+        for (int j = 0; j < kGroup; ++j) f[j] = absent;
+        if (!p) return;
+        if constexpr (VEC) {
+            if (at(v, 0) < n) {
+                const float4 a = __ldg(reinterpret_cast<const float4 *>(p + at(v, 0))), b = __ldg(reinterpret_cast<const float4 *>(p + at(v, 0)) + 1);
+                f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < kGroup; ++j)
+                if (at(v, j) < n) f[j] = __ldg(p + at(v, j));
+        }
+    }
+    template <typename T> __device__ __forceinline__ void store(T *p, const float (&f)[NV][8]) const {
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            if constexpr (VEC) {
+                if (at(v, 0) < n) st8(p + at(v, 0), f[v]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < kGroup; ++j)
+                    if (at(v, j) < n) p[at(v, j)] = from_float<T>(f[v][j]);
+            }
+        }
+    }
+    __device__ __forceinline__ void store_bytes(int8_t *p, const float (&f)[NV][8], float inv) const {
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            if constexpr (VEC) {
+                if (at(v, 0) < n) *reinterpret_cast<uint2 *>(p + at(v, 0)) = make_uint2(pack4_s8(f[v], inv), pack4_s8(f[v] + 4, inv));
+            } else {
+#pragma unroll
+                for (int j = 0; j < kGroup; ++j)
+                    if (at(v, j) < n) p[at(v, j)] = static_cast<int8_t>(quantise(f[v][j], inv));
+            }
+        }
+    }
+    __device__ __forceinline__ void store_as(int dtype, void *out, int64_t offset, const float (&f)[NV][8]) const {
+        if (dtype == ENN_B200_BF16) store(static_cast<__nv_bfloat16 *>(out) + offset, f);
+        else if (dtype == ENN_B200_F16) store(static_cast<__half *>(out) + offset, f);
+        else store(static_cast<float *>(out) + offset, f);
+    }
+};
+
+// Sum and maximum over the threads of a row: a warp, or the whole block.  Two sets of scratch words in turn, so that one barrier per
+// reduction is enough.
+struct Reduce {
+    float2 (*scratch)[32];
+    int nt, turn;
+    __device__ __forceinline__ void operator()(float &sum, uint32_t &largest) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        largest = __reduce_max_sync(0xffffffffu, largest);
+        if (nt == 32) return;
+        const int lane = threadIdx.x & 31, warps = nt >> 5;
+        if (lane == 0) scratch[turn][threadIdx.x >> 5] = make_float2(sum, __uint_as_float(largest));
+        __syncthreads();
+        const float2 v = lane < warps ? scratch[turn][lane] : make_float2(0.f, 0.f);
+        sum = v.x;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        largest = __reduce_max_sync(0xffffffffu, __float_as_uint(v.y));
+        turn ^= 1;
+    }
+    __device__ __forceinline__ float sum(float s) {
+        uint32_t m = 0;
+        (*this)(s, m);
+        return s;
+    }
+    __device__ __forceinline__ uint32_t largest(uint32_t m) {
+        float s = 0.f;
+        (*this)(s, m);
+        return m;
+    }
+};
+
+// f = norm(f).  With `largest` the bits of the largest magnitude of the result come back too; for an RMS norm without a bias they ride on
+// the sum of squares, since max |f r w| = r max |f w|.
+template <int NV, bool VEC>
+__device__ __forceinline__ void norm_row(const Row<NV, VEC> &row, float (&f)[NV][8], int c, int kind, float eps, const float *weight, const float *bias, Reduce &reduce,
+                                         uint32_t *largest) {
+    if (kind != ENN_B200_NORM_NONE) {
+        const float over = 1.f / static_cast<float>(c);
+        const bool joint = largest && kind == ENN_B200_NORM_RMS && !bias;
+        if (kind == ENN_B200_NORM_LAYER) {
+            float s = 0.f;
+#pragma unroll
+            for (int v = 0; v < NV; ++v)
+#pragma unroll
+                for (int j = 0; j < kGroup; ++j) s += f[v][j];
+            const float mean = reduce.sum(s) * over;
+#pragma unroll
+            for (int v = 0; v < NV; ++v)
+#pragma unroll
+                for (int j = 0; j < kGroup; ++j) f[v][j] = row.at(v, j) < row.n ? f[v][j] - mean : 0.f;
+        }
+        float s = 0.f;
+        uint32_t m = 0;
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            float w[8];
+            if (joint) row.constant(weight, v, 1.f, w);
+#pragma unroll
+            for (int j = 0; j < kGroup; ++j) {
+                s = fmaf(f[v][j], f[v][j], s);
+                if (joint) {
+                    f[v][j] *= w[j];
+                    m = max(m, magnitude(f[v][j]));
+                }
+            }
+        }
+        reduce(s, m);
+        const float r = rsqrtf(fmaf(s, over, eps));
+        if (joint) {
+#pragma unroll
+            for (int v = 0; v < NV; ++v)
+#pragma unroll
+                for (int j = 0; j < kGroup; ++j) f[v][j] *= r;
+            *largest = magnitude(__uint_as_float(m) * r);
+            return;
+        }
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            float w[8], b[8];
+            row.constant(weight, v, 1.f, w);
+            row.constant(bias, v, 0.f, b);
+#pragma unroll
+            for (int j = 0; j < kGroup; ++j) f[v][j] = fmaf(f[v][j] * r, w[j], b[j]);
+        }
+    }
+    if (largest) {
+        uint32_t m = 0;
+#pragma unroll
+        for (int v = 0; v < NV; ++v)
+#pragma unroll
+            for (int j = 0; j < kGroup; ++j)
+                if (row.at(v, j) < row.n) m = max(m, magnitude(f[v][j]));
+        *largest = reduce.largest(m);
+    }
+}
+
+template <typename T, int NV, bool VEC>
+__global__ void __launch_bounds__(kMaxThreads) token_norm_kernel(NormParams p, int32_t rows, int32_t out_dtype, const T *x, const T *residual, const T *gate, T *stream,
+                                                                 void *out, float *scale) {
+    __shared__ float2 scratch[2][32];
+    const int64_t t = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
+    Row<NV, VEC> row{p.c, static_cast<int>(threadIdx.x), static_cast<int>(blockDim.x)};
+    Reduce reduce{scratch, row.nt, 0};
     pdl_wait();
     pdl_trigger();
-    const int64_t t = blockIdx.x, at = t * p.c;
-    for (int i = threadIdx.x; i < p.c; i += kThreads) row[i] = to_float(x[at + i]);
-    norm_row(row, p.c, p.post_norm, p.post_eps, p.post_weight, p.post_bias, scratch);
-    for (int i = threadIdx.x; i < p.c; i += kThreads) {
-        float v = row[i];
-        if (gate) v *= to_float(gate[t / p.gate_tokens * p.c + i]);
-        v *= p.residual_scale;
-        if (residual) {
-            v += to_float(residual[at + i]);
-            stream[at + i] = from_float<T>(v);
+    if (t >= rows) return;      // a whole warp, and then the block has no barrier
+    float f[NV][8];
+    {
+        Raw<T> rx[NV], rr[NV];
+        row.load(x + t * p.c, rx);
+        if (residual) row.load(residual + t * p.c, rr);
+#pragma unroll
+        for (int v = 0; v < NV; ++v) widen(rx[v], f[v]);
+        norm_row(row, f, p.c, p.post_norm, p.post_eps, p.post_weight, p.post_bias, reduce, nullptr);
+        if (gate) {
+            Raw<T> rg[NV];
+            row.load(gate + t / p.gate_tokens * p.c, rg);
+#pragma unroll
+            for (int v = 0; v < NV; ++v) {
+                float g[8];
+                widen(rg[v], g);
+#pragma unroll
+                for (int j = 0; j < kGroup; ++j) f[v][j] *= g[j];
+            }
         }
-        row[i] = v;
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            float h[8] = {};
+            if (residual) widen(rr[v], h);
+#pragma unroll
+            for (int j = 0; j < kGroup; ++j) f[v][j] = row.at(v, j) < row.n ? fmaf(f[v][j], p.residual_scale, h[j]) : 0.f;
+        }
     }
-    norm_row(row, p.c, p.norm, p.eps, p.weight, p.bias, scratch);
-    if constexpr (sizeof(O) == 1) {
-        uint32_t largest = 0;
-        for (int i = threadIdx.x; i < p.c; i += kThreads) largest = max(largest, magnitude(row[i]));
-        const RowScale rs = row_scale(block_max_bits(largest, scratch));
-        for (int64_t i = threadIdx.x; i < p.pitch; i += kThreads) y[t * p.pitch + i] = i < p.c ? static_cast<O>(quantise(row[i], rs.inv)) : O(0);
-        if (threadIdx.x == 0) scale[t] = rs.scale;
+    if (residual) row.store(stream + t * p.c, f);
+    if (out_dtype != ENN_B200_S8) {
+        norm_row(row, f, p.c, p.norm, p.eps, p.weight, p.bias, reduce, nullptr);
+        row.store_as(out_dtype, out, t * p.c, f);
     } else {
-        for (int i = threadIdx.x; i < p.c; i += kThreads) y[at + i] = from_float<O>(row[i]);
+        uint32_t largest;
+        norm_row(row, f, p.c, p.norm, p.eps, p.weight, p.bias, reduce, &largest);
+        const RowScale rs = row_scale(largest);
+        int8_t *q = static_cast<int8_t *>(out) + t * p.pitch;
+        row.store_bytes(q, f, rs.inv);
+        for (int64_t i = p.c + row.tid; i < p.pitch; i += row.nt) q[i] = 0;
+        if (row.tid == 0) scale[t] = rs.scale;
     }
 }
 
-// 1 / (1 + e^-g) from an exponential that does not overflow.
+// 1 / (1 + e^-g) from an exponential that does not overflow; 2^x and the reciprocal are a unit or two off in the last place.
 __device__ __forceinline__ float sigmoid(float g) {
-    const float e = expf(-fabsf(g));
-    return (g >= 0.f ? 1.f : e) / (1.f + e);
+    float e, r;
+    asm("ex2.approx.f32 %0, %1;" : "=f"(e) : "f"(fabsf(g) * -1.4426950408889634f));
+    asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
+    return (g >= 0.f ? 1.f : e) * r;
 }
-
 __device__ __forceinline__ float gate_act(float g, int act) {
     switch (act) {
         case ENN_B200_GATE_SILU: return g * sigmoid(g);
         case ENN_B200_GATE_GELU: return 0.5f * g * (1.f + erff(g * 0.70710678118654752f));
-        case ENN_B200_GATE_GELU_TANH: return 0.5f * g * (1.f + tanhf(0.79788456080286536f * (g + 0.044715f * g * g * g)));
+        case ENN_B200_GATE_GELU_TANH: return g * sigmoid(2.f * 0.79788456080286536f * fmaf(0.044715f * g * g, g, g));      // (1 + tanh v) / 2 is the sigmoid of 2 v
         case ENN_B200_GATE_RELU: return g < 0.f ? 0.f : g;
         default: return sigmoid(g);
     }
 }
 
-template <typename T, typename O>
-__global__ void __launch_bounds__(kThreads) token_gate_kernel(GateParams p, const T *gates, const T *values, O *y, float *scale) {
-    __shared__ float scratch[kThreads / 32];
+// f = act(gates) * values of the thread's channels.
+template <typename T, int NV, bool VEC>
+__device__ __forceinline__ void gate_row(const Row<NV, VEC> &row, const T *gates, const T *values, int act, float (&f)[NV][8]) {
+    Raw<T> rg[NV], ru[NV];
+    row.load(gates, rg);
+    row.load(values, ru);
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+        float g[8], u[8];
+        widen(rg[v], g);
+        widen(ru[v], u);
+        switch (act) {      // once per group, not per channel
+#define ENN_ACT(A)                                                                        \
+    case A:                                                                               \
+        _Pragma("unroll") for (int j = 0; j < kGroup; ++j) f[v][j] = gate_act(g[j], A) * u[j]; \
+        break;
+            ENN_ACT(ENN_B200_GATE_SILU)
+            ENN_ACT(ENN_B200_GATE_GELU)
+            ENN_ACT(ENN_B200_GATE_GELU_TANH)
+            ENN_ACT(ENN_B200_GATE_RELU)
+            ENN_ACT(ENN_B200_GATE_SIGMOID)
+#undef ENN_ACT
+        }
+    }
+}
+
+// Row t / segs, segment t % segs of it: `seg` channels.  Floats leave at once.  Bytes need the row's largest magnitude first: the
+// segments of a row are then the CTAs of a cluster, which tell each other theirs.
+template <typename T, int NV, bool VEC>
+__global__ void __launch_bounds__(kMaxThreads) token_gate_kernel(GateParams p, int32_t rows, int32_t segs, int32_t seg, int32_t out_dtype, const T *gates, const T *values,
+                                                                 void *out, float *scale) {
+    __shared__ float2 scratch[2][32];
+    __shared__ uint32_t of_cluster[8];
+    const int64_t item = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y, t = item / segs;
+    const int32_t rank = static_cast<int32_t>(item - t * segs), c0 = rank * seg;
+    Row<NV, VEC> row{min(seg, p.c - c0), static_cast<int>(threadIdx.x), static_cast<int>(blockDim.x)};
+    // Seen by the others of the cluster before they write here: waited for below.
+    const bool clustered = segs > 1 && out_dtype == ENN_B200_S8;
+    if (clustered) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
     pdl_wait();
     pdl_trigger();
-    const int64_t t = blockIdx.x;
-    const T *g = gates + t * p.in_stride, *u = values + t * p.in_stride;
-    auto at = [&](int64_t i) { return gate_act(to_float(g[i]), p.act) * to_float(u[i]); };
-    if constexpr (sizeof(O) == 1) {
-        uint32_t largest = 0;
-        for (int i = threadIdx.x; i < p.c; i += kThreads) largest = max(largest, magnitude(at(i)));
-        const RowScale rs = row_scale(block_max_bits(largest, scratch));
-        for (int64_t i = threadIdx.x; i < p.pitch; i += kThreads) y[t * p.pitch + i] = i < p.c ? static_cast<O>(quantise(at(i), rs.inv)) : O(0);
-        if (threadIdx.x == 0) scale[t] = rs.scale;
-    } else {
-        for (int i = threadIdx.x; i < p.c; i += kThreads) y[t * p.c + i] = from_float<O>(at(i));
+    if (t >= rows) return;      // a whole warp, and then the block has no barrier
+    float f[NV][8];
+    gate_row(row, gates + t * p.in_stride + c0, values + t * p.in_stride + c0, p.act, f);
+    if (out_dtype != ENN_B200_S8) {
+        row.store_as(out_dtype, out, t * p.c + c0, f);
+        return;
+    }
+    uint32_t largest = 0;
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+#pragma unroll
+        for (int j = 0; j < kGroup; ++j)
+            if (row.at(v, j) < row.n) largest = max(largest, magnitude(f[v][j]));
+    Reduce reduce{scratch, row.nt, 0};
+    largest = reduce.largest(largest);
+    if (clustered) {
+        asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+        if (row.tid < segs) asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(mapa_rank(smem_u32(of_cluster + rank), row.tid)), "r"(largest) : "memory");
+        cluster_sync_all();     // the only writes to other CTAs come before it: nobody has to wait for them at the end
+        for (int s = 0; s < segs; ++s) largest = max(largest, of_cluster[s]);
+    }
+    const RowScale rs = row_scale(largest);
+    int8_t *q = static_cast<int8_t *>(out) + t * p.pitch;
+    row.store_bytes(q + c0, f, rs.inv);
+    if (rank == 0) {
+        for (int64_t i = p.c + row.tid; i < p.pitch; i += row.nt) q[i] = 0;
+        if (row.tid == 0) scale[t] = rs.scale;
     }
 }
 
-// f(T{}) with the element type of `dtype`.
+bool aligned(const void *p, size_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
+
+// Threads of a row and groups per thread for `n` channels.  `spread`: as many threads as there are groups (few rows: latency), else
+// two groups each (many rows: twice the bytes in flight per thread, half the threads in a reduction).
+struct Shape {
+    int nt, nv, per_block;
+};
+Shape row_shape(int n, bool vec, bool spread) {
+    const int groups = (n + kGroup - 1) / kGroup;
+    auto threads = [&](int nv) { return ((groups + nv - 1) / nv + 31) / 32 * 32; };
+    Shape s;
+    if (!vec) s.nv = 4;
+    else if (groups <= 32 || (spread && threads(1) <= kMaxThreads)) s.nv = 1;
+    else s.nv = groups <= 64 || (groups > 128 && threads(2) <= kMaxThreads) ? 2 : 4;
+    s.nt = threads(s.nv);
+    s.per_block = s.nt == 32 ? 8 : 1;
+    return s;
+}
+
 template <typename F>
-cudaError_t with_type(int32_t dtype, F f) {
-    switch (dtype) {
-        case ENN_B200_F32: return f(float{});
-        case ENN_B200_F16: return f(__half{});
-        case ENN_B200_BF16: return f(__nv_bfloat16{});
-        case ENN_B200_S8: return f(int8_t{});
-    }
-    return cudaErrorInvalidValue;
+cudaError_t with_shape(int nv, bool vec, F f) {
+    if (!vec) return f(std::integral_constant<int, 4>{}, std::false_type{});
+    if (nv == 1) return f(std::integral_constant<int, 1>{}, std::true_type{});
+    if (nv == 2) return f(std::integral_constant<int, 2>{}, std::true_type{});
+    return f(std::integral_constant<int, 4>{}, std::true_type{});
 }
 
-template <typename T, typename O>
-cudaError_t norm_typed(const TokenState &t, int32_t rows, const void *const *ins, void *const *outs, cudaStream_t stream) {
+template <typename T>
+cudaError_t norm_typed(const enn_b200_op *op, int32_t rows, const void *const *ins, void *const *outs) {
+    const TokenState &t = *op->token;
+    const NormParams &p = t.norm;
     int i = 0, o = 0;
     const T *x = static_cast<const T *>(ins[i++]);
     const T *residual = t.residual ? static_cast<const T *>(ins[i++]) : nullptr;
-    const T *gate = t.norm.gate_tokens ? static_cast<const T *>(ins[i++]) : nullptr;
-    T *h = t.residual ? static_cast<T *>(outs[o++]) : nullptr;
-    O *y = static_cast<O *>(outs[o++]);
-    float *scale = sizeof(O) == 1 ? static_cast<float *>(outs[o++]) : nullptr;
-    const size_t smem = sizeof(float) * static_cast<size_t>(t.norm.c);
-    if (smem > 32 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(token_norm_kernel<T, O>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-        if (e != cudaSuccess) return e;
-    }
-    return launch_pdl(token_norm_kernel<T, O>, dim3(static_cast<unsigned>(rows)), dim3(kThreads), smem, stream, t.norm, x, residual, gate, h, y, scale);
+    const T *gate = p.gate_tokens ? static_cast<const T *>(ins[i++]) : nullptr;
+    T *stream = t.residual ? static_cast<T *>(outs[o++]) : nullptr;
+    void *y = outs[o++];
+    float *scale = t.out_dtype == ENN_B200_S8 ? static_cast<float *>(outs[o++]) : nullptr;
+    const bool vec = p.c % kGroup == 0 && aligned(x, 16) && aligned(residual, 16) && aligned(gate, 16) && aligned(stream, 16) && aligned(y, scale ? 8 : 16);
+    const Shape s = row_shape(p.c, vec, rows <= 2 * op->ctx->sm_count);
+    const dim3 grid(static_cast<unsigned>((static_cast<int64_t>(rows) + s.per_block - 1) / s.per_block)), block(static_cast<unsigned>(s.nt), static_cast<unsigned>(s.per_block));
+    return with_shape(s.nv, vec, [&](auto nv, auto v) {
+        return launch_pdl(token_norm_kernel<T, decltype(nv)::value, decltype(v)::value>, grid, block, 0, op->ctx->stream, p, rows, t.out_dtype, x, residual, gate, stream, y, scale);
+    });
 }
 
-template <typename T, typename O>
-cudaError_t gate_typed(const TokenState &t, int32_t rows, const void *const *ins, void *const *outs, cudaStream_t stream) {
-    const T *g = static_cast<const T *>(ins[0]), *u = t.packed ? g + t.gate.c : static_cast<const T *>(ins[1]);
-    return launch_pdl(token_gate_kernel<T, O>, dim3(static_cast<unsigned>(rows)), dim3(kThreads), 0, stream, t.gate, g, u, static_cast<O *>(outs[0]),
-                      sizeof(O) == 1 ? static_cast<float *>(outs[1]) : nullptr);
+template <typename T>
+cudaError_t gate_typed(const enn_b200_op *op, int32_t rows, const void *const *ins, void *const *outs) {
+    const TokenState &t = *op->token;
+    const GateParams &p = t.gate;
+    const T *g = static_cast<const T *>(ins[0]), *u = t.packed ? g + p.c : static_cast<const T *>(ins[1]);
+    const bool bytes = t.out_dtype == ENN_B200_S8;
+    const bool vec = p.c % kGroup == 0 && aligned(g, 16) && aligned(u, 16) && aligned(outs[0], bytes ? 8 : 16);
+    // Segments: of up to 4096 channels; of bytes up to eight of them, more where the rows alone do not occupy the device.
+    int segs = 1;
+    if (!bytes) segs = (p.c + 4095) / 4096;
+    else
+        while (segs < 8 && (p.c > 8192 * segs || (static_cast<int64_t>(rows) * segs * 2 <= 2 * op->ctx->sm_count && p.c >= 2048 * segs))) segs *= 2;
+    const int seg = segs == 1 ? p.c : ((p.c + segs - 1) / segs + kGroup - 1) / kGroup * kGroup;
+    if (!bytes) segs = (p.c + seg - 1) / seg;
+    const Shape s = row_shape(seg, vec, static_cast<int64_t>(rows) * segs <= 2 * op->ctx->sm_count);
+    const int per_block = segs > 1 && bytes ? 1 : s.per_block;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>((static_cast<int64_t>(rows) * segs + per_block - 1) / per_block));
+    cfg.blockDim = dim3(static_cast<unsigned>(s.nt), static_cast<unsigned>(per_block));
+    cfg.stream = op->ctx->stream;
+    cudaLaunchAttribute attr[2] = {};
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = static_cast<unsigned>(bytes ? segs : 1);
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = bytes && segs > 1 ? 2 : 1;
+    return with_shape(s.nv, vec, [&](auto nv, auto v) {
+        return cudaLaunchKernelEx(&cfg, token_gate_kernel<T, decltype(nv)::value, decltype(v)::value>, p, rows, segs, seg, t.out_dtype, g, u, outs[0],
+                                  bytes ? static_cast<float *>(outs[1]) : nullptr);
+    });
 }
 
 }  // namespace
 
-cudaError_t token_norm_launch(const TokenState &t, int32_t rows, const void *const *ins, void *const *outs, cudaStream_t stream) {
-    return with_type(t.in_dtype, [&](auto in) {
-        return with_type(t.out_dtype, [&](auto out) {
-            if constexpr (sizeof(in) == 1) return cudaErrorInvalidValue;
-            else return norm_typed<decltype(in), decltype(out)>(t, rows, ins, outs, stream);
-        });
-    });
+cudaError_t token_norm_launch(const enn_b200_op *op, int32_t rows, const void *const *ins, void *const *outs) {
+    switch (op->token->in_dtype) {
+        case ENN_B200_F32: return norm_typed<float>(op, rows, ins, outs);
+        case ENN_B200_F16: return norm_typed<__half>(op, rows, ins, outs);
+        case ENN_B200_BF16: return norm_typed<__nv_bfloat16>(op, rows, ins, outs);
+    }
+    return cudaErrorInvalidValue;
 }
 
-cudaError_t token_gate_launch(const TokenState &t, int32_t rows, const void *const *ins, void *const *outs, cudaStream_t stream) {
-    return with_type(t.in_dtype, [&](auto in) {
-        return with_type(t.out_dtype, [&](auto out) {
-            if constexpr (sizeof(in) == 1) return cudaErrorInvalidValue;
-            else return gate_typed<decltype(in), decltype(out)>(t, rows, ins, outs, stream);
-        });
-    });
+cudaError_t token_gate_launch(const enn_b200_op *op, int32_t rows, const void *const *ins, void *const *outs) {
+    switch (op->token->in_dtype) {
+        case ENN_B200_F32: return gate_typed<float>(op, rows, ins, outs);
+        case ENN_B200_F16: return gate_typed<__half>(op, rows, ins, outs);
+        case ENN_B200_BF16: return gate_typed<__nv_bfloat16>(op, rows, ins, outs);
+    }
+    return cudaErrorInvalidValue;
 }
 
 }  // namespace enn_b200
