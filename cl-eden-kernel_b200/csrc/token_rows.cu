@@ -4,6 +4,10 @@
 // A row belongs to a warp (up to 1024 channels), a CTA, or for quantised gates a cluster; a thread holds up to four groups of eight
 // neighbouring channels, 16 bytes of a 16-bit type.  Constant vectors come from L1, which they share with nothing: the rows are loaded
 // and stored past it.
+#include <algorithm>
+#include <type_traits>
+
+#include "per_device.h"
 #include "tc_common.cuh"
 #include "token_ops.h"
 
@@ -11,7 +15,6 @@ namespace enn_b200 {
 namespace {
 
 constexpr int kGroup = 8;           // channels a thread handles together
-constexpr int kMaxThreads = 1024;
 
 __device__ __forceinline__ uint4 ld_stream(const void *p) {
     uint4 v;
@@ -66,6 +69,9 @@ __device__ __forceinline__ uint32_t pack4_s8(const float *f, float inv) {
     return d;
 }
 
+// What a thread holds of eight channels between their loads and their use: as they lie in memory, or as floats where they came one by one.
+template <typename T, bool VEC> using Held = std::conditional_t<VEC, Raw<T>, Raw<float>>;
+
 // The part of a row that a group of `nt` threads holds: channels [0, n) of a segment, NV groups per thread.  VEC: neighbouring channels
 // in 16-byte pieces (n, every address and every pitch allow it); else one channel at a time, neighbouring threads on neighbouring
 // channels, for rows that begin anywhere.
@@ -74,20 +80,20 @@ struct Row {
     int n, tid, nt;
     __device__ __forceinline__ int at(int v, int j) const { return VEC ? (v * nt + tid) * kGroup + j : (v * kGroup + j) * nt + tid; }
 
-    template <typename T> __device__ __forceinline__ void load(const T *p, Raw<T> (&raw)[NV]) const {
-        if constexpr (VEC) {
+    template <typename T> __device__ __forceinline__ void load(const T *p, Held<T, VEC> (&held)[NV]) const {
 #pragma unroll
-            for (int v = 0; v < NV; ++v) {
-                raw[v] = Raw<T>{};
-                if (at(v, 0) < n) raw[v] = ld8(p + at(v, 0));
-            }
-        } else {
+        for (int v = 0; v < NV; ++v) {
+            held[v] = Held<T, VEC>{};
+            if constexpr (VEC) {
+                if (at(v, 0) < n) held[v] = ld8(p + at(v, 0));
+            } else {
+                float f[kGroup] = {};
 #pragma unroll
-            for (int v = 0; v < NV; ++v) {
-                T e[kGroup];
+                for (int j = 0; j < kGroup; ++j)
+                    if (at(v, j) < n) f[j] = to_float(p[at(v, j)]);
 #pragma unroll
-                for (int j = 0; j < kGroup; ++j) e[j] = at(v, j) < n ? p[at(v, j)] : from_float<T>(0.f);
-                __builtin_memcpy(&raw[v], e, sizeof(e));
+                for (int i = 0; i < 2; ++i)
+                    held[v].v[i] = make_uint4(__float_as_uint(f[4 * i]), __float_as_uint(f[4 * i + 1]), __float_as_uint(f[4 * i + 2]), __float_as_uint(f[4 * i + 3]));
             }
         }
     }
@@ -235,55 +241,128 @@ __device__ __forceinline__ void norm_row(const Row<NV, VEC> &row, float (&f)[NV]
     }
 }
 
+// Threads a block has at most: what the registers of NV groups a thread allow.
+constexpr int max_threads(int nv) { return nv == 1 ? 1024 : 512; }
+
+// A thread's own ring in shared memory: `depth` rows ahead, each with `streams` tensors, filled by asynchronous copies.  A thread reads
+// what it copied itself, so that no barrier is needed; the bytes in flight do not depend on how long a row's reductions take.
+template <typename T, int NV>
+struct Ahead {
+    static constexpr int kPieces = sizeof(T) / 2;      // 16-byte pieces of a group
+    uint32_t base;                                     // of this thread
+    uint32_t piece;                                    // bytes from piece to piece: 16 for each thread of the block
+    int streams, depth, slot;
+    __device__ __forceinline__ uint32_t at(int s, int stream, int v, int i) const { return base + static_cast<uint32_t>(((s * streams + stream) * NV + v) * kPieces + i) * piece; }
+    __device__ __forceinline__ void fetch(const Row<NV, true> &row, int s, int stream, const T *p) const {
+#pragma unroll
+        for (int v = 0; v < NV; ++v)
+            if (row.at(v, 0) < row.n)
+#pragma unroll
+                for (int i = 0; i < kPieces; ++i)
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at(s, stream, v, i)), "l"(reinterpret_cast<const uint4 *>(p + row.at(v, 0)) + i) : "memory");
+    }
+    __device__ __forceinline__ void read(const Row<NV, true> &row, int stream, Raw<T> (&held)[NV]) const {
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            held[v] = Raw<T>{};
+            if (row.at(v, 0) < row.n)
+#pragma unroll
+                for (int i = 0; i < kPieces; ++i) {
+                    uint4 &q = held[v].v[i];
+                    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(q.x), "=r"(q.y), "=r"(q.z), "=r"(q.w) : "r"(at(slot, stream, v, i)) : "memory");
+                }
+        }
+    }
+};
+__device__ __forceinline__ void ahead_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// All but the `pending` youngest groups have arrived.
+__device__ __forceinline__ void ahead_wait(int pending) {
+    if (pending >= 3) asm volatile("cp.async.wait_group 3;" ::: "memory");
+    else if (pending == 2) asm volatile("cp.async.wait_group 2;" ::: "memory");
+    else if (pending == 1) asm volatile("cp.async.wait_group 1;" ::: "memory");
+    else asm volatile("cp.async.wait_group 0;" ::: "memory");
+}
+constexpr int kMaxDepth = 4;
+constexpr int kRingBytes = 220 * 1024;
+
 template <typename T, int NV, bool VEC>
-__global__ void __launch_bounds__(kMaxThreads) token_norm_kernel(NormParams p, int32_t rows, int32_t out_dtype, const T *x, const T *residual, const T *gate, T *stream,
-                                                                 void *out, float *scale) {
+__global__ void __launch_bounds__(max_threads(NV), NV == 2 ? 2 : 1) token_norm_kernel(NormParams p, int32_t rows, int32_t out_dtype, int32_t depth, const T *x,
+                                                                                       const T *residual, const T *gate, T *stream, void *out, float *scale) {
+    extern __shared__ __align__(16) uint8_t ring[];
     __shared__ float2 scratch[2][32];
-    const int64_t t = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
+    const int64_t step = static_cast<int64_t>(gridDim.x) * blockDim.y;
     Row<NV, VEC> row{p.c, static_cast<int>(threadIdx.x), static_cast<int>(blockDim.x)};
     Reduce reduce{scratch, row.nt, 0};
     pdl_wait();
     pdl_trigger();
-    if (t >= rows) return;      // a whole warp, and then the block has no barrier
-    float f[NV][8];
-    {
-        Raw<T> rx[NV], rr[NV];
-        row.load(x + t * p.c, rx);
-        if (residual) row.load(residual + t * p.c, rr);
+    const int64_t first = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
+    [[maybe_unused]] Ahead<T, NV> ahead{};
+    if constexpr (VEC) {
+        const uint32_t threads = blockDim.x * blockDim.y;
+        ahead = Ahead<T, NV>{smem_u32(ring) + 16 * (threadIdx.y * blockDim.x + threadIdx.x), 16 * threads, 1 + (residual != nullptr) + (gate != nullptr), depth, 0};
+    }
+    auto fetch = [&](int s, int64_t t) {
+        if constexpr (VEC) {
+            if (t < rows) {
+                ahead.fetch(row, s, 0, x + t * p.c);
+                if (residual) ahead.fetch(row, s, 1, residual + t * p.c);
+                if (gate) ahead.fetch(row, s, ahead.streams - 1, gate + t / p.gate_tokens * p.c);
+            }
+            ahead_commit();
+        }
+    };
+    // Tensor `which` of row t, from the ring or from memory.
+    auto take = [&](int which, const T *p_row, float (&f)[NV][8]) {
+        Held<T, VEC> held[NV];
+        if constexpr (VEC) ahead.read(row, which, held);
+        else row.load(p_row, held);
 #pragma unroll
-        for (int v = 0; v < NV; ++v) widen(rx[v], f[v]);
+        for (int v = 0; v < NV; ++v) widen(held[v], f[v]);
+    };
+    if constexpr (VEC)
+        for (int s = 0; s < depth; ++s) fetch(s, first + s * step);
+    for (int64_t t = first; t < rows; t += step) {      // t is the same for a whole warp, and for the whole block where a row has several warps
+        float f[NV][8];
+        if constexpr (VEC) ahead_wait(depth - 1);
+        take(0, x + t * p.c, f);
         norm_row(row, f, p.c, p.post_norm, p.post_eps, p.post_weight, p.post_bias, reduce, nullptr);
         if (gate) {
-            Raw<T> rg[NV];
-            row.load(gate + t / p.gate_tokens * p.c, rg);
+            float g[NV][8];
+            take(VEC ? ahead.streams - 1 : 0, gate + t / p.gate_tokens * p.c, g);
 #pragma unroll
-            for (int v = 0; v < NV; ++v) {
-                float g[8];
-                widen(rg[v], g);
+            for (int v = 0; v < NV; ++v)
 #pragma unroll
-                for (int j = 0; j < kGroup; ++j) f[v][j] *= g[j];
-            }
+                for (int j = 0; j < kGroup; ++j) f[v][j] *= g[v][j];
         }
 #pragma unroll
-        for (int v = 0; v < NV; ++v) {
-            float h[8] = {};
-            if (residual) widen(rr[v], h);
+        for (int v = 0; v < NV; ++v)
 #pragma unroll
-            for (int j = 0; j < kGroup; ++j) f[v][j] = row.at(v, j) < row.n ? fmaf(f[v][j], p.residual_scale, h[j]) : 0.f;
+            for (int j = 0; j < kGroup; ++j) f[v][j] = row.at(v, j) < row.n ? f[v][j] * p.residual_scale : 0.f;
+        if (residual) {
+            float r[NV][8];
+            take(1, residual + t * p.c, r);
+#pragma unroll
+            for (int v = 0; v < NV; ++v)
+#pragma unroll
+                for (int j = 0; j < kGroup; ++j) f[v][j] += r[v][j];
         }
-    }
-    if (residual) row.store(stream + t * p.c, f);
-    if (out_dtype != ENN_B200_S8) {
-        norm_row(row, f, p.c, p.norm, p.eps, p.weight, p.bias, reduce, nullptr);
-        row.store_as(out_dtype, out, t * p.c, f);
-    } else {
-        uint32_t largest;
-        norm_row(row, f, p.c, p.norm, p.eps, p.weight, p.bias, reduce, &largest);
-        const RowScale rs = row_scale(largest);
-        int8_t *q = static_cast<int8_t *>(out) + t * p.pitch;
-        row.store_bytes(q, f, rs.inv);
-        for (int64_t i = p.c + row.tid; i < p.pitch; i += row.nt) q[i] = 0;
-        if (row.tid == 0) scale[t] = rs.scale;
+        if constexpr (VEC) {
+            fetch(ahead.slot, t + depth * step);        // this row's memory has been read
+            if (++ahead.slot == depth) ahead.slot = 0;
+        }
+        if (residual) row.store(stream + t * p.c, f);
+        if (out_dtype != ENN_B200_S8) {
+            norm_row(row, f, p.c, p.norm, p.eps, p.weight, p.bias, reduce, nullptr);
+            row.store_as(out_dtype, out, t * p.c, f);
+        } else {
+            uint32_t largest;
+            norm_row(row, f, p.c, p.norm, p.eps, p.weight, p.bias, reduce, &largest);
+            const RowScale rs = row_scale(largest);
+            int8_t *q = static_cast<int8_t *>(out) + t * p.pitch;
+            row.store_bytes(q, f, rs.inv);
+            for (int64_t i = p.c + row.tid; i < p.pitch; i += row.nt) q[i] = 0;
+            if (row.tid == 0) scale[t] = rs.scale;
+        }
     }
 }
 
@@ -307,7 +386,7 @@ __device__ __forceinline__ float gate_act(float g, int act) {
 // f = act(gates) * values of the thread's channels.
 template <typename T, int NV, bool VEC>
 __device__ __forceinline__ void gate_row(const Row<NV, VEC> &row, const T *gates, const T *values, int act, float (&f)[NV][8]) {
-    Raw<T> rg[NV], ru[NV];
+    Held<T, VEC> rg[NV], ru[NV];
     row.load(gates, rg);
     row.load(values, ru);
 #pragma unroll
@@ -333,7 +412,7 @@ __device__ __forceinline__ void gate_row(const Row<NV, VEC> &row, const T *gates
 // Row t / segs, segment t % segs of it: `seg` channels.  Floats leave at once.  Bytes need the row's largest magnitude first: the
 // segments of a row are then the CTAs of a cluster, which tell each other theirs.
 template <typename T, int NV, bool VEC>
-__global__ void __launch_bounds__(kMaxThreads) token_gate_kernel(GateParams p, int32_t rows, int32_t segs, int32_t seg, int32_t out_dtype, const T *gates, const T *values,
+__global__ void __launch_bounds__(max_threads(NV)) token_gate_kernel(GateParams p, int32_t rows, int32_t segs, int32_t seg, int32_t out_dtype, const T *gates, const T *values,
                                                                  void *out, float *scale) {
     __shared__ float2 scratch[2][32];
     __shared__ uint32_t of_cluster[8];
@@ -386,9 +465,7 @@ Shape row_shape(int n, bool vec, bool spread) {
     const int groups = (n + kGroup - 1) / kGroup;
     auto threads = [&](int nv) { return ((groups + nv - 1) / nv + 31) / 32 * 32; };
     Shape s;
-    if (!vec) s.nv = 4;
-    else if (groups <= 32 || (spread && threads(1) <= kMaxThreads)) s.nv = 1;
-    else s.nv = groups <= 64 || (groups > 128 && threads(2) <= kMaxThreads) ? 2 : 4;
+    s.nv = groups <= 32 || (spread && groups <= 1024) || (!vec && groups > 128 && groups <= 1024) ? 1 : (groups <= 64 || (groups > 128 && groups <= 1024) ? 2 : (groups <= 2048 ? 4 : 8));
     s.nt = threads(s.nv);
     s.per_block = s.nt == 32 ? 8 : 1;
     return s;
@@ -396,10 +473,15 @@ Shape row_shape(int n, bool vec, bool spread) {
 
 template <typename F>
 cudaError_t with_shape(int nv, bool vec, F f) {
-    if (!vec) return f(std::integral_constant<int, 4>{}, std::false_type{});
-    if (nv == 1) return f(std::integral_constant<int, 1>{}, std::true_type{});
-    if (nv == 2) return f(std::integral_constant<int, 2>{}, std::true_type{});
-    return f(std::integral_constant<int, 4>{}, std::true_type{});
+    auto groups = [&](auto v) {
+        switch (nv) {
+            case 1: return f(std::integral_constant<int, 1>{}, v);
+            case 2: return f(std::integral_constant<int, 2>{}, v);
+            case 4: return f(std::integral_constant<int, 4>{}, v);
+            default: return f(std::integral_constant<int, 8>{}, v);
+        }
+    };
+    return vec ? groups(std::true_type{}) : groups(std::false_type{});
 }
 
 template <typename T>
@@ -413,11 +495,22 @@ cudaError_t norm_typed(const enn_b200_op *op, int32_t rows, const void *const *i
     T *stream = t.residual ? static_cast<T *>(outs[o++]) : nullptr;
     void *y = outs[o++];
     float *scale = t.out_dtype == ENN_B200_S8 ? static_cast<float *>(outs[o++]) : nullptr;
-    const bool vec = p.c % kGroup == 0 && aligned(x, 16) && aligned(residual, 16) && aligned(gate, 16) && aligned(stream, 16) && aligned(y, scale ? 8 : 16);
-    const Shape s = row_shape(p.c, vec, rows <= 2 * op->ctx->sm_count);
-    const dim3 grid(static_cast<unsigned>((static_cast<int64_t>(rows) + s.per_block - 1) / s.per_block)), block(static_cast<unsigned>(s.nt), static_cast<unsigned>(s.per_block));
+    const bool lines = p.c % kGroup == 0 && aligned(x, 16) && aligned(residual, 16) && aligned(gate, 16) && aligned(stream, 16) && aligned(y, scale ? 8 : 16);
+    const Shape s = row_shape(p.c, lines, rows <= 2 * op->ctx->sm_count);
+    // The ring: up to four rows and 72 KB, two rows at least where shared memory holds them.
+    const int ahead_bytes = s.nt * s.per_block * s.nv * kGroup * static_cast<int>(sizeof(T)) * (1 + (residual != nullptr) + (gate != nullptr));
+    const int depth = std::min(kMaxDepth, std::max(72 * 1024 / ahead_bytes, 2 * ahead_bytes <= kRingBytes ? 2 : 1));
+    const bool vec = lines && ahead_bytes <= kRingBytes;
+    // About 1024 threads an SM, half of that with more than two groups a thread.
+    const int64_t want = (static_cast<int64_t>(rows) + s.per_block - 1) / s.per_block;
+    const int64_t most = static_cast<int64_t>(op->ctx->launch_sms()) * std::max(1, (s.nv <= 2 ? 1024 : 512) / (s.nt * s.per_block));
+    const dim3 grid(static_cast<unsigned>(std::min(want, most))), block(static_cast<unsigned>(s.nt), static_cast<unsigned>(s.per_block));
     return with_shape(s.nv, vec, [&](auto nv, auto v) {
-        return launch_pdl(token_norm_kernel<T, decltype(nv)::value, decltype(v)::value>, grid, block, 0, op->ctx->stream, p, rows, t.out_dtype, x, residual, gate, stream, y, scale);
+        constexpr auto kernel = token_norm_kernel<T, decltype(nv)::value, decltype(v)::value>;
+        static PerDeviceInit once;
+        const cudaError_t e = once.run(op->ctx->device, [&] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBytes); });
+        if (e != cudaSuccess) return e;
+        return launch_pdl(kernel, grid, block, vec ? static_cast<size_t>(depth) * ahead_bytes : 0, op->ctx->stream, p, rows, t.out_dtype, depth, x, residual, gate, stream, y, scale);
     });
 }
 
