@@ -97,20 +97,23 @@ struct Row {
             }
         }
     }
-    // A constant vector, or `absent` where there is none.
-    __device__ __forceinline__ void constant(const float *p, int v, float absent, float (&f)[8]) const {
-#pragma unroll
-        for (int j = 0; j < kGroup; ++j) f[j] = absent;
+    // f(channel value, constant) over the thread's channels; nothing where the constant vector is not given.
+    template <typename F> __device__ __forceinline__ void with(const float *p, float (&f)[NV][8], F apply) const {
         if (!p) return;
-        if constexpr (VEC) {
-            if (at(v, 0) < n) {
-                const float4 a = __ldg(reinterpret_cast<const float4 *>(p + at(v, 0))), b = __ldg(reinterpret_cast<const float4 *>(p + at(v, 0)) + 1);
-                f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
-            }
-        } else {
 #pragma unroll
-            for (int j = 0; j < kGroup; ++j)
-                if (at(v, j) < n) f[j] = __ldg(p + at(v, j));
+        for (int v = 0; v < NV; ++v) {
+            if constexpr (VEC) {
+                if (at(v, 0) < n) {
+                    const float4 a = __ldg(reinterpret_cast<const float4 *>(p + at(v, 0))), b = __ldg(reinterpret_cast<const float4 *>(p + at(v, 0)) + 1);
+                    const float w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+                    for (int j = 0; j < kGroup; ++j) f[v][j] = apply(f[v][j], w[j]);
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < kGroup; ++j)
+                    if (at(v, j) < n) f[v][j] = apply(f[v][j], __ldg(p + at(v, j)));
+            }
         }
     }
     template <typename T> __device__ __forceinline__ void store(T *p, const float (&f)[NV][8]) const {
@@ -144,46 +147,76 @@ struct Row {
     }
 };
 
-// Sum and maximum over the threads of a row: a warp, or the whole block.  Two sets of scratch words in turn, so that one barrier per
+// Sums and maxima over the threads of a row: a warp, or the whole block.  Two sets of scratch words in turn, so that one barrier per
 // reduction is enough.
+__device__ __forceinline__ float warp_sum(float s) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    return s;
+}
 struct Reduce {
     float2 (*scratch)[32];
     int nt, turn;
-    __device__ __forceinline__ void operator()(float &sum, uint32_t &largest) {
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        largest = __reduce_max_sync(0xffffffffu, largest);
-        if (nt == 32) return;
-        const int lane = threadIdx.x & 31, warps = nt >> 5;
-        if (lane == 0) scratch[turn][threadIdx.x >> 5] = make_float2(sum, __uint_as_float(largest));
+    __device__ __forceinline__ float2 exchange(float2 v) {
+        const int lane = threadIdx.x & 31;
+        if (lane == 0) scratch[turn][threadIdx.x >> 5] = v;
         __syncthreads();
-        const float2 v = lane < warps ? scratch[turn][lane] : make_float2(0.f, 0.f);
-        sum = v.x;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        largest = __reduce_max_sync(0xffffffffu, __float_as_uint(v.y));
+        v = lane < nt >> 5 ? scratch[turn][lane] : make_float2(0.f, 0.f);
         turn ^= 1;
+        return v;
     }
     __device__ __forceinline__ float sum(float s) {
-        uint32_t m = 0;
-        (*this)(s, m);
-        return s;
+        s = warp_sum(s);
+        return nt == 32 ? s : warp_sum(exchange(make_float2(s, 0.f)).x);
     }
     __device__ __forceinline__ uint32_t largest(uint32_t m) {
-        float s = 0.f;
-        (*this)(s, m);
-        return m;
+        m = __reduce_max_sync(0xffffffffu, m);
+        return nt == 32 ? m : __reduce_max_sync(0xffffffffu, __float_as_uint(exchange(make_float2(0.f, __uint_as_float(m))).y));
+    }
+    __device__ __forceinline__ void both(float &s, uint32_t &m) {
+        s = warp_sum(s);
+        m = __reduce_max_sync(0xffffffffu, m);
+        if (nt == 32) return;
+        const float2 v = exchange(make_float2(s, __uint_as_float(m)));
+        s = warp_sum(v.x);
+        m = __reduce_max_sync(0xffffffffu, __float_as_uint(v.y));
     }
 };
 
-// f = norm(f).  With `largest` the bits of the largest magnitude of the result come back too; for an RMS norm without a bias they ride on
-// the sum of squares, since max |f r w| = r max |f w|.
+template <int NV>
+__device__ __forceinline__ float sum_of_squares(const float (&f)[NV][8]) {
+    float s = 0.f;
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+#pragma unroll
+        for (int j = 0; j < kGroup; ++j) s = fmaf(f[v][j], f[v][j], s);
+    return s;
+}
+template <int NV>
+__device__ __forceinline__ uint32_t largest_of(const float (&f)[NV][8]) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+#pragma unroll
+        for (int j = 0; j < kGroup; ++j) m = max(m, magnitude(f[v][j]));
+    return m;
+}
+template <int NV>
+__device__ __forceinline__ void multiply(float (&f)[NV][8], float by) {
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+#pragma unroll
+        for (int j = 0; j < kGroup; ++j) f[v][j] *= by;
+}
+
+// f = norm(f).  Channels past the row's end are 0 before and after.  With `largest` the bits of the largest magnitude of the result
+// come back too; for an RMS norm without a bias they ride on the sum of squares, since max |f r w| = r max |f w|.
 template <int NV, bool VEC>
 __device__ __forceinline__ void norm_row(const Row<NV, VEC> &row, float (&f)[NV][8], int c, int kind, float eps, const float *weight, const float *bias, Reduce &reduce,
                                          uint32_t *largest) {
+    const auto times = [](float a, float w) { return a * w; };
     if (kind != ENN_B200_NORM_NONE) {
         const float over = 1.f / static_cast<float>(c);
-        const bool joint = largest && kind == ENN_B200_NORM_RMS && !bias;
         if (kind == ENN_B200_NORM_LAYER) {
             float s = 0.f;
 #pragma unroll
@@ -194,51 +227,23 @@ __device__ __forceinline__ void norm_row(const Row<NV, VEC> &row, float (&f)[NV]
 #pragma unroll
             for (int v = 0; v < NV; ++v)
 #pragma unroll
-                for (int j = 0; j < kGroup; ++j) f[v][j] = row.at(v, j) < row.n ? f[v][j] - mean : 0.f;
+                for (int j = 0; j < kGroup; ++j) f[v][j] = row.at(v, VEC ? 0 : j) < row.n ? f[v][j] - mean : 0.f;
         }
-        float s = 0.f;
-        uint32_t m = 0;
-#pragma unroll
-        for (int v = 0; v < NV; ++v) {
-            float w[8];
-            if (joint) row.constant(weight, v, 1.f, w);
-#pragma unroll
-            for (int j = 0; j < kGroup; ++j) {
-                s = fmaf(f[v][j], f[v][j], s);
-                if (joint) {
-                    f[v][j] *= w[j];
-                    m = max(m, magnitude(f[v][j]));
-                }
-            }
-        }
-        reduce(s, m);
-        const float r = rsqrtf(fmaf(s, over, eps));
-        if (joint) {
-#pragma unroll
-            for (int v = 0; v < NV; ++v)
-#pragma unroll
-                for (int j = 0; j < kGroup; ++j) f[v][j] *= r;
+        float s = sum_of_squares(f);
+        if (largest && kind == ENN_B200_NORM_RMS && !bias) {
+            row.with(weight, f, times);
+            uint32_t m = largest_of(f);
+            reduce.both(s, m);
+            const float r = rsqrtf(fmaf(s, over, eps));
+            multiply(f, r);
             *largest = magnitude(__uint_as_float(m) * r);
             return;
         }
-#pragma unroll
-        for (int v = 0; v < NV; ++v) {
-            float w[8], b[8];
-            row.constant(weight, v, 1.f, w);
-            row.constant(bias, v, 0.f, b);
-#pragma unroll
-            for (int j = 0; j < kGroup; ++j) f[v][j] = fmaf(f[v][j] * r, w[j], b[j]);
-        }
+        multiply(f, rsqrtf(fmaf(reduce.sum(s), over, eps)));
+        row.with(weight, f, times);
+        row.with(bias, f, [](float a, float b) { return a + b; });
     }
-    if (largest) {
-        uint32_t m = 0;
-#pragma unroll
-        for (int v = 0; v < NV; ++v)
-#pragma unroll
-            for (int j = 0; j < kGroup; ++j)
-                if (row.at(v, j) < row.n) m = max(m, magnitude(f[v][j]));
-        *largest = reduce.largest(m);
-    }
+    if (largest) *largest = reduce.largest(largest_of(f));
 }
 
 // Threads a block has at most: what the registers of NV groups a thread allow.
@@ -334,17 +339,15 @@ __global__ void __launch_bounds__(max_threads(NV), NV == 2 ? 2 : 1) token_norm_k
 #pragma unroll
                 for (int j = 0; j < kGroup; ++j) f[v][j] *= g[v][j];
         }
-#pragma unroll
-        for (int v = 0; v < NV; ++v)
-#pragma unroll
-            for (int j = 0; j < kGroup; ++j) f[v][j] = row.at(v, j) < row.n ? f[v][j] * p.residual_scale : 0.f;
         if (residual) {
             float r[NV][8];
             take(1, residual + t * p.c, r);
 #pragma unroll
             for (int v = 0; v < NV; ++v)
 #pragma unroll
-                for (int j = 0; j < kGroup; ++j) f[v][j] += r[v][j];
+                for (int j = 0; j < kGroup; ++j) f[v][j] = fmaf(f[v][j], p.residual_scale, r[v][j]);
+        } else if (p.residual_scale != 1.f) {
+            multiply(f, p.residual_scale);
         }
         if constexpr (VEC) {
             fetch(ahead.slot, t + depth * step);        // this row's memory has been read
@@ -366,21 +369,30 @@ __global__ void __launch_bounds__(max_threads(NV), NV == 2 ? 2 : 1) token_norm_k
     }
 }
 
-// 1 / (1 + e^-g) from an exponential that does not overflow; 2^x and the reciprocal are a unit or two off in the last place.
-__device__ __forceinline__ float sigmoid(float g) {
-    float e, r;
-    asm("ex2.approx.f32 %0, %1;" : "=f"(e) : "f"(fabsf(g) * -1.4426950408889634f));
-    asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
-    return (g >= 0.f ? 1.f : e) * r;
+// 2^(-|g| log2(e) / 2), the root of e^-|g|: below 2^-126 only where its square is nothing to any result.  The instructions for 2^x and
+// the reciprocal are a unit or two off in the last place.
+__device__ __forceinline__ float root_exp(float g) {
+    float h;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(h) : "f"(fabsf(g) * -0.72134752044448170f));
+    return h;
 }
-__device__ __forceinline__ float gate_act(float g, int act) {
-    switch (act) {
-        case ENN_B200_GATE_SILU: return g * sigmoid(g);
-        case ENN_B200_GATE_GELU: return 0.5f * g * (1.f + erff(g * 0.70710678118654752f));
-        case ENN_B200_GATE_GELU_TANH: return g * sigmoid(2.f * 0.79788456080286536f * fmaf(0.044715f * g * g, g, g));      // (1 + tanh v) / 2 is the sigmoid of 2 v
-        case ENN_B200_GATE_RELU: return g < 0.f ? 0.f : g;
-        default: return sigmoid(g);
-    }
+__device__ __forceinline__ float reciprocal(float a) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(a));
+    return r;
+}
+// a / (1 + e^-g) from an exponential that does not overflow.
+__device__ __forceinline__ float times_sigmoid(float a, float g) {
+    const float h = root_exp(g), e = h * h;
+    return (g >= 0.f ? a : a * e) * reciprocal(1.f + e);
+}
+template <int ACT>
+__device__ __forceinline__ float gate_act(float g) {
+    if (ACT == ENN_B200_GATE_SILU) return times_sigmoid(g, g);
+    if (ACT == ENN_B200_GATE_GELU) return 0.5f * g * (1.f + erff(g * 0.70710678118654752f));
+    if (ACT == ENN_B200_GATE_GELU_TANH) return times_sigmoid(g, 2.f * 0.79788456080286536f * fmaf(0.044715f * g * g, g, g));      // (1 + tanh v) / 2 is the sigmoid of 2 v
+    if (ACT == ENN_B200_GATE_RELU) return g < 0.f ? 0.f : g;
+    return times_sigmoid(1.f, g);
 }
 
 // f = act(gates) * values of the thread's channels.
@@ -389,35 +401,34 @@ __device__ __forceinline__ void gate_row(const Row<NV, VEC> &row, const T *gates
     Held<T, VEC> rg[NV], ru[NV];
     row.load(gates, rg);
     row.load(values, ru);
+    auto apply = [&](auto which) {
 #pragma unroll
-    for (int v = 0; v < NV; ++v) {
-        float g[8], u[8];
-        widen(rg[v], g);
-        widen(ru[v], u);
-        switch (act) {      // once per group, not per channel
-#define ENN_ACT(A)                                                                        \
-    case A:                                                                               \
-        _Pragma("unroll") for (int j = 0; j < kGroup; ++j) f[v][j] = gate_act(g[j], A) * u[j]; \
-        break;
-            ENN_ACT(ENN_B200_GATE_SILU)
-            ENN_ACT(ENN_B200_GATE_GELU)
-            ENN_ACT(ENN_B200_GATE_GELU_TANH)
-            ENN_ACT(ENN_B200_GATE_RELU)
-            ENN_ACT(ENN_B200_GATE_SIGMOID)
-#undef ENN_ACT
+        for (int v = 0; v < NV; ++v) {
+            float g[8], u[8];
+            widen(rg[v], g);
+            widen(ru[v], u);
+#pragma unroll
+            for (int j = 0; j < kGroup; ++j) f[v][j] = gate_act<decltype(which)::value>(g[j]) * u[j];
         }
+    };
+    switch (act) {
+        case ENN_B200_GATE_SILU: apply(std::integral_constant<int, ENN_B200_GATE_SILU>{}); break;
+        case ENN_B200_GATE_GELU: apply(std::integral_constant<int, ENN_B200_GATE_GELU>{}); break;
+        case ENN_B200_GATE_GELU_TANH: apply(std::integral_constant<int, ENN_B200_GATE_GELU_TANH>{}); break;
+        case ENN_B200_GATE_RELU: apply(std::integral_constant<int, ENN_B200_GATE_RELU>{}); break;
+        default: apply(std::integral_constant<int, ENN_B200_GATE_SIGMOID>{});
     }
 }
 
-// Row t / segs, segment t % segs of it: `seg` channels.  Floats leave at once.  Bytes need the row's largest magnitude first: the
+// Grid: rows x segments of `seg` channels.  Floats leave at once.  Bytes need the row's largest magnitude first: the
 // segments of a row are then the CTAs of a cluster, which tell each other theirs.
 template <typename T, int NV, bool VEC>
-__global__ void __launch_bounds__(max_threads(NV)) token_gate_kernel(GateParams p, int32_t rows, int32_t segs, int32_t seg, int32_t out_dtype, const T *gates, const T *values,
+__global__ void __launch_bounds__(max_threads(NV)) token_gate_kernel(GateParams p, int32_t rows, int32_t seg, int32_t out_dtype, const T *gates, const T *values,
                                                                  void *out, float *scale) {
     __shared__ float2 scratch[2][32];
     __shared__ uint32_t of_cluster[8];
-    const int64_t item = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y, t = item / segs;
-    const int32_t rank = static_cast<int32_t>(item - t * segs), c0 = rank * seg;
+    const int64_t t = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
+    const int32_t segs = static_cast<int32_t>(gridDim.y), rank = static_cast<int32_t>(blockIdx.y), c0 = rank * seg;
     Row<NV, VEC> row{min(seg, p.c - c0), static_cast<int>(threadIdx.x), static_cast<int>(blockDim.x)};
     // Seen by the others of the cluster before they write here: waited for below.
     const bool clustered = segs > 1 && out_dtype == ENN_B200_S8;
@@ -431,14 +442,8 @@ __global__ void __launch_bounds__(max_threads(NV)) token_gate_kernel(GateParams 
         row.store_as(out_dtype, out, t * p.c + c0, f);
         return;
     }
-    uint32_t largest = 0;
-#pragma unroll
-    for (int v = 0; v < NV; ++v)
-#pragma unroll
-        for (int j = 0; j < kGroup; ++j)
-            if (row.at(v, j) < row.n) largest = max(largest, magnitude(f[v][j]));
     Reduce reduce{scratch, row.nt, 0};
-    largest = reduce.largest(largest);
+    uint32_t largest = reduce.largest(largest_of(f));      // 0 past the segment's end
     if (clustered) {
         asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
         if (row.tid < segs) asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(mapa_rank(smem_u32(of_cluster + rank), row.tid)), "r"(largest) : "memory");
@@ -457,7 +462,7 @@ __global__ void __launch_bounds__(max_threads(NV)) token_gate_kernel(GateParams 
 bool aligned(const void *p, size_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
 
 // Threads of a row and groups per thread for `n` channels.  `spread`: as many threads as there are groups (few rows: latency), else
-// two groups each (many rows: twice the bytes in flight per thread, half the threads in a reduction).
+// four groups each (many rows: what a row costs whatever its length, reductions and addresses, is shared by more channels).
 struct Shape {
     int nt, nv, per_block;
 };
@@ -465,7 +470,9 @@ Shape row_shape(int n, bool vec, bool spread) {
     const int groups = (n + kGroup - 1) / kGroup;
     auto threads = [&](int nv) { return ((groups + nv - 1) / nv + 31) / 32 * 32; };
     Shape s;
-    s.nv = groups <= 32 || (spread && groups <= 1024) || (!vec && groups > 128 && groups <= 1024) ? 1 : (groups <= 64 || (groups > 128 && groups <= 1024) ? 2 : (groups <= 2048 ? 4 : 8));
+    if (groups <= 32 || ((spread || !vec) && groups <= 1024)) s.nv = 1;
+    else if (groups <= 64 || (!vec && groups <= 1024)) s.nv = 2;
+    else s.nv = groups <= 2048 ? 4 : 8;
     s.nt = threads(s.nv);
     s.per_block = s.nt == 32 ? 8 : 1;
     return s;
@@ -521,9 +528,9 @@ cudaError_t gate_typed(const enn_b200_op *op, int32_t rows, const void *const *i
     const T *g = static_cast<const T *>(ins[0]), *u = t.packed ? g + p.c : static_cast<const T *>(ins[1]);
     const bool bytes = t.out_dtype == ENN_B200_S8;
     const bool vec = p.c % kGroup == 0 && aligned(g, 16) && aligned(u, 16) && aligned(outs[0], bytes ? 8 : 16);
-    // Segments: of up to 4096 channels; of bytes up to eight of them, more where the rows alone do not occupy the device.
+    // Segments: of up to 8192 channels; of bytes up to eight of them, more where the rows alone do not occupy the device.
     int segs = 1;
-    if (!bytes) segs = (p.c + 4095) / 4096;
+    if (!bytes) segs = (p.c + 8191) / 8192;
     else
         while (segs < 8 && (p.c > 8192 * segs || (static_cast<int64_t>(rows) * segs * 2 <= 2 * op->ctx->sm_count && p.c >= 2048 * segs))) segs *= 2;
     const int seg = segs == 1 ? p.c : ((p.c + segs - 1) / segs + kGroup - 1) / kGroup * kGroup;
@@ -531,19 +538,19 @@ cudaError_t gate_typed(const enn_b200_op *op, int32_t rows, const void *const *i
     const Shape s = row_shape(seg, vec, static_cast<int64_t>(rows) * segs <= 2 * op->ctx->sm_count);
     const int per_block = segs > 1 && bytes ? 1 : s.per_block;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(static_cast<unsigned>((static_cast<int64_t>(rows) * segs + per_block - 1) / per_block));
+    cfg.gridDim = dim3(static_cast<unsigned>((static_cast<int64_t>(rows) + per_block - 1) / per_block), static_cast<unsigned>(segs));
     cfg.blockDim = dim3(static_cast<unsigned>(s.nt), static_cast<unsigned>(per_block));
     cfg.stream = op->ctx->stream;
     cudaLaunchAttribute attr[2] = {};
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
     attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = static_cast<unsigned>(bytes ? segs : 1);
-    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    attr[1].val.clusterDim.x = attr[1].val.clusterDim.z = 1;
+    attr[1].val.clusterDim.y = static_cast<unsigned>(segs);
     cfg.attrs = attr;
     cfg.numAttrs = bytes && segs > 1 ? 2 : 1;
     return with_shape(s.nv, vec, [&](auto nv, auto v) {
-        return cudaLaunchKernelEx(&cfg, token_gate_kernel<T, decltype(nv)::value, decltype(v)::value>, p, rows, segs, seg, t.out_dtype, g, u, outs[0],
+        return cudaLaunchKernelEx(&cfg, token_gate_kernel<T, decltype(nv)::value, decltype(v)::value>, p, rows, seg, t.out_dtype, g, u, outs[0],
                                   bytes ? static_cast<float *>(outs[1]) : nullptr);
     });
 }
