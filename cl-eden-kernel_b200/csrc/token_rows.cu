@@ -247,7 +247,9 @@ __device__ __forceinline__ void norm_row(const Row<NV, VEC> &row, float (&f)[NV]
 }
 
 // Threads a block has at most: what the registers of NV groups a thread allow.
-constexpr int max_threads(int nv) { return nv == 1 ? 1024 : 512; }
+constexpr int max_threads(int nv) { return nv == 1 ? 1024 : (nv == 4 ? 256 : 512); }
+// Blocks of that size an SM is to hold: 64 registers a thread, 80 with four groups, 128 with eight.
+constexpr int min_blocks(int nv) { return nv == 4 ? 3 : (nv == 2 ? 2 : 1); }
 
 // A thread's own ring in shared memory: `depth` rows ahead, each with `streams` tensors, filled by asynchronous copies.  A thread reads
 // what it copied itself, so that no barrier is needed; the bytes in flight do not depend on how long a row's reductions take.
@@ -288,10 +290,10 @@ __device__ __forceinline__ void ahead_wait(int pending) {
     else asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 constexpr int kMaxDepth = 4;
-constexpr int kRingBytes = 220 * 1024;
+constexpr int kRingBytes = 216 * 1024;
 
 template <typename T, int NV, bool VEC>
-__global__ void __launch_bounds__(max_threads(NV), NV == 2 ? 2 : 1) token_norm_kernel(NormParams p, int32_t rows, int32_t out_dtype, int32_t depth, const T *x,
+__global__ void __launch_bounds__(max_threads(NV), min_blocks(NV)) token_norm_kernel(NormParams p, int32_t rows, int32_t out_dtype, int32_t depth, const T *x,
                                                                                        const T *residual, const T *gate, T *stream, void *out, float *scale) {
     extern __shared__ __align__(16) uint8_t ring[];
     __shared__ float2 scratch[2][32];
@@ -472,7 +474,7 @@ Shape row_shape(int n, bool vec, bool spread) {
     Shape s;
     if (groups <= 32 || ((spread || !vec) && groups <= 1024)) s.nv = 1;
     else if (groups <= 64 || (!vec && groups <= 1024)) s.nv = 2;
-    else s.nv = groups <= 2048 ? 4 : 8;
+    else s.nv = groups <= 1024 ? 4 : 8;
     s.nt = threads(s.nv);
     s.per_block = s.nt == 32 ? 8 : 1;
     return s;
@@ -504,13 +506,13 @@ cudaError_t norm_typed(const enn_b200_op *op, int32_t rows, const void *const *i
     float *scale = t.out_dtype == ENN_B200_S8 ? static_cast<float *>(outs[o++]) : nullptr;
     const bool lines = p.c % kGroup == 0 && aligned(x, 16) && aligned(residual, 16) && aligned(gate, 16) && aligned(stream, 16) && aligned(y, scale ? 8 : 16);
     const Shape s = row_shape(p.c, lines, rows <= 2 * op->ctx->sm_count);
-    // The ring: up to four rows and 72 KB, two rows at least where shared memory holds them.
-    const int ahead_bytes = s.nt * s.per_block * s.nv * kGroup * static_cast<int>(sizeof(T)) * (1 + (residual != nullptr) + (gate != nullptr));
-    const int depth = std::min(kMaxDepth, std::max(72 * 1024 / ahead_bytes, 2 * ahead_bytes <= kRingBytes ? 2 : 1));
+    // As many blocks as an SM holds, each taking rows in turn, and rings of up to four rows in what shared memory that leaves them.
+    const int threads = s.nt * s.per_block;
+    const int blocks = std::max(1, max_threads(s.nv) * min_blocks(s.nv) / threads);
+    const int ahead_bytes = threads * s.nv * kGroup * static_cast<int>(sizeof(T)) * (1 + (residual != nullptr) + (gate != nullptr));
+    const int depth = std::min(kMaxDepth, std::max(1, kRingBytes / blocks / ahead_bytes));
     const bool vec = lines && ahead_bytes <= kRingBytes;
-    // About 1024 threads an SM, half of that with more than two groups a thread.
-    const int64_t want = (static_cast<int64_t>(rows) + s.per_block - 1) / s.per_block;
-    const int64_t most = static_cast<int64_t>(op->ctx->launch_sms()) * std::max(1, (s.nv <= 2 ? 1024 : 512) / (s.nt * s.per_block));
+    const int64_t want = (static_cast<int64_t>(rows) + s.per_block - 1) / s.per_block, most = static_cast<int64_t>(op->ctx->launch_sms()) * blocks;
     const dim3 grid(static_cast<unsigned>(std::min(want, most))), block(static_cast<unsigned>(s.nt), static_cast<unsigned>(s.per_block));
     return with_shape(s.nv, vec, [&](auto nv, auto v) {
         constexpr auto kernel = token_norm_kernel<T, decltype(nv)::value, decltype(v)::value>;
