@@ -1,96 +1,369 @@
 // log_probs: log probabilities of given ids, entropy and the largest alternatives of rows of logits.
+//
+// Bound by reading the logits, which happens once: with k = scale * log2(e), m the running maximum and d = k (l - m), a thread keeps
+//   S = sum 2^d   and   U = sum d 2^d,
+// rescaled whenever m grows (S' = c S, U' = c (U + d S) with d = k (m - m'), c = 2^d).  Then
+//   log p = scale (l - m) - ln S,   entropy = ln S - ln 2 U / S.
+// The alternatives come from the same pass: a thread remembers where its largest logit was.  The n-th largest of the threads' maxima
+// bounds the n-th largest logit from below, so that what is above it lies with n threads, and their logits alone are looked at again.
+// A row is split over a cluster of up to eight CTAs where the rows alone do not occupy the device; the parts meet in the first CTA's
+// shared memory, without atomics or workspace.  All orders are total (value, then index), so that results do not depend on timing.
 #include <math_constants.h>
 
+#include <algorithm>
+
+#include "tc_common.cuh"
 #include "token_ops.h"
 
 namespace enn_b200 {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 512, kWarps = kThreads / 32;
+constexpr int kMaxTop = ENN_B200_LOG_PROBS_MAX_TOP;
+constexpr int kMaxSegments = 8;
+constexpr int kChunk = 4;               // 16-byte loads of a thread under way at a time
+constexpr int kCandidates = 2048;
+constexpr float kNothing = -1e4f;       // 2^-10000 is 0; keeps the products d 2^d away from infinity times 0
+constexpr float kLowest = -3.402823466e38f;
 
-// Order of the logits as unsigned integers: NaN above +inf, -0 equal to +0; the lower index first among equals.
+// Order of the logits as unsigned integers: NaN above +inf, -0 equal to +0; the lower index first among equals.  0 is below all keys.
 __device__ __forceinline__ uint64_t order_key(float v, int32_t index) {
     uint32_t b = __float_as_uint(v + 0.f);
     if (v != v) b = 0x7fffffffu;
     b = b & 0x80000000u ? ~b : b | 0x80000000u;
     return static_cast<uint64_t>(b) << 32 | (0xffffffffu - static_cast<uint32_t>(index));
 }
+__device__ __forceinline__ int32_t key_index(uint64_t key) { return static_cast<int32_t>(0xffffffffu - static_cast<uint32_t>(key)); }
+__device__ __forceinline__ float key_value(uint64_t key) {
+    const uint32_t b = static_cast<uint32_t>(key >> 32);
+    return __uint_as_float(b & 0x80000000u ? b & 0x7fffffffu : ~b);
+}
+
+__device__ __forceinline__ float exp2_fast(float x) {      // two units in the last place; 0 below 2^-126
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {      // NaN if either is
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
+// A segment [begin, end) of a row as 16-byte pieces at 16-byte addresses: piece g holds the logits begin - skip + g E .. + E, of which
+// those outside the segment (in the first and the last piece) read as -inf and are not loaded.
+template <typename T>
+struct Segment {
+    static constexpr int E = 16 / sizeof(T);
+    const T *row;
+    int32_t begin, end, skip, pieces;
+    __device__ __forceinline__ Segment(const T *r, int32_t b, int32_t e) : row(r), begin(b), end(e) {
+        skip = static_cast<int32_t>((reinterpret_cast<uintptr_t>(r + b) & 15) / sizeof(T));
+        pieces = e > b ? (e - b + skip + E - 1) / E : 0;
+    }
+    __device__ __forceinline__ int32_t first(int32_t g) const { return begin - skip + g * E; }
+    __device__ __forceinline__ bool whole(int32_t g) const { return first(g) >= begin && first(g) + E <= end; }
+    __device__ __forceinline__ void load(int32_t g, float (&x)[E]) const {
+        const int32_t at = first(g);
+        if (whole(g)) {
+            uint4 v;
+            asm volatile("ld.global.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(row + at));
+            T t[E];
+            __builtin_memcpy(t, &v, 16);
+#pragma unroll
+            for (int i = 0; i < E; ++i) x[i] = to_float(t[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < E; ++i) x[i] = at + i >= begin && at + i < end ? to_float(row[at + i]) : -CUDART_INF_F;
+        }
+    }
+    __device__ __forceinline__ bool holds(int32_t index) const { return index >= begin && index < end; }
+};
+
+struct Stats {
+    float m, s, u;
+    __device__ __forceinline__ void rescale(float to, float k) {
+        const float d = fmaxf((m - to) * k, kNothing), c = exp2_fast(d);
+        u = c * fmaf(d, s, u);
+        s *= c;
+        m = to;
+    }
+};
+
+// The `n` largest keys of up to 32 lists in descending order, 0 past their ends; one warp, lane i walks list i.
+__device__ __forceinline__ void take_largest(const uint64_t *lists, int n_lists, int length, int stride, int n, uint64_t *out) {
+    const int lane = threadIdx.x & 31;
+    int at = 0;
+    uint64_t head = lane < n_lists && length ? lists[lane * stride] : 0;
+    for (int i = 0; i < n; ++i) {
+        const uint32_t hi = __reduce_max_sync(0xffffffffu, static_cast<uint32_t>(head >> 32));
+        const uint32_t lo = __reduce_max_sync(0xffffffffu, static_cast<uint32_t>(head >> 32) == hi ? static_cast<uint32_t>(head) : 0u);
+        const uint64_t key = static_cast<uint64_t>(hi) << 32 | lo;
+        if (lane == 0) out[i] = key;
+        if (key && head == key) head = ++at < length ? lists[lane * stride + at] : 0;
+    }
+}
+
+struct Shared {
+    float part[3][kWarps];
+    uint64_t lists[kWarps][32];                 // the warps' maxima in descending order
+    uint64_t winners[kMaxTop];
+    uint64_t candidates[kCandidates];
+    int32_t n_candidates;
+    uint64_t sorted[kMaxTop];                   // the largest of this segment
+    Stats stats[kMaxSegments];                  // of the first CTA: what the segments found
+    uint64_t merged[kMaxSegments][kMaxTop];
+};
 
 template <typename V, typename F>
-__device__ __forceinline__ V block_reduce(V v, V *scratch, F join) {
+__device__ __forceinline__ V warp_join(V v, F join) {
+#pragma unroll
     for (int o = 16; o > 0; o >>= 1) v = join(v, __shfl_xor_sync(0xffffffffu, v, o));
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = scratch[threadIdx.x & (kThreads / 32 - 1)];
-    for (int o = kThreads / 64; o > 0; o >>= 1) v = join(v, __shfl_xor_sync(0xffffffffu, v, o));
     return v;
 }
 
+// Round by round over the whole segment: for rows with NaN or +inf, and where more candidates turn up than there is room for.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) log_probs_kernel(LogProbsParams p, const T *logits, const int32_t *ids, float *given, float *entropy, int32_t *top_ids, float *top) {
-    __shared__ float scratch[kThreads / 32];
-    __shared__ uint64_t scratch64[kThreads / 32];
+__device__ __noinline__ void largest_by_rounds(const Segment<T> &seg, int top, Shared &sh) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    uint64_t below = ~0ull;
+    for (int r = 0; r < top; ++r) {
+        uint64_t best = 0;
+        for (int32_t g = threadIdx.x; g < seg.pieces; g += kThreads) {
+            float x[Segment<T>::E];
+            seg.load(g, x);
+            for (int i = 0; i < Segment<T>::E; ++i) {
+                const int32_t at = seg.first(g) + i;
+                const uint64_t k = seg.holds(at) ? order_key(x[i], at) : 0;
+                if (k < below && k > best) best = k;
+            }
+        }
+        best = warp_join(best, [](uint64_t a, uint64_t b) { return a > b ? a : b; });
+        __syncthreads();
+        if (lane == 0) sh.lists[0][warp] = best;
+        __syncthreads();
+        for (int w = 0; w < kWarps; ++w) best = sh.lists[0][w] > best ? sh.lists[0][w] : best;
+        if (threadIdx.x == 0) sh.sorted[r] = best;
+        below = best;
+    }
+    __syncthreads();
+}
+
+// sh.sorted[0 .. top): the largest keys of the segment.  `mine`: the key of the thread's largest logit, 0 if it has none.
+template <typename T>
+__device__ __forceinline__ void largest_of_segment(const Segment<T> &seg, uint64_t mine, int top, Shared &sh) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    // a warp's maxima in descending order (bitonic)
+#pragma unroll
+    for (int size = 2; size <= 32; size <<= 1)
+#pragma unroll
+        for (int by = size >> 1; by > 0; by >>= 1) {
+            const uint64_t other = __shfl_xor_sync(0xffffffffu, mine, by);
+            const bool larger = ((lane & by) == 0) == ((lane & size) == 0 || size == 32);
+            if (larger == (other > mine)) mine = other;
+        }
+    sh.lists[warp][lane] = mine;
+    if (threadIdx.x == 0) sh.n_candidates = 0;
+    if (threadIdx.x < top) sh.sorted[threadIdx.x] = 0;
+    __syncthreads();
+    if (warp == 0) take_largest(&sh.lists[0][0], kWarps, 32, 32, top, sh.winners);
+    __syncthreads();
+    const uint64_t least = sh.winners[top - 1];      // 0 where fewer threads than that have logits: everything counts
+    for (int w = warp; w < top; w += kWarps) {
+        const uint64_t key = sh.winners[w];
+        if (!key) break;
+        const int32_t owner = ((key_index(key) - seg.begin + seg.skip) / Segment<T>::E) % kThreads;
+        for (int32_t g = owner + kThreads * lane; g < seg.pieces; g += kThreads * 32) {
+            float x[Segment<T>::E];
+            seg.load(g, x);
+            for (int i = 0; i < Segment<T>::E; ++i) {
+                const int32_t at = seg.first(g) + i;
+                const uint64_t k = seg.holds(at) ? order_key(x[i], at) : 0;
+                if (k && k >= least) {
+                    const int32_t slot = atomicAdd(&sh.n_candidates, 1);
+                    if (slot < kCandidates) sh.candidates[slot] = k;
+                }
+            }
+        }
+    }
+    __syncthreads();
+    const int n = sh.n_candidates;
+    if (n > kCandidates) {
+        largest_by_rounds(seg, top, sh);
+        return;
+    }
+    for (int i = threadIdx.x; i < n; i += kThreads) {      // its place is the number of larger ones
+        const uint64_t k = sh.candidates[i];
+        int place = 0;
+        for (int j = 0; j < n; ++j) place += sh.candidates[j] > k;
+        if (place < top) sh.sorted[place] = k;
+    }
+    __syncthreads();
+}
+
+// Grid: rows x segments, the segments of a row being a cluster.
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 2) log_probs_kernel(LogProbsParams p, int32_t seg_size, const T *logits, const int32_t *ids, float *given, float *entropy,
+                                                                int32_t *top_ids, float *top) {
+    __shared__ Shared sh;
+    constexpr int E = Segment<T>::E;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int segs = gridDim.y, rank = blockIdx.y;
+    const int64_t t = blockIdx.x;
+    if (segs > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");      // waited for before the first CTA's memory is written
+    const T *row = logits + t * p.pitch;
+    const Segment<T> seg(row, rank * seg_size, min(p.vocab, (rank + 1) * seg_size));
+    const float k = p.scale * 1.4426950408889634f;
     pdl_wait();
     pdl_trigger();
-    const int64_t t = blockIdx.x;
-    const T *row = logits + t * p.pitch;
-    float largest = -CUDART_INF_F;
-    for (int i = threadIdx.x; i < p.vocab; i += kThreads) largest = fmaxf(largest, to_float(row[i]) * p.scale);
-    largest = block_reduce(largest, scratch, [](float a, float b) { return fmaxf(a, b); });
-    // With d = z - largest: S = sum e^d, U = sum d e^d; lse = largest + log S, entropy = log S - U / S.
-    float s = 0.f, u = 0.f;
-    for (int i = threadIdx.x; i < p.vocab; i += kThreads) {
-        const float d = to_float(row[i]) * p.scale - largest, e = expf(d);
-        s += e;
-        u += d == -CUDART_INF_F ? 0.f : d * e;
+
+    Stats a{kLowest, 0.f, 0.f};
+    float best = -CUDART_INF_F;
+    int32_t best_at = threadIdx.x;      // first piece of the chunk with the thread's largest logit
+    for (int32_t g0 = threadIdx.x; g0 < seg.pieces; g0 += kThreads * kChunk) {
+        float x[kChunk][E];
+#pragma unroll
+        for (int c = 0; c < kChunk; ++c) {
+            const int32_t g = g0 + c * kThreads;
+            if (g < seg.pieces) {
+                seg.load(g, x[c]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < E; ++i) x[c][i] = -CUDART_INF_F;
+            }
+        }
+        float largest = x[0][0];
+#pragma unroll
+        for (int c = 0; c < kChunk; ++c)
+#pragma unroll
+            for (int i = 0; i < E; ++i) largest = fmaxf(largest, x[c][i]);
+        if (largest > best) {
+            best = largest;
+            best_at = g0;
+            a.rescale(fmaxf(largest, kLowest), k);
+        }
+#pragma unroll
+        for (int c = 0; c < kChunk; ++c)
+#pragma unroll
+            for (int i = 0; i < E; ++i) {
+                const float d = max_nan((x[c][i] - a.m) * k, kNothing), e = exp2_fast(d);
+                a.s += e;
+                a.u = fmaf(d, e, a.u);
+            }
     }
-    s = block_reduce(s, scratch, [](float a, float b) { return a + b; });
-    u = block_reduce(u, scratch, [](float a, float b) { return a + b; });
-    const float log_s = logf(s);
-    if (threadIdx.x == 0) entropy[t] = log_s - u / s;
+
+    // The statistics of the segment, the same in every thread.
+    float m = warp_join(a.m, [](float x, float y) { return fmaxf(x, y); });
+    if (lane == 0) sh.part[0][warp] = m;
+    __syncthreads();
+    m = warp_join(sh.part[0][lane % kWarps], [](float x, float y) { return fmaxf(x, y); });
+    a.rescale(m, k);
+    const auto plus = [](float x, float y) { return x + y; };
+    a.s = warp_join(a.s, plus);
+    a.u = warp_join(a.u, plus);
+    if (lane == 0) {
+        sh.part[1][warp] = a.s;
+        sh.part[2][warp] = a.u;
+    }
+    __syncthreads();
+    a.s = warp_join(lane < kWarps ? sh.part[1][lane] : 0.f, plus);
+    a.u = warp_join(lane < kWarps ? sh.part[2][lane] : 0.f, plus);
+
+    if (p.top) {
+        if (a.s != a.s) {
+            largest_by_rounds(seg, p.top, sh);
+        } else {
+            uint64_t mine = 0;
+            if (static_cast<int32_t>(threadIdx.x) < seg.pieces) {
+                for (int c = kChunk - 1; c >= 0; --c) {
+                    const int32_t g = best_at + c * kThreads;
+                    if (g >= seg.pieces) continue;
+                    float x[E];
+                    seg.load(g, x);
+#pragma unroll
+                    for (int i = E - 1; i >= 0; --i)
+                        if (x[i] == best && seg.holds(seg.first(g) + i)) mine = order_key(x[i], seg.first(g) + i);
+                }
+            }
+            largest_of_segment(seg, mine, p.top, sh);
+        }
+    }
+    if (segs > 1) {
+        asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+        if (threadIdx.x < p.top) {
+            const uint64_t key = sh.sorted[threadIdx.x];
+            asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(mapa_rank(smem_u32(&sh.merged[rank][threadIdx.x]), 0)), "l"(key) : "memory");
+        }
+        if (threadIdx.x == 0) {
+            const uint32_t at = mapa_rank(smem_u32(&sh.stats[rank]), 0);
+            asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at), "f"(a.m) : "memory");
+            asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at + 4), "f"(a.s) : "memory");
+            asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at + 8), "f"(a.u) : "memory");
+        }
+        cluster_sync_all();
+        if (rank != 0) return;
+        a = sh.stats[0];
+        for (int s = 1; s < segs; ++s) {
+            Stats b = sh.stats[s];
+            const float to = fmaxf(a.m, b.m);
+            a.rescale(to, k);
+            b.rescale(to, k);
+            a.s += b.s;
+            a.u += b.u;
+        }
+        if (warp == 0 && p.top) take_largest(&sh.merged[0][0], segs, p.top, kMaxTop, p.top, sh.sorted);
+        __syncthreads();
+    }
+    // A row that is ruled out as a whole has no exponentials at all.
+    const float log_s = a.s == 0.f ? CUDART_NAN_F : logf(a.s);
+    const auto log_p = [&](float l) { return (l - a.m) * p.scale - log_s; };
+    if (threadIdx.x == 0) entropy[t] = log_s - 0.69314718055994531f * (a.u / a.s);
     for (int j = threadIdx.x; j < p.given; j += kThreads) {
         const int32_t id = ids[t * p.given + j];
-        given[t * p.given + j] = id < 0 ? 0.f : (id >= p.vocab ? CUDART_NAN_F : (to_float(row[id]) * p.scale - largest) - log_s);
+        given[t * p.given + j] = id < 0 ? 0.f : (id >= p.vocab ? CUDART_NAN_F : log_p(to_float(row[id])));
     }
-    uint64_t below = ~0ull;
-    for (int j = 0; j < p.top; ++j) {
-        uint64_t best = 0;
-        for (int i = threadIdx.x; i < p.vocab; i += kThreads) {
-            const uint64_t k = order_key(to_float(row[i]), i);
-            if (k < below && k > best) best = k;
-        }
-        best = block_reduce(best, scratch64, [](uint64_t a, uint64_t b) { return a > b ? a : b; });
-        below = best;
-        const int32_t id = static_cast<int32_t>(0xffffffffu - static_cast<uint32_t>(best));
-        if (threadIdx.x == 0) {
-            top_ids[t * p.top + j] = id;
-            top[t * p.top + j] = (to_float(row[id]) * p.scale - largest) - log_s;
-        }
+    if (threadIdx.x < p.top) {
+        const uint64_t key = sh.sorted[threadIdx.x];
+        top_ids[t * p.top + threadIdx.x] = key_index(key);
+        top[t * p.top + threadIdx.x] = log_p(key_value(key));
     }
 }
 
 template <typename T>
-cudaError_t launch_typed(const TokenState &t, int32_t rows, const void *const *ins, void *const *outs, cudaStream_t stream) {
-    const LogProbsParams &p = t.log_probs;
+cudaError_t launch_typed(const enn_b200_op *op, int32_t rows, const void *const *ins, void *const *outs) {
+    const LogProbsParams &p = op->token->log_probs;
     int o = 0;
     const int32_t *ids = p.given ? static_cast<const int32_t *>(ins[1]) : nullptr;
     float *given = p.given ? static_cast<float *>(outs[o++]) : nullptr;
     float *entropy = static_cast<float *>(outs[o++]);
     int32_t *top_ids = p.top ? static_cast<int32_t *>(outs[o++]) : nullptr;
     float *top = p.top ? static_cast<float *>(outs[o++]) : nullptr;
-    return launch_pdl(log_probs_kernel<T>, dim3(static_cast<unsigned>(rows)), dim3(kThreads), 0, stream, p, static_cast<const T *>(ins[0]), ids, given, entropy, top_ids, top);
+    // Segments while the device has room for two CTAs an SM and a segment keeps a chunk for every thread.
+    int segs = 1;
+    while (segs < kMaxSegments && static_cast<int64_t>(rows) * segs * 2 <= 2 * op->ctx->sm_count && p.vocab / (segs * 2) >= 4096) segs *= 2;
+    const int32_t seg_size = (p.vocab + segs - 1) / segs;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>(rows), static_cast<unsigned>(segs));
+    cfg.blockDim = dim3(kThreads);
+    cfg.stream = op->ctx->stream;
+    cudaLaunchAttribute attr[2] = {};
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = attr[1].val.clusterDim.z = 1;
+    attr[1].val.clusterDim.y = static_cast<unsigned>(segs);
+    cfg.attrs = attr;
+    cfg.numAttrs = segs > 1 ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, log_probs_kernel<T>, p, seg_size, static_cast<const T *>(ins[0]), ids, given, entropy, top_ids, top);
 }
 
 }  // namespace
 
 cudaError_t log_probs_launch(const enn_b200_op *op, int32_t rows, const void *const *ins, void *const *outs) {
-    const TokenState &t = *op->token;
-    const cudaStream_t stream = op->ctx->stream;
-    switch (t.in_dtype) {
-        case ENN_B200_F32: return launch_typed<float>(t, rows, ins, outs, stream);
-        case ENN_B200_F16: return launch_typed<__half>(t, rows, ins, outs, stream);
-        case ENN_B200_BF16: return launch_typed<__nv_bfloat16>(t, rows, ins, outs, stream);
+    switch (op->token->in_dtype) {
+        case ENN_B200_F32: return launch_typed<float>(op, rows, ins, outs);
+        case ENN_B200_F16: return launch_typed<__half>(op, rows, ins, outs);
+        case ENN_B200_BF16: return launch_typed<__nv_bfloat16>(op, rows, ins, outs);
     }
     return cudaErrorInvalidValue;
 }
