@@ -12,17 +12,21 @@
 
 #include <algorithm>
 
+#include "per_device.h"
 #include "tc_common.cuh"
 #include "token_ops.h"
 
 namespace enn_b200 {
 namespace {
 
-constexpr int kThreads = 512, kWarps = kThreads / 32;
+constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kMaxTop = ENN_B200_LOG_PROBS_MAX_TOP;
 constexpr int kMaxSegments = 8;
-constexpr int kChunk = 4;               // 16-byte loads of a thread under way at a time
-constexpr int kCandidates = 2048;
+constexpr int kChunk = 4;               // 16-byte pieces a thread works on at a time
+constexpr int kDepth = 3;               // chunks a thread asks for ahead
+constexpr int kBlocks = 3;              // CTAs an SM is to hold
+constexpr int kCandidates = 1024;
+constexpr int kLookers = 8;             // threads that look at one thread's logits again
 constexpr float kNothing = -1e4f;       // 2^-10000 is 0; keeps the products d 2^d away from infinity times 0
 constexpr float kLowest = -3.402823466e38f;
 
@@ -63,22 +67,45 @@ struct Segment {
     }
     __device__ __forceinline__ int32_t first(int32_t g) const { return begin - skip + g * E; }
     __device__ __forceinline__ bool whole(int32_t g) const { return first(g) >= begin && first(g) + E <= end; }
-    __device__ __forceinline__ void load(int32_t g, float (&x)[E]) const {
-        const int32_t at = first(g);
+    __device__ __forceinline__ uint4 load(int32_t g) const {
+        uint4 v;
         if (whole(g)) {
-            uint4 v;
-            asm volatile("ld.global.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(row + at));
-            T t[E];
-            __builtin_memcpy(t, &v, 16);
-#pragma unroll
-            for (int i = 0; i < E; ++i) x[i] = to_float(t[i]);
+            asm volatile("ld.global.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(row + first(g)));
         } else {
+            T t[E];
 #pragma unroll
-            for (int i = 0; i < E; ++i) x[i] = at + i >= begin && at + i < end ? to_float(row[at + i]) : -CUDART_INF_F;
+            for (int i = 0; i < E; ++i) t[i] = holds(first(g) + i) ? row[first(g) + i] : from_float<T>(-CUDART_INF_F);
+            __builtin_memcpy(&v, t, 16);
         }
+        return v;
     }
+    // The key of logit i of piece g, 0 outside the segment.
+    __device__ __forceinline__ uint64_t key(int32_t g, int i, float v) const { return holds(first(g) + i) ? order_key(v, first(g) + i) : 0; }
     __device__ __forceinline__ bool holds(int32_t index) const { return index >= begin && index < end; }
 };
+
+__device__ __forceinline__ void unpack(uint4 v, float (&x)[4], float) {
+    x[0] = __uint_as_float(v.x); x[1] = __uint_as_float(v.y); x[2] = __uint_as_float(v.z); x[3] = __uint_as_float(v.w);
+}
+__device__ __forceinline__ float2 unpack2(uint32_t w, __half) { return __half22float2(*reinterpret_cast<const __half2 *>(&w)); }
+__device__ __forceinline__ float2 unpack2(uint32_t w, __nv_bfloat16) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
+template <typename T> __device__ __forceinline__ void unpack(uint4 v, float (&x)[8], T) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = unpack2(w[i], T{});
+        x[2 * i] = f.x;
+        x[2 * i + 1] = f.y;
+    }
+}
+template <typename T> __device__ __forceinline__ uint4 nothing() {      // a piece of -inf
+    const float2 f = make_float2(-CUDART_INF_F, -CUDART_INF_F);
+    if constexpr (sizeof(T) == 4) return make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u);
+    T t[2] = {from_float<T>(f.x), from_float<T>(f.y)};
+    uint32_t w;
+    __builtin_memcpy(&w, t, 4);
+    return make_uint4(w, w, w, w);
+}
 
 struct Stats {
     float m, s, u;
@@ -131,10 +158,9 @@ __device__ __noinline__ void largest_by_rounds(const Segment<T> &seg, int top, S
         uint64_t best = 0;
         for (int32_t g = threadIdx.x; g < seg.pieces; g += kThreads) {
             float x[Segment<T>::E];
-            seg.load(g, x);
+            unpack(seg.load(g), x, T{});
             for (int i = 0; i < Segment<T>::E; ++i) {
-                const int32_t at = seg.first(g) + i;
-                const uint64_t k = seg.holds(at) ? order_key(x[i], at) : 0;
+                const uint64_t k = seg.key(g, i, x[i]);
                 if (k < below && k > best) best = k;
             }
         }
@@ -166,19 +192,20 @@ __device__ __forceinline__ void largest_of_segment(const Segment<T> &seg, uint64
     if (threadIdx.x == 0) sh.n_candidates = 0;
     if (threadIdx.x < top) sh.sorted[threadIdx.x] = 0;
     __syncthreads();
-    if (warp == 0) take_largest(&sh.lists[0][0], kWarps, 32, 32, top, sh.winners);
+    if (warp == 0) take_largest(&sh.lists[0][0], kWarps, 32, 32, top, top == 1 ? sh.sorted : sh.winners);
     __syncthreads();
+    if (top == 1) return;      // the largest of the maxima is the largest
     const uint64_t least = sh.winners[top - 1];      // 0 where fewer threads than that have logits: everything counts
-    for (int w = warp; w < top; w += kWarps) {
+    for (int w = threadIdx.x / kLookers; w < top; w += kThreads / kLookers) {      // a few threads look at the logits of each of them
         const uint64_t key = sh.winners[w];
         if (!key) break;
         const int32_t owner = ((key_index(key) - seg.begin + seg.skip) / Segment<T>::E) % kThreads;
-        for (int32_t g = owner + kThreads * lane; g < seg.pieces; g += kThreads * 32) {
+        for (int32_t g = owner + kThreads * static_cast<int32_t>(threadIdx.x % kLookers); g < seg.pieces; g += kThreads * kLookers) {
             float x[Segment<T>::E];
-            seg.load(g, x);
+            unpack(seg.load(g), x, T{});
+#pragma unroll
             for (int i = 0; i < Segment<T>::E; ++i) {
-                const int32_t at = seg.first(g) + i;
-                const uint64_t k = seg.holds(at) ? order_key(x[i], at) : 0;
+                const uint64_t k = seg.key(g, i, x[i]);
                 if (k && k >= least) {
                     const int32_t slot = atomicAdd(&sh.n_candidates, 1);
                     if (slot < kCandidates) sh.candidates[slot] = k;
@@ -201,131 +228,160 @@ __device__ __forceinline__ void largest_of_segment(const Segment<T> &seg, uint64
     __syncthreads();
 }
 
-// Grid: rows x segments, the segments of a row being a cluster.
+// Grid: rows x segments, the segments of a row being a cluster.  Where rows have one segment a CTA takes several of them, and the copies
+// of the next row's first chunks are under way while the alternatives of this one are sorted out.
 template <typename T>
-__global__ void __launch_bounds__(kThreads, 2) log_probs_kernel(LogProbsParams p, int32_t seg_size, const T *logits, const int32_t *ids, float *given, float *entropy,
-                                                                int32_t *top_ids, float *top) {
+__global__ void __launch_bounds__(kThreads, kBlocks) log_probs_kernel(LogProbsParams p, int32_t rows, int32_t seg_size, const T *logits, const int32_t *ids, float *given,
+                                                                      float *entropy, int32_t *top_ids, float *top) {
+    extern __shared__ __align__(16) uint8_t ring[];      // [kDepth][kChunk][kThreads] pieces: a thread reads what it copied itself
     __shared__ Shared sh;
     constexpr int E = Segment<T>::E;
+    constexpr int kStep = kThreads * kChunk;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int segs = gridDim.y, rank = blockIdx.y;
-    const int64_t t = blockIdx.x;
     if (segs > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");      // waited for before the first CTA's memory is written
-    const T *row = logits + t * p.pitch;
-    const Segment<T> seg(row, rank * seg_size, min(p.vocab, (rank + 1) * seg_size));
+    const auto segment = [&](int64_t t) { return Segment<T>(logits + t * p.pitch, rank * seg_size, min(p.vocab, (rank + 1) * seg_size)); };
     const float k = p.scale * 1.4426950408889634f;
+    const uint32_t mine0 = smem_u32(ring) + threadIdx.x * 16;
+    const auto place = [&](int slot, int c) { return mine0 + static_cast<uint32_t>(slot * kChunk + c) * (kThreads * 16); };
     pdl_wait();
     pdl_trigger();
 
-    Stats a{kLowest, 0.f, 0.f};
-    float best = -CUDART_INF_F;
-    int32_t best_at = threadIdx.x;      // first piece of the chunk with the thread's largest logit
-    for (int32_t g0 = threadIdx.x; g0 < seg.pieces; g0 += kThreads * kChunk) {
-        float x[kChunk][E];
+    // What is copied next: piece g_next (of thread 0) of row t_next.
+    int64_t t_next = blockIdx.x;
+    int32_t g_next = 0;
+    Segment<T> ahead = segment(min(t_next, static_cast<int64_t>(rows) - 1));
+    const auto fetch = [&](int slot) {
+        if (t_next < rows) {
 #pragma unroll
-        for (int c = 0; c < kChunk; ++c) {
-            const int32_t g = g0 + c * kThreads;
-            if (g < seg.pieces) {
-                seg.load(g, x[c]);
-            } else {
-#pragma unroll
-                for (int i = 0; i < E; ++i) x[c][i] = -CUDART_INF_F;
+            for (int c = 0; c < kChunk; ++c) {
+                const int32_t g = g_next + c * kThreads + static_cast<int32_t>(threadIdx.x);
+                if (g < ahead.pieces && ahead.whole(g)) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(place(slot, c)), "l"(ahead.row + ahead.first(g)) : "memory");
+            }
+            g_next += kStep;
+            if (g_next >= ahead.pieces) {
+                g_next = 0;
+                t_next += gridDim.x;
+                if (t_next < rows) ahead = segment(t_next);
             }
         }
-        float largest = x[0][0];
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    for (int s = 0; s < kDepth; ++s) fetch(s);
+    int slot = 0;
+
+    for (int64_t t = blockIdx.x; t < rows; t += gridDim.x) {
+        const Segment<T> seg = segment(t);
+        Stats a{kLowest, 0.f, 0.f};
+        float best = -CUDART_INF_F;
+        int32_t best_at = max(seg.first(threadIdx.x), seg.begin);      // of the thread's largest logit
+        for (int32_t g0 = 0; g0 < seg.pieces; g0 += kStep) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 1) : "memory");
+            uint4 raw[kChunk];
+            float largest = -CUDART_INF_F;
 #pragma unroll
-        for (int c = 0; c < kChunk; ++c)
+            for (int c = 0; c < kChunk; ++c) {
+                const int32_t g = g0 + c * kThreads + static_cast<int32_t>(threadIdx.x);
+                raw[c] = nothing<T>();
+                if (g < seg.pieces) {
+                    if (seg.whole(g))
+                        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(raw[c].x), "=r"(raw[c].y), "=r"(raw[c].z), "=r"(raw[c].w) : "r"(place(slot, c)) : "memory");
+                    else
+                        raw[c] = seg.load(g);
+                }
+                float x[E];
+                unpack(raw[c], x, T{});
 #pragma unroll
-            for (int i = 0; i < E; ++i) largest = fmaxf(largest, x[c][i]);
-        if (largest > best) {
-            best = largest;
-            best_at = g0;
-            a.rescale(fmaxf(largest, kLowest), k);
-        }
-#pragma unroll
-        for (int c = 0; c < kChunk; ++c)
-#pragma unroll
-            for (int i = 0; i < E; ++i) {
-                const float d = max_nan((x[c][i] - a.m) * k, kNothing), e = exp2_fast(d);
-                a.s += e;
-                a.u = fmaf(d, e, a.u);
+                for (int i = 0; i < E; ++i) largest = fmaxf(largest, x[i]);
             }
-    }
-
-    // The statistics of the segment, the same in every thread.
-    float m = warp_join(a.m, [](float x, float y) { return fmaxf(x, y); });
-    if (lane == 0) sh.part[0][warp] = m;
-    __syncthreads();
-    m = warp_join(sh.part[0][lane % kWarps], [](float x, float y) { return fmaxf(x, y); });
-    a.rescale(m, k);
-    const auto plus = [](float x, float y) { return x + y; };
-    a.s = warp_join(a.s, plus);
-    a.u = warp_join(a.u, plus);
-    if (lane == 0) {
-        sh.part[1][warp] = a.s;
-        sh.part[2][warp] = a.u;
-    }
-    __syncthreads();
-    a.s = warp_join(lane < kWarps ? sh.part[1][lane] : 0.f, plus);
-    a.u = warp_join(lane < kWarps ? sh.part[2][lane] : 0.f, plus);
-
-    if (p.top) {
-        if (a.s != a.s) {
-            largest_by_rounds(seg, p.top, sh);
-        } else {
-            uint64_t mine = 0;
-            if (static_cast<int32_t>(threadIdx.x) < seg.pieces) {
+            fetch(slot);
+            if (++slot == kDepth) slot = 0;
+            if (largest > best) {
+                best = largest;
+                int32_t where = 0;
+#pragma unroll
                 for (int c = kChunk - 1; c >= 0; --c) {
-                    const int32_t g = best_at + c * kThreads;
-                    if (g >= seg.pieces) continue;
                     float x[E];
-                    seg.load(g, x);
+                    unpack(raw[c], x, T{});
 #pragma unroll
-                    for (int i = E - 1; i >= 0; --i)
-                        if (x[i] == best && seg.holds(seg.first(g) + i)) mine = order_key(x[i], seg.first(g) + i);
+                    for (int i = E - 1; i >= 0; --i) where = x[i] == largest ? c * (kThreads * E) + i : where;
+                }
+                best_at = seg.first(g0 + static_cast<int32_t>(threadIdx.x)) + where;
+                a.rescale(fmaxf(largest, kLowest), k);
+            }
+#pragma unroll
+            for (int c = 0; c < kChunk; ++c) {
+                float x[E];
+                unpack(raw[c], x, T{});
+#pragma unroll
+                for (int i = 0; i < E; ++i) {
+                    const float d = max_nan((x[i] - a.m) * k, kNothing), e = exp2_fast(d);
+                    a.s += e;
+                    a.u = fmaf(d, e, a.u);
                 }
             }
-            largest_of_segment(seg, mine, p.top, sh);
         }
-    }
-    if (segs > 1) {
-        asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+
+        // The statistics of the segment, the same in every thread.
+        float m = warp_join(a.m, [](float x, float y) { return fmaxf(x, y); });
+        if (lane == 0) sh.part[0][warp] = m;
+        __syncthreads();
+        m = warp_join(sh.part[0][lane % kWarps], [](float x, float y) { return fmaxf(x, y); });
+        a.rescale(m, k);
+        const auto plus = [](float x, float y) { return x + y; };
+        a.s = warp_join(a.s, plus);
+        a.u = warp_join(a.u, plus);
+        if (lane == 0) {
+            sh.part[1][warp] = a.s;
+            sh.part[2][warp] = a.u;
+        }
+        __syncthreads();
+        a.s = warp_join(lane < kWarps ? sh.part[1][lane] : 0.f, plus);
+        a.u = warp_join(lane < kWarps ? sh.part[2][lane] : 0.f, plus);
+
+        if (p.top) {
+            if (a.s != a.s) largest_by_rounds(seg, p.top, sh);
+            else largest_of_segment(seg, static_cast<int32_t>(threadIdx.x) < seg.pieces ? order_key(best, best_at) : 0, p.top, sh);
+        }
+        if (segs > 1) {
+            asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+            if (threadIdx.x < p.top) {
+                const uint64_t key = sh.sorted[threadIdx.x];
+                asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(mapa_rank(smem_u32(&sh.merged[rank][threadIdx.x]), 0)), "l"(key) : "memory");
+            }
+            if (threadIdx.x == 0) {
+                const uint32_t at = mapa_rank(smem_u32(&sh.stats[rank]), 0);
+                asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at), "f"(a.m) : "memory");
+                asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at + 4), "f"(a.s) : "memory");
+                asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at + 8), "f"(a.u) : "memory");
+            }
+            cluster_sync_all();
+            if (rank != 0) return;      // a cluster has one row
+            a = sh.stats[0];
+            for (int s = 1; s < segs; ++s) {
+                Stats b = sh.stats[s];
+                const float to = fmaxf(a.m, b.m);
+                a.rescale(to, k);
+                b.rescale(to, k);
+                a.s += b.s;
+                a.u += b.u;
+            }
+            if (warp == 0 && p.top) take_largest(&sh.merged[0][0], segs, p.top, kMaxTop, p.top, sh.sorted);
+            __syncthreads();
+        }
+        // A row that is ruled out as a whole has no exponentials at all.
+        const float log_s = a.s == 0.f ? CUDART_NAN_F : logf(a.s);
+        const auto log_p = [&](float l) { return (l - a.m) * p.scale - log_s; };
+        if (threadIdx.x == 0) entropy[t] = log_s - 0.69314718055994531f * (a.u / a.s);
+        for (int j = threadIdx.x; j < p.given; j += kThreads) {
+            const int32_t id = ids[t * p.given + j];
+            given[t * p.given + j] = id < 0 ? 0.f : (id >= p.vocab ? CUDART_NAN_F : log_p(to_float(seg.row[id])));
+        }
         if (threadIdx.x < p.top) {
             const uint64_t key = sh.sorted[threadIdx.x];
-            asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(mapa_rank(smem_u32(&sh.merged[rank][threadIdx.x]), 0)), "l"(key) : "memory");
+            top_ids[t * p.top + threadIdx.x] = key_index(key);
+            top[t * p.top + threadIdx.x] = log_p(key_value(key));
         }
-        if (threadIdx.x == 0) {
-            const uint32_t at = mapa_rank(smem_u32(&sh.stats[rank]), 0);
-            asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at), "f"(a.m) : "memory");
-            asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at + 4), "f"(a.s) : "memory");
-            asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at + 8), "f"(a.u) : "memory");
-        }
-        cluster_sync_all();
-        if (rank != 0) return;
-        a = sh.stats[0];
-        for (int s = 1; s < segs; ++s) {
-            Stats b = sh.stats[s];
-            const float to = fmaxf(a.m, b.m);
-            a.rescale(to, k);
-            b.rescale(to, k);
-            a.s += b.s;
-            a.u += b.u;
-        }
-        if (warp == 0 && p.top) take_largest(&sh.merged[0][0], segs, p.top, kMaxTop, p.top, sh.sorted);
-        __syncthreads();
-    }
-    // A row that is ruled out as a whole has no exponentials at all.
-    const float log_s = a.s == 0.f ? CUDART_NAN_F : logf(a.s);
-    const auto log_p = [&](float l) { return (l - a.m) * p.scale - log_s; };
-    if (threadIdx.x == 0) entropy[t] = log_s - 0.69314718055994531f * (a.u / a.s);
-    for (int j = threadIdx.x; j < p.given; j += kThreads) {
-        const int32_t id = ids[t * p.given + j];
-        given[t * p.given + j] = id < 0 ? 0.f : (id >= p.vocab ? CUDART_NAN_F : log_p(to_float(row[id])));
-    }
-    if (threadIdx.x < p.top) {
-        const uint64_t key = sh.sorted[threadIdx.x];
-        top_ids[t * p.top + threadIdx.x] = key_index(key);
-        top[t * p.top + threadIdx.x] = log_p(key_value(key));
     }
 }
 
@@ -338,12 +394,18 @@ cudaError_t launch_typed(const enn_b200_op *op, int32_t rows, const void *const 
     float *entropy = static_cast<float *>(outs[o++]);
     int32_t *top_ids = p.top ? static_cast<int32_t *>(outs[o++]) : nullptr;
     float *top = p.top ? static_cast<float *>(outs[o++]) : nullptr;
-    // Segments while the device has room for two CTAs an SM and a segment keeps a chunk for every thread.
+    // Segments while the device has room for them and a segment keeps a chunk for every thread.
+    const int64_t slots = static_cast<int64_t>(kBlocks) * op->ctx->sm_count;
     int segs = 1;
-    while (segs < kMaxSegments && static_cast<int64_t>(rows) * segs * 2 <= 2 * op->ctx->sm_count && p.vocab / (segs * 2) >= 4096) segs *= 2;
+    while (segs < kMaxSegments && static_cast<int64_t>(rows) * segs * 2 <= slots && p.vocab / (segs * 2) >= 4096) segs *= 2;
     const int32_t seg_size = (p.vocab + segs - 1) / segs;
+    static PerDeviceInit once;
+    constexpr int kRing = kDepth * kChunk * kThreads * 16;
+    const cudaError_t e = once.run(op->ctx->device, [] { return cudaFuncSetAttribute(log_probs_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRing); });
+    if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(static_cast<unsigned>(rows), static_cast<unsigned>(segs));
+    cfg.gridDim = dim3(static_cast<unsigned>(segs > 1 ? rows : std::min<int64_t>(rows, slots)), static_cast<unsigned>(segs));
+    cfg.dynamicSmemBytes = kRing;
     cfg.blockDim = dim3(kThreads);
     cfg.stream = op->ctx->stream;
     cudaLaunchAttribute attr[2] = {};
@@ -354,7 +416,7 @@ cudaError_t launch_typed(const enn_b200_op *op, int32_t rows, const void *const 
     attr[1].val.clusterDim.y = static_cast<unsigned>(segs);
     cfg.attrs = attr;
     cfg.numAttrs = segs > 1 ? 2 : 1;
-    return cudaLaunchKernelEx(&cfg, log_probs_kernel<T>, p, seg_size, static_cast<const T *>(ins[0]), ids, given, entropy, top_ids, top);
+    return cudaLaunchKernelEx(&cfg, log_probs_kernel<T>, p, rows, seg_size, static_cast<const T *>(ins[0]), ids, given, entropy, top_ids, top);
 }
 
 }  // namespace
