@@ -65,6 +65,8 @@ struct Segment {
         skip = static_cast<int32_t>((reinterpret_cast<uintptr_t>(r + b) & 15) / sizeof(T));
         pieces = e > b ? (e - b + skip + E - 1) / E : 0;
     }
+    // Pieces [g, g + n) lie in the segment as a whole.
+    __device__ __forceinline__ bool inside(int32_t g, int32_t n) const { return first(g) >= begin && first(g + n) <= end; }
     __device__ __forceinline__ int32_t first(int32_t g) const { return begin - skip + g * E; }
     __device__ __forceinline__ bool whole(int32_t g) const { return first(g) >= begin && first(g) + E <= end; }
     __device__ __forceinline__ uint4 load(int32_t g) const {
@@ -253,10 +255,13 @@ __global__ void __launch_bounds__(kThreads, kBlocks) log_probs_kernel(LogProbsPa
     Segment<T> ahead = segment(min(t_next, static_cast<int64_t>(rows) - 1));
     const auto fetch = [&](int slot) {
         if (t_next < rows) {
+            const T *from = ahead.row + ahead.first(g_next + static_cast<int32_t>(threadIdx.x));
+            const bool all = ahead.inside(g_next, kStep);      // of every thread: no tests in the middle of a row
 #pragma unroll
             for (int c = 0; c < kChunk; ++c) {
                 const int32_t g = g_next + c * kThreads + static_cast<int32_t>(threadIdx.x);
-                if (g < ahead.pieces && ahead.whole(g)) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(place(slot, c)), "l"(ahead.row + ahead.first(g)) : "memory");
+                if (all || (g < ahead.pieces && ahead.whole(g)))
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(place(slot, c)), "l"(from + c * (kThreads * E)) : "memory");
             }
             g_next += kStep;
             if (g_next >= ahead.pieces) {
@@ -274,39 +279,50 @@ __global__ void __launch_bounds__(kThreads, kBlocks) log_probs_kernel(LogProbsPa
         const Segment<T> seg = segment(t);
         Stats a{kLowest, 0.f, 0.f};
         float best = -CUDART_INF_F;
-        int32_t best_at = max(seg.first(threadIdx.x), seg.begin);      // of the thread's largest logit
+        uint4 best_raw = nothing<T>();
+        int32_t best_piece = threadIdx.x;      // with the thread's largest logit, and what it holds
         for (int32_t g0 = 0; g0 < seg.pieces; g0 += kStep) {
             asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 1) : "memory");
             uint4 raw[kChunk];
-            float largest = -CUDART_INF_F;
+            const auto take = [&](int c) {
+                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(raw[c].x), "=r"(raw[c].y), "=r"(raw[c].z), "=r"(raw[c].w) : "r"(place(slot, c)) : "memory");
+            };
+            if (seg.inside(g0, kStep)) {
 #pragma unroll
-            for (int c = 0; c < kChunk; ++c) {
-                const int32_t g = g0 + c * kThreads + static_cast<int32_t>(threadIdx.x);
-                raw[c] = nothing<T>();
-                if (g < seg.pieces) {
-                    if (seg.whole(g))
-                        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(raw[c].x), "=r"(raw[c].y), "=r"(raw[c].z), "=r"(raw[c].w) : "r"(place(slot, c)) : "memory");
-                    else
-                        raw[c] = seg.load(g);
+                for (int c = 0; c < kChunk; ++c) take(c);
+            } else {
+#pragma unroll
+                for (int c = 0; c < kChunk; ++c) {
+                    const int32_t g = g0 + c * kThreads + static_cast<int32_t>(threadIdx.x);
+                    raw[c] = nothing<T>();
+                    if (g < seg.pieces) {
+                        if (seg.whole(g)) take(c);
+                        else raw[c] = seg.load(g);
+                    }
                 }
-                float x[E];
-                unpack(raw[c], x, T{});
-#pragma unroll
-                for (int i = 0; i < E; ++i) largest = fmaxf(largest, x[i]);
             }
             fetch(slot);
             if (++slot == kDepth) slot = 0;
+            float of_piece[kChunk];
+#pragma unroll
+            for (int c = 0; c < kChunk; ++c) {
+                float x[E];
+                unpack(raw[c], x, T{});
+                of_piece[c] = x[0];
+#pragma unroll
+                for (int i = 1; i < E; ++i) of_piece[c] = fmaxf(of_piece[c], x[i]);
+            }
+            float largest = of_piece[0];
+#pragma unroll
+            for (int c = 1; c < kChunk; ++c) largest = fmaxf(largest, of_piece[c]);
             if (largest > best) {
                 best = largest;
-                int32_t where = 0;
 #pragma unroll
-                for (int c = kChunk - 1; c >= 0; --c) {
-                    float x[E];
-                    unpack(raw[c], x, T{});
-#pragma unroll
-                    for (int i = E - 1; i >= 0; --i) where = x[i] == largest ? c * (kThreads * E) + i : where;
-                }
-                best_at = seg.first(g0 + static_cast<int32_t>(threadIdx.x)) + where;
+                for (int c = kChunk - 1; c >= 0; --c)
+                    if (of_piece[c] == largest) {
+                        best_raw = raw[c];
+                        best_piece = g0 + c * kThreads + static_cast<int32_t>(threadIdx.x);
+                    }
                 a.rescale(fmaxf(largest, kLowest), k);
             }
 #pragma unroll
@@ -340,8 +356,19 @@ __global__ void __launch_bounds__(kThreads, kBlocks) log_probs_kernel(LogProbsPa
         a.u = warp_join(lane < kWarps ? sh.part[2][lane] : 0.f, plus);
 
         if (p.top) {
-            if (a.s != a.s) largest_by_rounds(seg, p.top, sh);
-            else largest_of_segment(seg, static_cast<int32_t>(threadIdx.x) < seg.pieces ? order_key(best, best_at) : 0, p.top, sh);
+            if (a.s != a.s) {
+                largest_by_rounds(seg, p.top, sh);
+            } else {
+                uint64_t mine = 0;
+                if (static_cast<int32_t>(threadIdx.x) < seg.pieces) {
+                    float x[E];
+                    unpack(best_raw, x, T{});
+#pragma unroll
+                    for (int i = E - 1; i >= 0; --i)
+                        if (x[i] == best && seg.holds(seg.first(best_piece) + i)) mine = order_key(best, seg.first(best_piece) + i);
+                }
+                largest_of_segment(seg, mine, p.top, sh);
+            }
         }
         if (segs > 1) {
             asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
