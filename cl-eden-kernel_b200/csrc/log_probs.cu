@@ -1,6 +1,6 @@
 // log_probs: log probabilities of given ids, entropy and the largest alternatives of rows of logits.
 //
-// Bound by reading the logits, which happens once: with k = scale * log2(e), m the running maximum and d = k (l - m), a thread keeps
+// Bound by reading the logits, which happens once: with k = scale * log2(e), m near the running maximum and d = k (l - m), a thread keeps
 //   S = sum 2^d   and   U = sum d 2^d,
 // rescaled whenever m grows (S' = c S, U' = c (U + d S) with d = k (m - m'), c = 2^d).  Then
 //   log p = scale (l - m) - ln S,   entropy = ln S - ln 2 U / S.
@@ -28,6 +28,7 @@ constexpr int kBlocks = 3;              // CTAs an SM is to hold
 constexpr int kCandidates = 1024;
 constexpr int kLookers = 8;             // threads that look at one thread's logits again
 constexpr float kNothing = -1e4f;       // 2^-10000 is 0; keeps the products d 2^d away from infinity times 0
+constexpr float kSlack = 20.f;
 constexpr float kLowest = -3.402823466e38f;
 
 // Order of the logits as unsigned integers: NaN above +inf, -0 equal to +0; the lower index first among equals.  0 is below all keys.
@@ -61,14 +62,17 @@ struct Segment {
     static constexpr int E = 16 / sizeof(T);
     const T *row;
     int32_t begin, end, skip, pieces;
+    int32_t whole_begin, whole_end;      // the whole pieces
     __device__ __forceinline__ Segment(const T *r, int32_t b, int32_t e) : row(r), begin(b), end(e) {
         skip = static_cast<int32_t>((reinterpret_cast<uintptr_t>(r + b) & 15) / sizeof(T));
         pieces = e > b ? (e - b + skip + E - 1) / E : 0;
+        whole_begin = skip ? 1 : 0;
+        whole_end = e > b ? (e - b + skip) / E : 0;
     }
     // Pieces [g, g + n) lie in the segment as a whole.
-    __device__ __forceinline__ bool inside(int32_t g, int32_t n) const { return first(g) >= begin && first(g + n) <= end; }
+    __device__ __forceinline__ bool inside(int32_t g, int32_t n) const { return g + n <= whole_end && g >= whole_begin; }
     __device__ __forceinline__ int32_t first(int32_t g) const { return begin - skip + g * E; }
-    __device__ __forceinline__ bool whole(int32_t g) const { return first(g) >= begin && first(g) + E <= end; }
+    __device__ __forceinline__ bool whole(int32_t g) const { return g >= whole_begin && g < whole_end; }
     __device__ __forceinline__ uint4 load(int32_t g) const {
         uint4 v;
         if (whole(g)) {
@@ -253,9 +257,9 @@ __global__ void __launch_bounds__(kThreads, kBlocks) log_probs_kernel(LogProbsPa
     int64_t t_next = blockIdx.x;
     int32_t g_next = 0;
     Segment<T> ahead = segment(min(t_next, static_cast<int64_t>(rows) - 1));
+    const T *from = ahead.row + ahead.first(threadIdx.x);
     const auto fetch = [&](int slot) {
         if (t_next < rows) {
-            const T *from = ahead.row + ahead.first(g_next + static_cast<int32_t>(threadIdx.x));
             const bool all = ahead.inside(g_next, kStep);      // of every thread: no tests in the middle of a row
 #pragma unroll
             for (int c = 0; c < kChunk; ++c) {
@@ -264,10 +268,14 @@ __global__ void __launch_bounds__(kThreads, kBlocks) log_probs_kernel(LogProbsPa
                     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(place(slot, c)), "l"(from + c * (kThreads * E)) : "memory");
             }
             g_next += kStep;
+            from += kStep * E;
             if (g_next >= ahead.pieces) {
                 g_next = 0;
                 t_next += gridDim.x;
-                if (t_next < rows) ahead = segment(t_next);
+                if (t_next < rows) {
+                    ahead = segment(t_next);
+                    from = ahead.row + ahead.first(threadIdx.x);
+                }
             }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
@@ -279,8 +287,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks) log_probs_kernel(LogProbsPa
         const Segment<T> seg = segment(t);
         Stats a{kLowest, 0.f, 0.f};
         float best = -CUDART_INF_F;
-        uint4 best_raw = nothing<T>();
-        int32_t best_piece = threadIdx.x;      // with the thread's largest logit, and what it holds
+        int32_t best_piece = threadIdx.x;      // with the thread's largest logit
         for (int32_t g0 = 0; g0 < seg.pieces; g0 += kStep) {
             asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 1) : "memory");
             uint4 raw[kChunk];
@@ -318,13 +325,10 @@ __global__ void __launch_bounds__(kThreads, kBlocks) log_probs_kernel(LogProbsPa
             if (largest > best) {
                 best = largest;
 #pragma unroll
-                for (int c = kChunk - 1; c >= 0; --c)
-                    if (of_piece[c] == largest) {
-                        best_raw = raw[c];
-                        best_piece = g0 + c * kThreads + static_cast<int32_t>(threadIdx.x);
-                    }
-                a.rescale(fmaxf(largest, kLowest), k);
+                for (int c = kChunk - 1; c >= 0; --c) best_piece = of_piece[c] == largest ? g0 + c * kThreads + static_cast<int32_t>(threadIdx.x) : best_piece;
             }
+            // m stays while nothing exceeds it by more than a factor of 2^kSlack: the sums have room for that.
+            if ((largest - a.m) * k > kSlack) a.rescale(fmaxf(largest, kLowest), k);
 #pragma unroll
             for (int c = 0; c < kChunk; ++c) {
                 float x[E];
@@ -362,7 +366,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks) log_probs_kernel(LogProbsPa
                 uint64_t mine = 0;
                 if (static_cast<int32_t>(threadIdx.x) < seg.pieces) {
                     float x[E];
-                    unpack(best_raw, x, T{});
+                    unpack(seg.load(best_piece), x, T{});
 #pragma unroll
                     for (int i = E - 1; i >= 0; --i)
                         if (x[i] == best && seg.holds(seg.first(best_piece) + i)) mine = order_key(best, seg.first(best_piece) + i);
