@@ -4,8 +4,8 @@
 //   S = sum 2^d   and   U = sum d 2^d,
 // rescaled whenever m grows (S' = c S, U' = c (U + d S) with d = k (m - m'), c = 2^d).  Then
 //   log p = scale (l - m) - ln S,   entropy = ln S - ln 2 U / S.
-// The alternatives come from the same pass: a thread remembers where its largest logit was.  The n-th largest of the threads' maxima
-// bounds the n-th largest logit from below, so that what is above it lies with n threads, and their logits alone are looked at again.
+// The alternatives come from the same pass: a thread remembers where its largest logit was.  A value that n of the threads' maxima reach
+// bounds the n-th largest logit from below, so that what is above it lies with those threads, and their logits alone are looked at again.
 // A row is split over a cluster of up to eight CTAs where the rows alone do not occupy the device; the parts meet in the first CTA's
 // shared memory, without atomics or workspace.  All orders are total (value, then index), so that results do not depend on timing.
 #include <math_constants.h>
@@ -113,6 +113,50 @@ template <typename T> __device__ __forceinline__ uint4 nothing() {      // a pie
     return make_uint4(w, w, w, w);
 }
 
+// Largest and smallest of a piece; NaN is passed over.
+__device__ __forceinline__ void extremes(uint4 v, float &largest, float &smallest, float) {
+    float x[4];
+    unpack(v, x, float{});
+    largest = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+    smallest = fminf(fminf(x[0], x[1]), fminf(x[2], x[3]));
+}
+template <typename T2> __device__ __forceinline__ void extremes2(uint4 v, float &largest, float &smallest) {
+    T2 t[4];
+    __builtin_memcpy(t, &v, 16);
+    const T2 hi = __hmax2(__hmax2(t[0], t[1]), __hmax2(t[2], t[3])), lo = __hmin2(__hmin2(t[0], t[1]), __hmin2(t[2], t[3]));
+    largest = fmaxf(to_float(hi.x), to_float(hi.y));
+    smallest = fminf(to_float(lo.x), to_float(lo.y));
+}
+__device__ __forceinline__ void extremes(uint4 v, float &largest, float &smallest, __half) { extremes2<__half2>(v, largest, smallest); }
+__device__ __forceinline__ void extremes(uint4 v, float &largest, float &smallest, __nv_bfloat16) { extremes2<__nv_bfloat162>(v, largest, smallest); }
+
+// Two floats in one register pair, for the instructions that work on both.
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+    uint64_t p;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(lo), "f"(hi));
+    return p;
+}
+__device__ __forceinline__ float2 unpair(uint64_t p) {
+    float2 f;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(p));
+    return f;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+
 struct Stats {
     float m, s, u;
     __device__ __forceinline__ void rescale(float to, float k) {
@@ -123,15 +167,19 @@ struct Stats {
     }
 };
 
+__device__ __forceinline__ uint64_t warp_largest(uint64_t key) {
+    const uint32_t hi = __reduce_max_sync(0xffffffffu, static_cast<uint32_t>(key >> 32));
+    const uint32_t lo = __reduce_max_sync(0xffffffffu, static_cast<uint32_t>(key >> 32) == hi ? static_cast<uint32_t>(key) : 0u);
+    return static_cast<uint64_t>(hi) << 32 | lo;
+}
+
 // The `n` largest keys of up to 32 lists in descending order, 0 past their ends; one warp, lane i walks list i.
 __device__ __forceinline__ void take_largest(const uint64_t *lists, int n_lists, int length, int stride, int n, uint64_t *out) {
     const int lane = threadIdx.x & 31;
     int at = 0;
     uint64_t head = lane < n_lists && length ? lists[lane * stride] : 0;
     for (int i = 0; i < n; ++i) {
-        const uint32_t hi = __reduce_max_sync(0xffffffffu, static_cast<uint32_t>(head >> 32));
-        const uint32_t lo = __reduce_max_sync(0xffffffffu, static_cast<uint32_t>(head >> 32) == hi ? static_cast<uint32_t>(head) : 0u);
-        const uint64_t key = static_cast<uint64_t>(hi) << 32 | lo;
+        const uint64_t key = warp_largest(head);
         if (lane == 0) out[i] = key;
         if (key && head == key) head = ++at < length ? lists[lane * stride + at] : 0;
     }
@@ -139,8 +187,9 @@ __device__ __forceinline__ void take_largest(const uint64_t *lists, int n_lists,
 
 struct Shared {
     float part[3][kWarps];
-    uint64_t lists[kWarps][32];                 // the warps' maxima in descending order
-    uint64_t winners[kMaxTop];
+    uint64_t of_warp[kWarps];
+    int32_t n_lookups;
+    int32_t lookups[kThreads];                  // threads whose logits are looked at again
     uint64_t candidates[kCandidates];
     int32_t n_candidates;
     uint64_t sorted[kMaxTop];                   // the largest of this segment
@@ -172,9 +221,9 @@ __device__ __noinline__ void largest_by_rounds(const Segment<T> &seg, int top, S
         }
         best = warp_join(best, [](uint64_t a, uint64_t b) { return a > b ? a : b; });
         __syncthreads();
-        if (lane == 0) sh.lists[0][warp] = best;
+        if (lane == 0) sh.of_warp[warp] = best;
         __syncthreads();
-        for (int w = 0; w < kWarps; ++w) best = sh.lists[0][w] > best ? sh.lists[0][w] : best;
+        for (int w = 0; w < kWarps; ++w) best = sh.of_warp[w] > best ? sh.of_warp[w] : best;
         if (threadIdx.x == 0) sh.sorted[r] = best;
         below = best;
     }
@@ -185,28 +234,32 @@ __device__ __noinline__ void largest_by_rounds(const Segment<T> &seg, int top, S
 template <typename T>
 __device__ __forceinline__ void largest_of_segment(const Segment<T> &seg, uint64_t mine, int top, Shared &sh) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    // a warp's maxima in descending order (bitonic)
-#pragma unroll
-    for (int size = 2; size <= 32; size <<= 1)
-#pragma unroll
-        for (int by = size >> 1; by > 0; by >>= 1) {
-            const uint64_t other = __shfl_xor_sync(0xffffffffu, mine, by);
-            const bool larger = ((lane & by) == 0) == ((lane & size) == 0 || size == 32);
-            if (larger == (other > mine)) mine = other;
-        }
-    sh.lists[warp][lane] = mine;
-    if (threadIdx.x == 0) sh.n_candidates = 0;
+    // The r-th largest of every warp's maxima with r kWarps >= top: the least of them has `top` maxima at or above it.
+    uint64_t left = mine, found = 0;
+    for (int r = 0; r < top; r += kWarps) {
+        found = warp_largest(left);
+        if (left == found) left = 0;
+    }
+    if (lane == 0) sh.of_warp[warp] = found;
+    if (threadIdx.x == 0) sh.n_candidates = sh.n_lookups = 0;
     if (threadIdx.x < top) sh.sorted[threadIdx.x] = 0;
     __syncthreads();
-    if (warp == 0) take_largest(&sh.lists[0][0], kWarps, 32, 32, top, top == 1 ? sh.sorted : sh.winners);
+    uint64_t least = sh.of_warp[0];      // 0 where fewer threads than that have logits: everything counts
+#pragma unroll
+    for (int w = 1; w < kWarps; ++w) least = sh.of_warp[w] < least ? sh.of_warp[w] : least;
+    if (top == 1) {      // the largest of the maxima is the largest
+        if (mine && found == mine) {
+            bool first = true;
+            for (int w = 0; w < kWarps; ++w) first = first && sh.of_warp[w] <= mine;
+            if (first) sh.sorted[0] = mine;
+        }
+        __syncthreads();
+        return;
+    }
+    if (mine && mine >= least) sh.lookups[atomicAdd(&sh.n_lookups, 1)] = threadIdx.x;
     __syncthreads();
-    if (top == 1) return;      // the largest of the maxima is the largest
-    const uint64_t least = sh.winners[top - 1];      // 0 where fewer threads than that have logits: everything counts
-    for (int w = threadIdx.x / kLookers; w < top; w += kThreads / kLookers) {      // a few threads look at the logits of each of them
-        const uint64_t key = sh.winners[w];
-        if (!key) break;
-        const int32_t owner = ((key_index(key) - seg.begin + seg.skip) / Segment<T>::E) % kThreads;
-        for (int32_t g = owner + kThreads * static_cast<int32_t>(threadIdx.x % kLookers); g < seg.pieces; g += kThreads * kLookers) {
+    for (int w = threadIdx.x / kLookers; w < sh.n_lookups; w += kThreads / kLookers) {      // a few threads look at the logits of each of them
+        for (int32_t g = sh.lookups[w] + kThreads * static_cast<int32_t>(threadIdx.x % kLookers); g < seg.pieces; g += kThreads * kLookers) {
             float x[Segment<T>::E];
             unpack(seg.load(g), x, T{});
 #pragma unroll
@@ -310,18 +363,14 @@ __global__ void __launch_bounds__(kThreads, kBlocks) log_probs_kernel(LogProbsPa
             }
             fetch(slot);
             if (++slot == kDepth) slot = 0;
-            float of_piece[kChunk];
+            float of_piece[kChunk], largest = -CUDART_INF_F, smallest = CUDART_INF_F;
 #pragma unroll
             for (int c = 0; c < kChunk; ++c) {
-                float x[E];
-                unpack(raw[c], x, T{});
-                of_piece[c] = x[0];
-#pragma unroll
-                for (int i = 1; i < E; ++i) of_piece[c] = fmaxf(of_piece[c], x[i]);
+                float low;
+                extremes(raw[c], of_piece[c], low, T{});
+                largest = fmaxf(largest, of_piece[c]);
+                smallest = fminf(smallest, low);
             }
-            float largest = of_piece[0];
-#pragma unroll
-            for (int c = 1; c < kChunk; ++c) largest = fmaxf(largest, of_piece[c]);
             if (largest > best) {
                 best = largest;
 #pragma unroll
@@ -329,15 +378,36 @@ __global__ void __launch_bounds__(kThreads, kBlocks) log_probs_kernel(LogProbsPa
             }
             // m stays while nothing exceeds it by more than a factor of 2^kSlack: the sums have room for that.
             if ((largest - a.m) * k > kSlack) a.rescale(fmaxf(largest, kLowest), k);
+            if ((smallest - a.m) * k > kNothing) {      // nothing is ruled out: two at a time
+                const uint64_t minus_m = pair(-a.m, -a.m), k2 = pair(k, k);
+                uint64_t s2 = pair(a.s, 0.f), u2 = pair(a.u, 0.f);
 #pragma unroll
-            for (int c = 0; c < kChunk; ++c) {
-                float x[E];
-                unpack(raw[c], x, T{});
+                for (int c = 0; c < kChunk; ++c) {
+                    float x[E];
+                    unpack(raw[c], x, T{});
 #pragma unroll
-                for (int i = 0; i < E; ++i) {
-                    const float d = max_nan((x[i] - a.m) * k, kNothing), e = exp2_fast(d);
-                    a.s += e;
-                    a.u = fmaf(d, e, a.u);
+                    for (int i = 0; i < E; i += 2) {
+                        const uint64_t d2 = mul2(add2(pair(x[i], x[i + 1]), minus_m), k2);
+                        const float2 d = unpair(d2);
+                        const uint64_t e2 = pair(exp2_fast(d.x), exp2_fast(d.y));
+                        s2 = add2(s2, e2);
+                        u2 = fma2(d2, e2, u2);
+                    }
+                }
+                const float2 s = unpair(s2), u = unpair(u2);
+                a.s = s.x + s.y;
+                a.u = u.x + u.y;
+            } else {
+#pragma unroll
+                for (int c = 0; c < kChunk; ++c) {
+                    float x[E];
+                    unpack(raw[c], x, T{});
+#pragma unroll
+                    for (int i = 0; i < E; ++i) {
+                        const float d = max_nan((x[i] - a.m) * k, kNothing), e = exp2_fast(d);
+                        a.s += e;
+                        a.u = fmaf(d, e, a.u);
+                    }
                 }
             }
         }
