@@ -139,46 +139,6 @@ __device__ __forceinline__ void tile_coords(const TcParams &p, int tile, int &tg
     tg = g0 + (r - tn * gw);
 }
 
-// The k loop of one accumulator tile for the common big-GEMM shape (four K slices per k-block, one k-block per stage),
-// unrolled over the D stages of the ring: stage addresses, barrier addresses and descriptors are then loop invariants
-// held in registers, and a k-block costs the MMA thread a barrier look-up, the four MMAs, a commit and a counter.
-// The ring position carries over from tile to tile, so the unrolled sequence is entered at the current stage.
-#define ENN_KB(S)                                                                                                        \
-    {                                                                                                                    \
-        const uint32_t bar = full0 + 8 * (S);                                                                            \
-        if (!mbar_test_wait(bar, phase) && !mbar_wait_fast(bar, phase, abort_flag, err, 3)) return false;                \
-        umma_i8_run<TWO, 4>(d_tmem, desc_hi, lo0 + (S) * stage16, lo0 + (S) * stage16 + a16, idesc, acc);                \
-        acc = 1;                                                                                                         \
-        if (TWO) umma_commit_pair(empty0 + 8 * (S));                                                                     \
-        else umma_commit(empty0 + 8 * (S));                                                                              \
-        if (--n == 0) {                                                                                                  \
-            stage = (S) + 1;                                                                                             \
-            break;                                                                                                       \
-        }                                                                                                                \
-    }
-#define ENN_TILE_FN(NAME, D, CASES)                                                                                      \
-    template <bool TWO>                                                                                                  \
-    __device__ __forceinline__ bool NAME(uint32_t d_tmem, int n, uint32_t &stage, uint32_t &phase, uint32_t full0,       \
-                                         uint32_t empty0, uint32_t desc_hi, uint32_t lo0, uint32_t stage16, uint32_t a16, \
-                                         uint32_t idesc, volatile int *abort_flag, int32_t *err) {                      \
-        uint32_t acc = 0;                                                                                                \
-        for (;;) {                                                                                                       \
-            switch (stage) { CASES }                                                                                     \
-            if (n == 0) break;                                                                                           \
-            stage = 0;                                                                                                   \
-            phase ^= 1;                                                                                                  \
-        }                                                                                                                \
-        if (stage == (D)) {                                                                                              \
-            stage = 0;                                                                                                   \
-            phase ^= 1;                                                                                                  \
-        }                                                                                                                \
-        return true;                                                                                                     \
-    }
-ENN_TILE_FN(mma_tile_d4, 4, case 0: ENN_KB(0) case 1: ENN_KB(1) case 2: ENN_KB(2) case 3: ENN_KB(3))
-ENN_TILE_FN(mma_tile_d6, 6, case 0: ENN_KB(0) case 1: ENN_KB(1) case 2: ENN_KB(2) case 3: ENN_KB(3) case 4: ENN_KB(4) case 5: ENN_KB(5))
-#undef ENN_TILE_FN
-#undef ENN_KB
-
 // TWO: CTA-pair mode (launched as clusters of 2; plain GEMM operands only, group == 1, kpack == 1): the pair owns M
 // tiles 2t and 2t + 1 of one N tile, every B byte is read from L2 once per pair, and a stage per CTA is A plus half of B.
 template <bool ASUM, int MODE, bool TWO, bool FADD = false>

@@ -113,22 +113,30 @@ template <typename T> __device__ __forceinline__ uint4 nothing() {      // a pie
     return make_uint4(w, w, w, w);
 }
 
-// Largest and smallest of a piece; NaN is passed over.
-__device__ __forceinline__ void extremes(uint4 v, float &largest, float &smallest, float) {
-    float x[4];
-    unpack(v, x, float{});
-    largest = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
-    smallest = fminf(fminf(x[0], x[1]), fminf(x[2], x[3]));
+// Largest of a few pieces; NaN is passed over.
+template <int N> __device__ __forceinline__ float largest_of(const uint4 (&v)[N], float) {
+    float m = -CUDART_INF_F;
+#pragma unroll
+    for (int c = 0; c < N; ++c) {
+        float x[4];
+        unpack(v[c], x, float{});
+        m = fmaxf(m, fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])));
+    }
+    return m;
 }
-template <typename T2> __device__ __forceinline__ void extremes2(uint4 v, float &largest, float &smallest) {
-    T2 t[4];
-    __builtin_memcpy(t, &v, 16);
-    const T2 hi = __hmax2(__hmax2(t[0], t[1]), __hmax2(t[2], t[3])), lo = __hmin2(__hmin2(t[0], t[1]), __hmin2(t[2], t[3]));
-    largest = fmaxf(to_float(hi.x), to_float(hi.y));
-    smallest = fminf(to_float(lo.x), to_float(lo.y));
+template <typename T2, int N> __device__ __forceinline__ float largest_of2(const uint4 (&v)[N]) {
+    T2 m;
+#pragma unroll
+    for (int c = 0; c < N; ++c) {
+        T2 t[4];
+        __builtin_memcpy(t, &v[c], 16);
+        const T2 of = __hmax2(__hmax2(t[0], t[1]), __hmax2(t[2], t[3]));
+        m = c ? __hmax2(m, of) : of;
+    }
+    return fmaxf(to_float(m.x), to_float(m.y));
 }
-__device__ __forceinline__ void extremes(uint4 v, float &largest, float &smallest, __half) { extremes2<__half2>(v, largest, smallest); }
-__device__ __forceinline__ void extremes(uint4 v, float &largest, float &smallest, __nv_bfloat16) { extremes2<__nv_bfloat162>(v, largest, smallest); }
+template <int N> __device__ __forceinline__ float largest_of(const uint4 (&v)[N], __half) { return largest_of2<__half2>(v); }
+template <int N> __device__ __forceinline__ float largest_of(const uint4 (&v)[N], __nv_bfloat16) { return largest_of2<__nv_bfloat162>(v); }
 
 // Two floats in one register pair, for the instructions that work on both.
 __device__ __forceinline__ uint64_t pair(float lo, float hi) {
@@ -188,6 +196,7 @@ __device__ __forceinline__ void take_largest(const uint64_t *lists, int n_lists,
 struct Shared {
     float part[3][kWarps];
     uint64_t of_warp[kWarps];
+    uint64_t firsts[kWarps * (kMaxTop / kWarps + 2)], bound;
     int32_t n_lookups;
     int32_t lookups[kThreads];                  // threads whose logits are looked at again
     uint64_t candidates[kCandidates];
@@ -230,54 +239,88 @@ __device__ __noinline__ void largest_by_rounds(const Segment<T> &seg, int top, S
     __syncthreads();
 }
 
-// sh.sorted[0 .. top): the largest keys of the segment.  `mine`: the key of the thread's largest logit, 0 if it has none.
+// The logits of the threads whose maximum reaches `least`, as far as they reach it themselves, into sh.candidates.  `mine`: a key of the
+// thread's maximum.  Returns their number, which may be above what there is room for.
 template <typename T>
-__device__ __forceinline__ void largest_of_segment(const Segment<T> &seg, uint64_t mine, int top, Shared &sh) {
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    // The r-th largest of every warp's maxima with r kWarps >= top: the least of them has `top` maxima at or above it.
-    uint64_t left = mine, found = 0;
-    for (int r = 0; r < top; r += kWarps) {
-        found = warp_largest(left);
-        if (left == found) left = 0;
-    }
-    if (lane == 0) sh.of_warp[warp] = found;
+__device__ __forceinline__ int collect(const Segment<T> &seg, uint64_t mine, uint64_t least, Shared &sh) {
     if (threadIdx.x == 0) sh.n_candidates = sh.n_lookups = 0;
-    if (threadIdx.x < top) sh.sorted[threadIdx.x] = 0;
     __syncthreads();
-    uint64_t least = sh.of_warp[0];      // 0 where fewer threads than that have logits: everything counts
-#pragma unroll
-    for (int w = 1; w < kWarps; ++w) least = sh.of_warp[w] < least ? sh.of_warp[w] : least;
-    if (top == 1) {      // the largest of the maxima is the largest
-        if (mine && found == mine) {
-            bool first = true;
-            for (int w = 0; w < kWarps; ++w) first = first && sh.of_warp[w] <= mine;
-            if (first) sh.sorted[0] = mine;
-        }
-        __syncthreads();
-        return;
-    }
     if (mine && mine >= least) sh.lookups[atomicAdd(&sh.n_lookups, 1)] = threadIdx.x;
     __syncthreads();
-    for (int w = threadIdx.x / kLookers; w < sh.n_lookups; w += kThreads / kLookers) {      // a few threads look at the logits of each of them
+    const float reach = least ? key_value(least) : -CUDART_INF_F;
+    const int n = sh.n_lookups;
+    for (int w = threadIdx.x / kLookers; w < n; w += kThreads / kLookers)      // a few threads look at the logits of each of them
         for (int32_t g = sh.lookups[w] + kThreads * static_cast<int32_t>(threadIdx.x % kLookers); g < seg.pieces; g += kThreads * kLookers) {
             float x[Segment<T>::E];
             unpack(seg.load(g), x, T{});
 #pragma unroll
-            for (int i = 0; i < Segment<T>::E; ++i) {
-                const uint64_t k = seg.key(g, i, x[i]);
-                if (k && k >= least) {
-                    const int32_t slot = atomicAdd(&sh.n_candidates, 1);
-                    if (slot < kCandidates) sh.candidates[slot] = k;
+            for (int i = 0; i < Segment<T>::E; ++i)
+                if (x[i] >= reach) {
+                    const uint64_t k = seg.key(g, i, x[i]);
+                    if (k && k >= least) {
+                        const int32_t slot = atomicAdd(&sh.n_candidates, 1);
+                        if (slot < kCandidates) sh.candidates[slot] = k;
+                    }
                 }
-            }
+        }
+    __syncthreads();
+    return sh.n_candidates;
+}
+
+// A key that `top` of the keys `mine` of the threads reach, 0 if fewer of them have one: the top-th largest among the first few of every
+// warp, two more than would do, so that hardly more threads than `top` reach it.
+__device__ __forceinline__ uint64_t reached_by(uint64_t mine, int top, Shared &sh) {
+    const int rounds = min(top, (top + kWarps - 1) / kWarps + 2), n = rounds * kWarps;
+    __syncthreads();
+    for (int r = 0; r < rounds; ++r) {
+        const uint64_t found = warp_largest(mine);
+        const uint32_t holders = __ballot_sync(0xffffffffu, mine == found);
+        if (static_cast<int>(threadIdx.x & 31) == __ffs(holders) - 1) {      // equal ones one after the other
+            sh.firsts[r * kWarps + (threadIdx.x >> 5)] = found;
+            mine = 0;
         }
     }
     __syncthreads();
-    const int n = sh.n_candidates;
-    if (n > kCandidates) {
-        largest_by_rounds(seg, top, sh);
-        return;
+    if (static_cast<int>(threadIdx.x) < n) {
+        const uint64_t k = sh.firsts[threadIdx.x];
+        int place = 0;
+        for (int j = 0; j < n; ++j) {
+            const uint64_t other = sh.firsts[j];
+            place += other > k || (other == k && j < static_cast<int>(threadIdx.x));
+        }
+        if (place == top - 1) sh.bound = k;
     }
+    __syncthreads();
+    return sh.bound;
+}
+
+// sh.sorted[0 .. top): the largest keys of a segment without NaN.  `best`: the thread's largest logit.
+template <typename T>
+__device__ __forceinline__ void largest_of_segment(const Segment<T> &seg, float best, int top, Shared &sh) {
+    const bool has = static_cast<int32_t>(threadIdx.x) < seg.pieces;
+    // By value first: all that equal the bound are candidates.
+    uint64_t mine = has ? order_key(best, -1) : 0;
+    uint64_t least = reached_by(mine, top, sh);
+    int n = collect(seg, mine, least & 0xffffffff00000000ull, sh);
+    if (n > kCandidates) {
+        // Many equal logits (a vocabulary with few left and the others at one value): the threads' maxima with their indexes.
+        mine = 0;
+        for (int32_t g = threadIdx.x; g < seg.pieces && !mine; g += kThreads) {
+            float x[Segment<T>::E];
+            unpack(seg.load(g), x, T{});
+#pragma unroll
+            for (int i = Segment<T>::E - 1; i >= 0; --i)
+                if (x[i] == best && seg.holds(seg.first(g) + i)) mine = order_key(best, seg.first(g) + i);
+        }
+        least = reached_by(mine, top, sh);
+        n = collect(seg, mine, least, sh);
+        if (n > kCandidates) {
+            largest_by_rounds(seg, top, sh);
+            return;
+        }
+    }
+    if (threadIdx.x < top) sh.sorted[threadIdx.x] = 0;
+    __syncthreads();
     for (int i = threadIdx.x; i < n; i += kThreads) {      // its place is the number of larger ones
         const uint64_t k = sh.candidates[i];
         int place = 0;
@@ -302,7 +345,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks) log_probs_kernel(LogProbsPa
     const auto segment = [&](int64_t t) { return Segment<T>(logits + t * p.pitch, rank * seg_size, min(p.vocab, (rank + 1) * seg_size)); };
     const float k = p.scale * 1.4426950408889634f;
     const uint32_t mine0 = smem_u32(ring) + threadIdx.x * 16;
-    const auto place = [&](int slot, int c) { return mine0 + static_cast<uint32_t>(slot * kChunk + c) * (kThreads * 16); };
+    constexpr uint32_t kPiece = kThreads * 16, kSlot = kChunk * kPiece;      // bytes from piece to piece of a thread, from chunk to chunk
     pdl_wait();
     pdl_trigger();
 
@@ -311,14 +354,16 @@ __global__ void __launch_bounds__(kThreads, kBlocks) log_probs_kernel(LogProbsPa
     int32_t g_next = 0;
     Segment<T> ahead = segment(min(t_next, static_cast<int64_t>(rows) - 1));
     const T *from = ahead.row + ahead.first(threadIdx.x);
-    const auto fetch = [&](int slot) {
+    const auto fetch = [&](uint32_t at) {
+        const auto copy = [&](int c) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at + c * kPiece), "l"(from + c * (kThreads * E)) : "memory"); };
         if (t_next < rows) {
-            const bool all = ahead.inside(g_next, kStep);      // of every thread: no tests in the middle of a row
+            if (ahead.inside(g_next, kStep)) {      // of every thread: no tests in the middle of a row
 #pragma unroll
-            for (int c = 0; c < kChunk; ++c) {
-                const int32_t g = g_next + c * kThreads + static_cast<int32_t>(threadIdx.x);
-                if (all || (g < ahead.pieces && ahead.whole(g)))
-                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(place(slot, c)), "l"(from + c * (kThreads * E)) : "memory");
+                for (int c = 0; c < kChunk; ++c) copy(c);
+            } else {
+#pragma unroll
+                for (int c = 0; c < kChunk; ++c)
+                    if (ahead.whole(g_next + c * kThreads + static_cast<int32_t>(threadIdx.x))) copy(c);
             }
             g_next += kStep;
             from += kStep * E;
@@ -333,19 +378,19 @@ __global__ void __launch_bounds__(kThreads, kBlocks) log_probs_kernel(LogProbsPa
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    for (int s = 0; s < kDepth; ++s) fetch(s);
-    int slot = 0;
+    for (int s = 0; s < kDepth; ++s) fetch(mine0 + s * kSlot);
+    uint32_t at = mine0;      // the chunk that is worked on
+    bool careful = false;
 
     for (int64_t t = blockIdx.x; t < rows; t += gridDim.x) {
         const Segment<T> seg = segment(t);
         Stats a{kLowest, 0.f, 0.f};
         float best = -CUDART_INF_F;
-        int32_t best_piece = threadIdx.x;      // with the thread's largest logit
         for (int32_t g0 = 0; g0 < seg.pieces; g0 += kStep) {
             asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 1) : "memory");
             uint4 raw[kChunk];
             const auto take = [&](int c) {
-                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(raw[c].x), "=r"(raw[c].y), "=r"(raw[c].z), "=r"(raw[c].w) : "r"(place(slot, c)) : "memory");
+                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(raw[c].x), "=r"(raw[c].y), "=r"(raw[c].z), "=r"(raw[c].w) : "r"(at + c * kPiece) : "memory");
             };
             if (seg.inside(g0, kStep)) {
 #pragma unroll
@@ -355,31 +400,20 @@ __global__ void __launch_bounds__(kThreads, kBlocks) log_probs_kernel(LogProbsPa
                 for (int c = 0; c < kChunk; ++c) {
                     const int32_t g = g0 + c * kThreads + static_cast<int32_t>(threadIdx.x);
                     raw[c] = nothing<T>();
-                    if (g < seg.pieces) {
-                        if (seg.whole(g)) take(c);
-                        else raw[c] = seg.load(g);
-                    }
+                    if (seg.whole(g)) take(c);
+                    else if (g < seg.pieces) raw[c] = seg.load(g);
                 }
             }
-            fetch(slot);
-            if (++slot == kDepth) slot = 0;
-            float of_piece[kChunk], largest = -CUDART_INF_F, smallest = CUDART_INF_F;
-#pragma unroll
-            for (int c = 0; c < kChunk; ++c) {
-                float low;
-                extremes(raw[c], of_piece[c], low, T{});
-                largest = fmaxf(largest, of_piece[c]);
-                smallest = fminf(smallest, low);
-            }
-            if (largest > best) {
-                best = largest;
-#pragma unroll
-                for (int c = kChunk - 1; c >= 0; --c) best_piece = of_piece[c] == largest ? g0 + c * kThreads + static_cast<int32_t>(threadIdx.x) : best_piece;
-            }
+            fetch(at);
+            at = at == mine0 + (kDepth - 1) * kSlot ? mine0 : at + kSlot;
+            const float largest = largest_of(raw, T{});
+            best = fmaxf(best, largest);
             // m stays while nothing exceeds it by more than a factor of 2^kSlack: the sums have room for that.
             if ((largest - a.m) * k > kSlack) a.rescale(fmaxf(largest, kLowest), k);
-            if ((smallest - a.m) * k > kNothing) {      // nothing is ruled out: two at a time
-                const uint64_t minus_m = pair(-a.m, -a.m), k2 = pair(k, k);
+            // Two at a time.  What is ruled out makes 0 times -inf of d 2^d, seen in U: the chunk is then done again with care, as are those
+            // after it (a vocabulary is ruled out all over).
+            const uint64_t minus_m = pair(-a.m, -a.m), k2 = pair(k, k);
+            const auto sum = [&](auto limit) {
                 uint64_t s2 = pair(a.s, 0.f), u2 = pair(a.u, 0.f);
 #pragma unroll
                 for (int c = 0; c < kChunk; ++c) {
@@ -387,7 +421,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks) log_probs_kernel(LogProbsPa
                     unpack(raw[c], x, T{});
 #pragma unroll
                     for (int i = 0; i < E; i += 2) {
-                        const uint64_t d2 = mul2(add2(pair(x[i], x[i + 1]), minus_m), k2);
+                        const uint64_t d2 = limit(mul2(add2(pair(x[i], x[i + 1]), minus_m), k2));
                         const float2 d = unpair(d2);
                         const uint64_t e2 = pair(exp2_fast(d.x), exp2_fast(d.y));
                         s2 = add2(s2, e2);
@@ -395,21 +429,20 @@ __global__ void __launch_bounds__(kThreads, kBlocks) log_probs_kernel(LogProbsPa
                     }
                 }
                 const float2 s = unpair(s2), u = unpair(u2);
-                a.s = s.x + s.y;
-                a.u = u.x + u.y;
-            } else {
-#pragma unroll
-                for (int c = 0; c < kChunk; ++c) {
-                    float x[E];
-                    unpack(raw[c], x, T{});
-#pragma unroll
-                    for (int i = 0; i < E; ++i) {
-                        const float d = max_nan((x[i] - a.m) * k, kNothing), e = exp2_fast(d);
-                        a.s += e;
-                        a.u = fmaf(d, e, a.u);
-                    }
-                }
+                return make_float2(s.x + s.y, u.x + u.y);
+            };
+            float2 su;
+            if (!careful) {
+                su = sum([](uint64_t d2) { return d2; });
+                careful = su.y != su.y;
             }
+            if (careful)
+                su = sum([](uint64_t d2) {
+                    const float2 d = unpair(d2);
+                    return pair(max_nan(d.x, kNothing), max_nan(d.y, kNothing));
+                });
+            a.s = su.x;
+            a.u = su.y;
         }
 
         // The statistics of the segment, the same in every thread.
@@ -433,15 +466,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks) log_probs_kernel(LogProbsPa
             if (a.s != a.s) {
                 largest_by_rounds(seg, p.top, sh);
             } else {
-                uint64_t mine = 0;
-                if (static_cast<int32_t>(threadIdx.x) < seg.pieces) {
-                    float x[E];
-                    unpack(seg.load(best_piece), x, T{});
-#pragma unroll
-                    for (int i = E - 1; i >= 0; --i)
-                        if (x[i] == best && seg.holds(seg.first(best_piece) + i)) mine = order_key(best, seg.first(best_piece) + i);
-                }
-                largest_of_segment(seg, mine, p.top, sh);
+                largest_of_segment(seg, best, p.top, sh);
             }
         }
         if (segs > 1) {

@@ -69,7 +69,7 @@ __global__ void __launch_bounds__(kDirectThreads) token_fc_direct_kernel(TokenFc
 //   all              add the partial sums, scale and store
 constexpr int kChannels = kBM;
 constexpr int kTcThreads = 192;
-constexpr int kMaxTokens = kMaxBN;
+constexpr int kMaxTokens = kMaxBN;      // of a tile of a pair; 128 of a single CTA
 constexpr int kMaxSplits = 8;       // portable cluster size
 constexpr int kMaxStages = 12;
 
@@ -234,62 +234,271 @@ __global__ void __launch_bounds__(kTcThreads) token_fc_kernel(const __grid_const
     }
 }
 
+// ---- tensor-core kernel for large products: persistent pairs of CTAs (cta_group::2), 256 channels x bn tokens per tile.
+// A CTA of the pair holds 128 channels of the weights and half of the tokens of every k-block, so that each operand byte comes from L2 once
+// per pair, and the accumulators of its 128 channels.  Two accumulators of up to 256 columns take all of tensor memory: one is multiplied
+// into while the other is scaled and stored.  A thread of the epilogue has one channel, whose scale and bias stay in registers; a
+// warp stores 32 neighbouring channels of a token, whole sectors whatever n and the address are.
+//   warp 0, 1        as above, of both CTAs; warp 1 is the issuer in the first CTA and allocates in both
+//   warps 2 .. 9     epilogue: lane quarter warp & 3, every other group of 32 tokens
+//   warp 10          copies the token tiles
+constexpr int kPairStages = 6;
+constexpr int kPairEpiWarps = 8;
+constexpr int kPairThreads = (kPairEpiWarps + 3) * 32;
+constexpr int kPairStageBytes = (kBM + kMaxBN / 2) * kBK;
+
+struct PairCall {
+    int32_t rows, n, kb_total;
+    int32_t tiles_c, tiles_t, bn;       // channel tiles of 256, token tiles of bn
+    int32_t band;                       // channel tiles that are walked together: their operands stay in L2
+    uint32_t idesc;
+    const float *token_scale, *channel_scale, *bias;
+    int32_t *err;
+    int32_t starve;
+};
+
+__device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t (&r)[32]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, "
+                 "%23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]),
+                   "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]),
+                   "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+                 : "r"(addr));
+}
+
+// Tile number -> channel tile and token tile: bands of channel tiles, the channel tile running fastest within a band.
+__device__ __forceinline__ void pair_tile(const PairCall &p, int tile, int &tc, int &tt) {
+    const int per = p.band * p.tiles_t, b = tile / per, r = tile - b * per, width = min(p.band, p.tiles_c - b * p.band);
+    tt = r / width;
+    tc = b * p.band + (r - tt * width);
+}
+
+template <typename O>
+__global__ void __launch_bounds__(kPairThreads, 1) token_fc_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_q, const PairCall p,
+                                                                         O *out) {
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ uint64_t bars[2 * kPairStages + 4];
+    __shared__ uint32_t tmem_slot;
+    __shared__ int abort_word;
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+    volatile int *abort_flag = &abort_word;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_ctarank();
+    const uint32_t full0 = smem_u32(bars), empty0 = full0 + 8 * kPairStages, tfull0 = empty0 + 8 * kPairStages, tempty0 = tfull0 + 16;
+    const uint32_t ring = smem_u32(smem), w_bytes = kBM * kBK, q_bytes = static_cast<uint32_t>(p.bn / 2) * kBK;
+    const int first = static_cast<int>(blockIdx.x >> 1), step = static_cast<int>(gridDim.x >> 1), total = p.tiles_c * p.tiles_t;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kPairStages; ++s) {
+            mbar_init(full0 + 8 * s, 2);        // an expect-tx arrival of either producer of the first CTA
+            mbar_init(empty0 + 8 * s, 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(tfull0 + 8 * b, 1);
+            mbar_init(tempty0 + 8 * b, 2 * kPairEpiWarps);
+        }
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) tmem_alloc_pair(smem_u32(&tmem_slot), 512);
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync_all();                         // the peer's barriers exist before anything signals them
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot;
+    pdl_trigger();
+
+    // A role that gives up stops its own CTA and the peer.
+    const auto give_up = [&] { asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(mapa_rank(smem_u32(&abort_word), rank ^ 1)), "r"(1) : "memory"); };
+    uint32_t stage = 0, phase = 0;
+    if (warp == 0 || warp == kPairEpiWarps + 2) {
+        // Two lanes take the k-blocks in turn (a thread issues a tensor copy in about the time a k-block is multiplied); a stage keeps its lane.
+        if (lane < 2 && !p.starve) {
+            const bool is_w = warp == 0;
+            if (!is_w) pdl_wait();
+            const CUtensorMap *map = is_w ? &map_w : &map_q;
+            const uint32_t bytes = is_w ? w_bytes : q_bytes, dst = ring + (is_w ? 0 : w_bytes);
+            const int tiles = first < total ? (total - first + step - 1) / step : 0;
+            int t = 0, t_row = -1, kb = lane, row = 0;
+            stage = lane;
+            while (kb >= p.kb_total) { kb -= p.kb_total; ++t; }
+            while (t < tiles) {
+                if (t != t_row) {
+                    t_row = t;
+                    int tc, tt;
+                    pair_tile(p, first + t * step, tc, tt);
+                    row = is_w ? (tc * 2 + static_cast<int>(rank)) * kBM : tt * p.bn + static_cast<int>(rank) * (p.bn / 2);
+                }
+                if (!mbar_test_wait(empty0 + 8 * stage, phase ^ 1) && !mbar_wait_fast(empty0 + 8 * stage, phase ^ 1, abort_flag, p.err, 1)) {
+                    give_up();
+                    break;
+                }
+                if (rank == 0) mbar_expect_tx(full0 + 8 * stage, 2 * bytes);      // of both CTAs; every copy reports to the first
+                tma_load_2d_pair(dst + stage * kPairStageBytes, map, mapa_rank(full0 + 8 * stage, 0), kb * kBK, row);
+                stage += 2;
+                if (stage >= kPairStages) { stage -= kPairStages; phase ^= 1; }
+                kb += 2;
+                while (kb >= p.kb_total) { kb -= p.kb_total; ++t; }
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0 && rank == 0) {
+            const uint32_t desc_hi = static_cast<uint32_t>(make_smem_desc(0) >> 32);
+            int it = 0;
+            for (int tile = first; tile < total; tile += step, ++it) {
+                const uint32_t ab = it & 1, use = it >> 1;
+                if (!mbar_wait_fast(tempty0 + 8 * ab, (use & 1) ^ 1, abort_flag, p.err, 2)) { give_up(); break; }
+                asm volatile("fence.acq_rel.cluster;" ::: "memory");      // half of the arrivals came from the peer
+                tc_fence_after();
+                if (p.starve) {      // self-test: nothing was copied, so that this wait runs out
+                    mbar_wait_fast(full0, 0, abort_flag, p.err, 3, 64u);
+                    give_up();
+                    break;
+                }
+                if (!mma_tile_d6<true>(tmem + ab * kMaxBN, p.kb_total, stage, phase, full0, empty0, desc_hi, ring >> 4, kPairStageBytes >> 4, w_bytes >> 4, p.idesc, abort_flag,
+                                       p.err)) {
+                    give_up();
+                    break;
+                }
+                umma_commit_pair(tfull0 + 8 * ab);
+            }
+        }
+    } else {
+        const int q = warp & 3, half = (warp - 2) >> 2;
+        pdl_wait();
+        int it = 0;
+        for (int tile = first; tile < total; tile += step, ++it) {
+            int tc, tt;
+            pair_tile(p, tile, tc, tt);
+            const uint32_t ab = it & 1, use = it >> 1;
+            const int n = (tc * 2 + static_cast<int>(rank)) * kBM + q * 32 + lane;
+            const bool live = n < p.n;
+            const float cs = live ? p.channel_scale[n] : 0.f, b = live && p.bias ? p.bias[n] : 0.f;
+            if (!mbar_wait(tfull0 + 8 * ab, use & 1, abort_flag, p.err, 4)) {
+                if (lane == 0) give_up();
+                break;
+            }
+            tc_fence_after();
+            const uint32_t t_row = tmem + ab * kMaxBN + (static_cast<uint32_t>(q * 32) << 16);
+            for (int c = half * 32; c < p.bn; c += 64) {
+                const int64_t m = static_cast<int64_t>(tt) * p.bn + c;
+                if (m >= p.rows) break;
+                const int tokens = static_cast<int>(min(static_cast<int64_t>(min(32, p.bn - c)), p.rows - m));
+                uint32_t r[32];
+                tmem_ld32(t_row + c, r);
+                const float ts = lane < tokens ? p.token_scale[m + lane] : 0.f;
+                O *o = out + m * p.n + n;
+                tmem_ld_wait();
+#pragma unroll
+                for (int j = 0; j < 32; ++j) {
+                    const float s = __shfl_sync(0xffffffffu, ts, j);
+                    if (live && j < tokens) *o = from_float<O>(scaled(static_cast<int32_t>(r[j]), s, cs, b));
+                    o += p.n;
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(mapa_rank(tempty0 + 8 * ab, 0));
+        }
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    // No copy may land in memory that is given back (a pair's copies report to the first CTA).
+    if (*abort_flag && rank == 0 && (warp == 0 || warp == kPairEpiWarps + 2) && lane < 2 && !p.starve) drain_stages(full0, kPairStages, stage, phase, lane, 2);
+    __syncwarp();
+    cluster_sync_all();                         // no signal may reach a CTA that has left
+    tc_fence_after();
+    if (warp == 1) tmem_dealloc_pair(tmem, 512);
+}
+
 template <typename O>
 cudaError_t kernel_init(int device) {
     static PerDeviceInit once;
-    return once.run(device, [] { return cudaFuncSetAttribute(token_fc_kernel<O>, cudaFuncAttributeMaxDynamicSharedMemorySize, 226 * 1024); });
+    return once.run(device, [] {
+        const cudaError_t e = cudaFuncSetAttribute(token_fc_kernel<O>, cudaFuncAttributeMaxDynamicSharedMemorySize, 226 * 1024);
+        return e != cudaSuccess ? e : cudaFuncSetAttribute(token_fc_pair_kernel<O>, cudaFuncAttributeMaxDynamicSharedMemorySize, 226 * 1024);
+    });
 }
 
 constexpr uint32_t kSignedBytes = (2u << 4) | (1u << 7) | (1u << 10);      // s32 sums of s8 x s8
+
+template <typename K, typename... Args>
+cudaError_t launch_clusters(K kernel, unsigned grid, unsigned threads, size_t smem, unsigned cluster, cudaStream_t stream, const Args &...args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2] = {};
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+// Token tiles of at most `most` tokens, as even as multiples of `unit` allow.
+void token_tiles(int32_t rows, int32_t most, int32_t unit, int32_t *tiles, int32_t *bn) {
+    *tiles = (rows + most - 1) / most;
+    *bn = ((rows + *tiles - 1) / *tiles + unit - 1) / unit * unit;
+}
 
 template <typename O>
 cudaError_t launch_tc(enn_b200_op *op, int32_t rows, const void *const *ins, void *const *outs) {
     TokenState &t = *op->token;
     enn_b200_context *ctx = op->ctx;
+    const TokenFcParams &f = t.fc;
+    const cudaError_t e = kernel_init<O>(ctx->device);
+    if (e != cudaSuccess) return e;
+    const int32_t kb_total = (f.k + kBK - 1) / kBK;
+    const float *token_scale = static_cast<const float *>(ins[1]);
+    O *out = static_cast<O *>(outs[0]);
+    const int32_t starve = t.fc.starve_next;
+    t.fc.starve_next = false;
+    CUtensorMap map_q;
+    const auto encode = [&](int32_t box) {
+        return encode_2d(ctx, &map_q, ins[0], static_cast<uint64_t>(f.k), static_cast<uint64_t>(rows), static_cast<uint64_t>(f.in_pitch), kBK, static_cast<uint32_t>(box));
+    };
+    const int pairs = ctx->launch_sms() / 2;
+
+    // Large products: pairs of CTAs, once their tiles occupy most of the device.
+    PairCall c2{};
+    token_tiles(rows, kMaxTokens, 32, &c2.tiles_t, &c2.bn);
+    c2.tiles_c = (f.n + 2 * kBM - 1) / (2 * kBM);
+    const int64_t tiles2 = static_cast<int64_t>(c2.tiles_c) * c2.tiles_t;
+    if (rows > 128 && pairs > 0 && tiles2 * 4 >= pairs * 3) {
+        c2.rows = rows; c2.n = f.n; c2.kb_total = kb_total;
+        c2.band = std::min(8, c2.tiles_c);
+        c2.idesc = kSignedBytes | (static_cast<uint32_t>(c2.bn >> 3) << 17) | (static_cast<uint32_t>(2 * kBM >> 4) << 24);
+        c2.token_scale = token_scale; c2.channel_scale = f.channel_scale; c2.bias = f.bias;
+        c2.err = f.err_dev; c2.starve = starve;
+        if (!encode(c2.bn / 2)) return cudaErrorInvalidValue;
+        return launch_clusters(token_fc_pair_kernel<O>, static_cast<unsigned>(2 * std::min<int64_t>(tiles2, pairs)), kPairThreads, 1024 + kPairStages * kPairStageBytes, 2, ctx->stream,
+                               f.map_w, map_q, c2, out);
+    }
+
+    // Two CTAs share an SM: while one waits for its first tiles or stores its results, the other keeps the SM busy.
     TcCall c{};
-    c.rows = rows;
-    c.n = t.fc.n;
-    c.kb_total = (t.fc.k + kBK - 1) / kBK;
-    c.m_tiles = (rows + kMaxTokens - 1) / kMaxTokens;
-    c.bn = ((rows + c.m_tiles - 1) / c.m_tiles + 15) / 16 * 16;
-    const int64_t n_tiles = (t.fc.n + kChannels - 1) / kChannels, tiles = n_tiles * c.m_tiles;
-    // Two CTAs share an SM while their rings fit (up to 128 tokens).
-    const int per_sm = c.bn <= 128 ? 2 : 1;
-    const int slots = per_sm * ctx->launch_sms();
+    c.rows = rows; c.n = f.n; c.kb_total = kb_total;
+    token_tiles(rows, 128, 16, &c.m_tiles, &c.bn);
+    const int64_t tiles = static_cast<int64_t>((f.n + kChannels - 1) / kChannels) * c.m_tiles;
     c.splits = 1;
-    while (c.splits < kMaxSplits && tiles * c.splits * 2 <= slots && c.kb_total >= 4 * c.splits) c.splits *= 2;
-    const int stage_bytes = (kChannels + c.bn) * kBK, budget = (per_sm == 2 ? 111 : 222) * 1024;
-    c.stages = std::min({budget / stage_bytes, (c.kb_total + c.splits - 1) / c.splits, kMaxStages});
+    while (c.splits < kMaxSplits && tiles * c.splits * 2 <= 2 * ctx->launch_sms() && kb_total >= 4 * c.splits) c.splits *= 2;
+    const int stage_bytes = (kChannels + c.bn) * kBK;
+    c.stages = std::min({111 * 1024 / stage_bytes, (kb_total + c.splits - 1) / c.splits, kMaxStages});
     const size_t smem = 1024 + static_cast<size_t>(std::max(c.stages * stage_bytes, c.bn * kChannels * 4));
     c.tmem_cols = 32;
     while (c.tmem_cols < static_cast<uint32_t>(c.bn)) c.tmem_cols *= 2;
     c.idesc = kSignedBytes | (static_cast<uint32_t>(c.bn >> 3) << 17) | (static_cast<uint32_t>(kChannels >> 4) << 24);
-    c.token_scale = static_cast<const float *>(ins[1]);
-    c.channel_scale = t.fc.channel_scale;
-    c.bias = t.fc.bias;
-    c.err = t.fc.err_dev;
-    c.starve = t.fc.starve_next;
-    t.fc.starve_next = false;
-    c.vec = t.fc.n % 4 == 0 && reinterpret_cast<uintptr_t>(outs[0]) % (4 * sizeof(O)) == 0;
-    CUtensorMap map_q;
-    if (!encode_2d(ctx, &map_q, ins[0], static_cast<uint64_t>(t.fc.k), static_cast<uint64_t>(rows), static_cast<uint64_t>(t.fc.in_pitch), kBK, static_cast<uint32_t>(c.bn)))
-        return cudaErrorInvalidValue;
-    const cudaError_t e = kernel_init<O>(ctx->device);
-    if (e != cudaSuccess) return e;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(static_cast<unsigned>(tiles * c.splits));
-    cfg.blockDim = dim3(kTcThreads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = ctx->stream;
-    cudaLaunchAttribute attr[2] = {};
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = static_cast<unsigned>(c.splits);
-    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 2;
-    return cudaLaunchKernelEx(&cfg, token_fc_kernel<O>, t.fc.map_w, map_q, c, static_cast<O *>(outs[0]));
+    c.token_scale = token_scale; c.channel_scale = f.channel_scale; c.bias = f.bias;
+    c.err = f.err_dev; c.starve = starve;
+    c.vec = f.n % 4 == 0 && reinterpret_cast<uintptr_t>(out) % (4 * sizeof(O)) == 0;
+    if (!encode(c.bn)) return cudaErrorInvalidValue;
+    return launch_clusters(token_fc_kernel<O>, static_cast<unsigned>(tiles * c.splits), kTcThreads, smem, static_cast<unsigned>(c.splits), ctx->stream, f.map_w, map_q, c, out);
 }
 
 template <typename O>

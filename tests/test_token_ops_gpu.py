@@ -92,6 +92,35 @@ def test_token_fc(enn, ctx, m, k, n, out):
         op.release()
 
 
+@pytest.mark.parametrize("out", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("m,k,n", [(129, 64, 19000), (300, 129, 9001), (1000, 200, 4000), (1037, 1365, 5003), (2500, 16, 2000), (2049, 900, 1795), (4097, 1040, 2304)])
+def test_token_fc_large_products(enn, ctx, m, k, n, out):
+    """Products whose tiles occupy the device, ragged in every direction."""
+    q, w, s, sw, bias = fc_inputs(m + n, m, k, n)
+    for b in (None, bias):
+        op = enn.token_fc(ctx, enn.TokenFcDesc(m=m, k=k, n=n, out_dtype=code(enn, out)), w.data_ptr(), sw.data_ptr(), None if b is None else b.data_ptr())
+        y = guarded(m, n, TYPES[out])
+        execute(op, m, [q, s], [y])
+        fc_check(y[:m], q, w, s, sw, b, out, k)
+        assert untouched(y, m)
+        op.release()
+
+
+def test_token_fc_large_product_with_fewer_rows_and_any_address(enn, ctx):
+    m, k, n = 2000, 300, 4100
+    q, w, s, sw, _ = fc_inputs(3, m, k, n)
+    s[1234:] = math.nan
+    op = enn.token_fc(ctx, enn.TokenFcDesc(m=m, k=k, n=n, out_dtype=enn.F16), w.data_ptr(), sw.data_ptr())
+    y = guarded(m, n, torch.float16)
+    execute(op, 1234, [q, s], [y])
+    fc_check(y[:1234], q[:1234], w, s[:1234], sw, None, "f16", k)
+    assert untouched(y, 1234)
+    y = guarded(m, n, torch.float16, 1)
+    execute(op, 1234, [q, s], [y])
+    fc_check(y[:1234], q[:1234], w, s[:1234], sw, None, "f16", k)
+    op.release()
+
+
 @pytest.mark.parametrize("rows", [0, 1, 5, 31, 64, 100, 190, 300])
 def test_token_fc_fewer_rows_than_prepared(enn, ctx, rows):
     """One handle serves decode steps and prompts: rows past the given number are neither read nor written."""
@@ -176,11 +205,11 @@ def test_token_fc_implementations_agree(enn, ctx):
 
 def test_token_fc_that_gives_up_on_a_wait(enn, ctx):
     """A kernel whose wait ran out leaves a code; later calls fail until it is cleared, and then run as before."""
-    for m in (3, 300):
-        q, w, s, sw, _ = fc_inputs(14, m, 4096, 256)
-        op = enn.token_fc(ctx, enn.TokenFcDesc(m=m, k=4096, n=256, out_dtype=enn.F32), w.data_ptr(), sw.data_ptr())
+    for m, n in ((3, 256), (300, 256), (2000, 4096)):
+        q, w, s, sw, _ = fc_inputs(14, m, 4096, n)
+        op = enn.token_fc(ctx, enn.TokenFcDesc(m=m, k=4096, n=n, out_dtype=enn.F32), w.data_ptr(), sw.data_ptr())
         assert op.info.impl == enn.IMPL_TCGEN05
-        y = guarded(m, 256, torch.float32)
+        y = guarded(m, n, torch.float32)
         op.test_starve_next()
         execute(op, m, [q, s], [y])
         with pytest.raises(enn.EnnError) as e:
