@@ -69,7 +69,7 @@ __global__ void __launch_bounds__(kDirectThreads) token_fc_direct_kernel(TokenFc
 //   all              add the partial sums, scale and store
 constexpr int kChannels = kBM;
 constexpr int kTcThreads = 192;
-constexpr int kMaxTokens = kMaxBN;      // of a tile of a pair; 128 of a single CTA
+constexpr int kTcTokens = 128;      // most tokens of a tile
 constexpr int kMaxSplits = 8;       // portable cluster size
 constexpr int kMaxStages = 12;
 
@@ -113,6 +113,7 @@ __global__ void __launch_bounds__(kTcThreads) token_fc_kernel(const __grid_const
     __shared__ uint64_t bars[2 * kMaxStages + 1];
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_word;
+    __shared__ float scales[kTcTokens];         // of the tile's tokens
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
     volatile int *abort_flag = &abort_word;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -143,6 +144,14 @@ __global__ void __launch_bounds__(kTcThreads) token_fc_kernel(const __grid_const
     const uint32_t tmem = tmem_slot;
     pdl_trigger();
 
+    // A lane of the write-out has four channels; their constants and the tokens' scales are on the way while the tile is multiplied.
+    const int n = n0 + lane * 4, tokens = static_cast<int>(min(static_cast<int64_t>(p.bn), p.rows - m0));
+    float cs[4], b[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        cs[i] = n + i < p.n ? p.channel_scale[n + i] : 0.f;
+        b[i] = p.bias && n + i < p.n ? p.bias[n + i] : 0.f;
+    }
     uint32_t stage = 0, phase = 0;      // a producer's next fill, the issuer's next k-block
     if (warp < 2) {
         if (lane == 0 && !p.starve) {
@@ -171,6 +180,9 @@ __global__ void __launch_bounds__(kTcThreads) token_fc_kernel(const __grid_const
             if (!*abort_flag) umma_commit(tfull);
         }
         __syncwarp();
+        pdl_wait();
+        const int mine = static_cast<int>(threadIdx.x) - 64;      // warps 2 .. 5: 128 threads
+        if (mine < tokens) scales[mine] = p.token_scale[m0 + mine];
         if (mbar_wait(tfull, 0, abort_flag, p.err, 3)) {
             // Every matrix instruction has read its operands: their memory takes the sums, [token][channel].
             tc_fence_after();
@@ -195,16 +207,10 @@ __global__ void __launch_bounds__(kTcThreads) token_fc_kernel(const __grid_const
     } else {
         // The CTAs of the cluster take the tokens in turn; a warp stores the 128 channels of a token, a lane four of them.
         pdl_wait();
-        const int n = n0 + lane * 4;
-        float cs[4], b[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            cs[i] = n + i < p.n ? p.channel_scale[n + i] : 0.f;
-            b[i] = p.bias && n + i < p.n ? p.bias[n + i] : 0.f;
-        }
-        const int tokens = static_cast<int>(min(static_cast<int64_t>(p.bn), p.rows - m0));
-        for (int j = split + p.splits * warp; j < tokens; j += p.splits * (kTcThreads / 32)) {
-            const float ts = p.token_scale[m0 + j];
+        const int per = p.splits * (kTcThreads / 32);
+#pragma unroll 4
+        for (int j = split + p.splits * warp; j < tokens; j += per) {
+            const float ts = scales[j];
             const uint32_t at = ring + j * (kChannels * 4) + lane * 16;
             int4 a = make_int4(0, 0, 0, 0);
             if (p.splits == 1) {
@@ -237,8 +243,9 @@ __global__ void __launch_bounds__(kTcThreads) token_fc_kernel(const __grid_const
 // ---- tensor-core kernel for large products: persistent pairs of CTAs (cta_group::2), 256 channels x bn tokens per tile.
 // A CTA of the pair holds 128 channels of the weights and half of the tokens of every k-block, so that each operand byte comes from L2 once
 // per pair, and the accumulators of its 128 channels.  Two accumulators of up to 256 columns take all of tensor memory: one is multiplied
-// into while the other is scaled and stored.  A thread of the epilogue has one channel, whose scale and bias stay in registers; a
-// warp stores 32 neighbouring channels of a token, whole sectors whatever n and the address are.
+// into while the other is scaled and stored, 32 channels x 32 tokens at a time by a warp of the epilogue.  16-bit results are transposed
+// on their way through shared memory and leave in 16-byte pieces, 64 bytes of a token; others (n not a multiple of eight, 32-bit
+// results) leave straight from the accumulators' layout, where a thread has one channel: 32 neighbouring channels of a token per instruction.
 //   warp 0, 1        as above, of both CTAs; warp 1 is the issuer in the first CTA and allocates in both
 //   warps 2 .. 9     epilogue: lane quarter warp & 3, every other group of 32 tokens
 //   warp 10          copies the token tiles
@@ -246,6 +253,7 @@ constexpr int kPairStages = 6;
 constexpr int kPairEpiWarps = 8;
 constexpr int kPairThreads = (kPairEpiWarps + 3) * 32;
 constexpr int kPairStageBytes = (kBM + kMaxBN / 2) * kBK;
+constexpr int kPairOutBytes = 32 * 32 * 2;      // results of a warp on their way out
 
 struct PairCall {
     int32_t rows, n, kb_total;
@@ -255,7 +263,21 @@ struct PairCall {
     const float *token_scale, *channel_scale, *bias;
     int32_t *err;
     int32_t starve;
+    int32_t vec;                        // 16-bit results in pieces of eight channels: n and the address allow it
 };
+
+__device__ __forceinline__ uint32_t pack_results(float a, float b, __half) {
+    const __half2 p = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&p);
+}
+__device__ __forceinline__ uint32_t pack_results(float a, float b, __nv_bfloat16) {
+    const __nv_bfloat162 p = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&p);
+}
+// Four 8 x 8 matrices of 16-bit values, transposed: lane i gives the address of row i % 8 of matrix i / 8.
+__device__ __forceinline__ void store_matrices_transposed(uint32_t addr, const uint32_t (&r)[4]) {
+    asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]) : "memory");
+}
 
 __device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t (&r)[32]) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, "
@@ -365,35 +387,84 @@ __global__ void __launch_bounds__(kPairThreads, 1) token_fc_pair_kernel(const __
         }
     } else {
         const int q = warp & 3, half = (warp - 2) >> 2;
+        const uint32_t stage_out = ring + kPairStages * kPairStageBytes + (warp - 2) * kPairOutBytes;
         pdl_wait();
         int it = 0;
         for (int tile = first; tile < total; tile += step, ++it) {
             int tc, tt;
             pair_tile(p, tile, tc, tt);
             const uint32_t ab = it & 1, use = it >> 1;
-            const int n = (tc * 2 + static_cast<int>(rank)) * kBM + q * 32 + lane;
-            const bool live = n < p.n;
-            const float cs = live ? p.channel_scale[n] : 0.f, b = live && p.bias ? p.bias[n] : 0.f;
+            const int n_warp = (tc * 2 + static_cast<int>(rank)) * kBM + q * 32;
+            float cs[4], b[4];      // of channels 8 k + lane / 4, or of channel lane
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int n = n_warp + (p.vec ? 8 * k + (lane >> 2) : lane);
+                cs[k] = n < p.n ? p.channel_scale[n] : 0.f;
+                b[k] = p.bias && n < p.n ? p.bias[n] : 0.f;
+            }
+            float scales[kMaxBN / 64];      // of the tokens of this warp's groups, a lane one of each
+#pragma unroll
+            for (int g = 0; g < kMaxBN / 64; ++g) {
+                const int c = half * 32 + 64 * g + lane;
+                const int64_t m = static_cast<int64_t>(tt) * p.bn + c;
+                scales[g] = c < p.bn && m < p.rows ? p.token_scale[m] : 0.f;
+            }
             if (!mbar_wait(tfull0 + 8 * ab, use & 1, abort_flag, p.err, 4)) {
                 if (lane == 0) give_up();
                 break;
             }
             tc_fence_after();
             const uint32_t t_row = tmem + ab * kMaxBN + (static_cast<uint32_t>(q * 32) << 16);
-            for (int c = half * 32; c < p.bn; c += 64) {
+#pragma unroll
+            for (int g = 0; g < kMaxBN / 64; ++g) {
+                const int c = half * 32 + 64 * g;
+                if (c >= p.bn) break;
                 const int64_t m = static_cast<int64_t>(tt) * p.bn + c;
                 if (m >= p.rows) break;
                 const int tokens = static_cast<int>(min(static_cast<int64_t>(min(32, p.bn - c)), p.rows - m));
-                uint32_t r[32];
-                tmem_ld32(t_row + c, r);
-                const float ts = lane < tokens ? p.token_scale[m + lane] : 0.f;
-                O *o = out + m * p.n + n;
-                tmem_ld_wait();
+                if (sizeof(O) == 2 && p.vec) {
+                    if constexpr (sizeof(O) == 2) {
+                        uint32_t r[2][16];      // [channels 16 h ..][4 j + 2 i + s]: channel lane / 4 + 8 i, token 8 j + 2 (lane & 3) + s
+                        tmem_ld_16x256<4>(t_row + c, r[0]);
+                        tmem_ld_16x256<4>(t_row + c + (16u << 16), r[1]);
+                        tmem_ld_wait();
 #pragma unroll
-                for (int j = 0; j < 32; ++j) {
-                    const float s = __shfl_sync(0xffffffffu, ts, j);
-                    if (live && j < tokens) *o = from_float<O>(scaled(static_cast<int32_t>(r[j]), s, cs, b));
-                    o += p.n;
+                        for (int j = 0; j < 4; ++j) {
+                            const float s0 = __shfl_sync(0xffffffffu, scales[g], 8 * j + 2 * (lane & 3)), s1 = __shfl_sync(0xffffffffu, scales[g], 8 * j + 2 * (lane & 3) + 1);
+                            uint32_t v[4];
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {      // channels 8 k + lane / 4
+                                const uint32_t *a = r[k >> 1] + 4 * j + 2 * (k & 1);
+                                v[k] = pack_results(scaled(static_cast<int32_t>(a[0]), s0, cs[k], b[k]), scaled(static_cast<int32_t>(a[1]), s1, cs[k], b[k]), O{});
+                            }
+                            const int token = 8 * j + (lane & 7);      // 64 bytes each; the pieces of neighbours change places, for the banks
+                            store_matrices_transposed(stage_out + token * 64 + (((lane >> 3) ^ (token >> 1)) & 3) * 16, v);
+                        }
+                        __syncwarp();
+                        O *o = out + (m + (lane >> 2)) * p.n + n_warp + (lane & 3) * 8;
+                        const bool mine = n_warp + (lane & 3) * 8 < p.n;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int token = 8 * i + (lane >> 2);
+                            uint4 v;
+                            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                                         : "r"(stage_out + token * 64 + (((lane & 3) ^ (token >> 1)) & 3) * 16) : "memory");
+                            if (mine && token < tokens) *reinterpret_cast<uint4 *>(o) = v;
+                            o += 8 * static_cast<int64_t>(p.n);
+                        }
+                        __syncwarp();
+                    }
+                } else {
+                    uint32_t r[32];
+                    tmem_ld32(t_row + c, r);
+                    O *o = out + m * p.n + n_warp + lane;
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) {
+                        const float s = __shfl_sync(0xffffffffu, scales[g], j);
+                        if (n_warp + lane < p.n && j < tokens) *o = from_float<O>(scaled(static_cast<int32_t>(r[j]), s, cs[0], b[0]));
+                        o += p.n;
+                    }
                 }
             }
             tc_fence_before();
@@ -467,24 +538,25 @@ cudaError_t launch_tc(enn_b200_op *op, int32_t rows, const void *const *ins, voi
 
     // Large products: pairs of CTAs, once their tiles occupy most of the device.
     PairCall c2{};
-    token_tiles(rows, kMaxTokens, 32, &c2.tiles_t, &c2.bn);
+    token_tiles(rows, kMaxBN, 32, &c2.tiles_t, &c2.bn);
     c2.tiles_c = (f.n + 2 * kBM - 1) / (2 * kBM);
     const int64_t tiles2 = static_cast<int64_t>(c2.tiles_c) * c2.tiles_t;
     if (rows > 128 && pairs > 0 && tiles2 * 4 >= pairs * 3) {
         c2.rows = rows; c2.n = f.n; c2.kb_total = kb_total;
-        c2.band = std::min(8, c2.tiles_c);
+        c2.band = std::min(16, c2.tiles_c);
         c2.idesc = kSignedBytes | (static_cast<uint32_t>(c2.bn >> 3) << 17) | (static_cast<uint32_t>(2 * kBM >> 4) << 24);
         c2.token_scale = token_scale; c2.channel_scale = f.channel_scale; c2.bias = f.bias;
         c2.err = f.err_dev; c2.starve = starve;
+        c2.vec = sizeof(O) == 2 && f.n % 8 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
         if (!encode(c2.bn / 2)) return cudaErrorInvalidValue;
-        return launch_clusters(token_fc_pair_kernel<O>, static_cast<unsigned>(2 * std::min<int64_t>(tiles2, pairs)), kPairThreads, 1024 + kPairStages * kPairStageBytes, 2, ctx->stream,
+        return launch_clusters(token_fc_pair_kernel<O>, static_cast<unsigned>(2 * std::min<int64_t>(tiles2, pairs)), kPairThreads, 1024 + kPairStages * kPairStageBytes + kPairEpiWarps * kPairOutBytes, 2, ctx->stream,
                                f.map_w, map_q, c2, out);
     }
 
     // Two CTAs share an SM: while one waits for its first tiles or stores its results, the other keeps the SM busy.
     TcCall c{};
     c.rows = rows; c.n = f.n; c.kb_total = kb_total;
-    token_tiles(rows, 128, 16, &c.m_tiles, &c.bn);
+    token_tiles(rows, kTcTokens, 16, &c.m_tiles, &c.bn);
     const int64_t tiles = static_cast<int64_t>((f.n + kChannels - 1) / kChannels) * c.m_tiles;
     c.splits = 1;
     while (c.splits < kMaxSplits && tiles * c.splits * 2 <= 2 * ctx->launch_sms() && kb_total >= 4 * c.splits) c.splits *= 2;
