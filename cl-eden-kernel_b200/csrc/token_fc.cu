@@ -208,7 +208,7 @@ __global__ void __launch_bounds__(kTcThreads) token_fc_kernel(const __grid_const
         // The CTAs of the cluster take the tokens in turn; a warp stores the 128 channels of a token, a lane four of them.
         pdl_wait();
         const int per = p.splits * (kTcThreads / 32);
-#pragma unroll 4
+#pragma unroll 2
         for (int j = split + p.splits * warp; j < tokens; j += per) {
             const float ts = scales[j];
             const uint32_t at = ring + j * (kChannels * 4) + lane * 16;
@@ -232,7 +232,8 @@ __global__ void __launch_bounds__(kTcThreads) token_fc_kernel(const __grid_const
             }
         }
     }
-    if (p.splits > 1) cluster_sync_all();       // nobody leaves while its sums are still read
+    // Nobody leaves while its sums are still read; the results' stores need not be waited for.
+    if (p.splits > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
     else __syncthreads();
     if (warp == 2) {
         tc_fence_after();
@@ -293,6 +294,11 @@ __device__ __forceinline__ void pair_tile(const PairCall &p, int tile, int &tc, 
     const int per = p.band * p.tiles_t, b = tile / per, r = tile - b * per, width = min(p.band, p.tiles_c - b * p.band);
     tt = r / width;
     tc = b * p.band + (r - tt * width);
+}
+
+// The accumulators have been read into registers: that needs no order with the results' stores, for which a release would wait.
+__device__ __forceinline__ void arrive_relaxed(uint32_t cluster_addr) {
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 
 template <typename O>
@@ -469,7 +475,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) token_fc_pair_kernel(const __
             }
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive_cluster(mapa_rank(tempty0 + 8 * ab, 0));
+            if (lane == 0) arrive_relaxed(mapa_rank(tempty0 + 8 * ab, 0));
         }
     }
     __syncwarp();
