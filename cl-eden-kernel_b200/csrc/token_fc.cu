@@ -254,6 +254,7 @@ constexpr int kPairStages = 6;
 constexpr int kPairEpiWarps = 8;
 constexpr int kPairThreads = (kPairEpiWarps + 3) * 32;
 constexpr int kPairStageBytes = (kBM + kMaxBN / 2) * kBK;
+constexpr int kPairRows = 192, kTileCost = 48;
 constexpr int kPairOutBytes = 32 * 32 * 2;      // results of a warp on their way out
 
 struct PairCall {
@@ -542,12 +543,22 @@ cudaError_t launch_tc(enn_b200_op *op, int32_t rows, const void *const *ins, voi
     };
     const int pairs = ctx->launch_sms() / 2;
 
-    // Large products: pairs of CTAs, once their tiles occupy most of the device.
+    // Large products: pairs of CTAs.  The width of the token tiles is the one whose rounds over the device take least, a tile costing its
+    // columns and about as much as kTileCost more.
     PairCall c2{};
-    token_tiles(rows, kMaxBN, 32, &c2.tiles_t, &c2.bn);
     c2.tiles_c = (f.n + 2 * kBM - 1) / (2 * kBM);
-    const int64_t tiles2 = static_cast<int64_t>(c2.tiles_c) * c2.tiles_t;
-    if (rows > 128 && pairs > 0 && tiles2 * 4 >= pairs * 3) {
+    int64_t least = INT64_MAX, tiles2 = 0;
+    for (int32_t bn = kMaxBN; bn >= 64 && pairs > 0; bn -= 32) {
+        const int32_t tiles_t = (rows + bn - 1) / bn;
+        const int64_t tiles = static_cast<int64_t>(c2.tiles_c) * tiles_t, cost = (tiles + pairs - 1) / pairs * (bn + kTileCost);
+        if (cost < least) {
+            least = cost;
+            tiles2 = tiles;
+            c2.tiles_t = tiles_t;
+            c2.bn = bn;
+        }
+    }
+    if (rows >= kPairRows && pairs > 0 && tiles2 * 2 >= pairs) {
         c2.rows = rows; c2.n = f.n; c2.kb_total = kb_total;
         c2.band = std::min(16, c2.tiles_c);
         c2.idesc = kSignedBytes | (static_cast<uint32_t>(c2.bn >> 3) << 17) | (static_cast<uint32_t>(2 * kBM >> 4) << 24);
