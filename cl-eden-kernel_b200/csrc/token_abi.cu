@@ -62,13 +62,19 @@ struct Building {
         e = cudaMemcpy2DAsync(*dst, pitch, src, width, width, height, cudaMemcpyDefault, op->ctx->stream);
         return e == cudaSuccess ? cudaStreamSynchronize(op->ctx->stream) : e;
     }
-    cudaError_t vector(const float *src, int32_t n, const float **dst) {
-        void *d = nullptr;
+    // `copies` times, copy i shifted by i floats within `stride`.
+    cudaError_t vector(const float *src, int32_t n, const float **dst, int copies = 1, int32_t stride = 0) {
         if (!src) return cudaSuccess;
         op->info.algorithmic_bytes += int64_t{4} * n;
-        const cudaError_t e = constant(src, sizeof(float) * static_cast<size_t>(n), 1, sizeof(float) * static_cast<size_t>(n), &d);
-        *dst = static_cast<const float *>(d);
-        return e;
+        const size_t bytes = sizeof(float) * static_cast<size_t>(n);
+        float *d = nullptr;
+        cudaError_t e = cudaMalloc(&d, sizeof(float) * static_cast<size_t>(stride) * (copies - 1) + bytes + sizeof(float) * (copies - 1));
+        if (e != cudaSuccess) return e;
+        op->owned.push_back(d);
+        for (int i = 0; i < copies && e == cudaSuccess; ++i)
+            e = cudaMemcpyAsync(d + static_cast<size_t>(i) * stride + i, src, bytes, cudaMemcpyDefault, op->ctx->stream);
+        *dst = d;
+        return e == cudaSuccess ? cudaStreamSynchronize(op->ctx->stream) : e;
     }
     int32_t finish(enn_b200_op **out) {
         *out = op;
@@ -149,10 +155,11 @@ int32_t enn_b200_token_norm_prepare(enn_b200_context *ctx, const enn_b200_token_
     p.gate_tokens = d->gate_tokens;
     p.eps = d->eps; p.post_eps = d->post_eps; p.residual_scale = d->residual_scale;
     p.pitch = token_pitch(d->c);
-    cudaError_t e = b.vector(weight, d->c, &p.weight);
-    if (e == cudaSuccess) e = b.vector(bias, d->c, &p.bias);
-    if (e == cudaSuccess) e = b.vector(post_weight, d->c, &p.post_weight);
-    if (e == cudaSuccess) e = b.vector(post_bias, d->c, &p.post_bias);
+    p.stride = (d->c + 3) / 4 * 4 + 4;
+    cudaError_t e = b.vector(weight, d->c, &p.weight, 4, p.stride);
+    if (e == cudaSuccess) e = b.vector(bias, d->c, &p.bias, 4, p.stride);
+    if (e == cudaSuccess) e = b.vector(post_weight, d->c, &p.post_weight, 4, p.stride);
+    if (e == cudaSuccess) e = b.vector(post_bias, d->c, &p.post_bias, 4, p.stride);
     if (e != cudaSuccess) return cfail(ctx, e);
     b.op->info.out_c = d->c;
     return b.finish(out);

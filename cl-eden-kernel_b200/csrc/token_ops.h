@@ -14,7 +14,8 @@ struct NormParams {
     int32_t norm, post_norm;
     int32_t gate_tokens;
     float eps, post_eps, residual_scale;
-    const float *weight, *bias, *post_weight, *post_bias;      // null: ones / zeros
+    const float *weight, *bias, *post_weight, *post_bias;      // null: ones / zeros; each four times, copy i at i * stride + i
+    int32_t stride;
     int64_t pitch;                                              // bytes from row to row of byte rows
 };
 

@@ -69,74 +69,90 @@ __device__ __forceinline__ uint32_t pack4_s8(const float *f, float inv) {
     return d;
 }
 
-// What a thread holds of eight channels between their loads and their use: as they lie in memory, or as floats where they came one by one.
-template <typename T, bool VEC> using Held = std::conditional_t<VEC, Raw<T>, Raw<float>>;
-
-// The part of a row that a group of `nt` threads holds: channels [0, n) of a segment, NV groups per thread.  VEC: neighbouring channels
-// in 16-byte pieces (n, every address and every pitch allow it); else one channel at a time, neighbouring threads on neighbouring
-// channels, for rows that begin anywhere.
-template <int NV, bool VEC>
+// The part of a row that a group of `nt` threads holds: channels [0, n) of a segment in groups of eight neighbours, NV per thread.
+// LINES: every group is whole and lies on 16-byte lines (n, every address and every pitch allow it).  Else the groups are shifted
+// by `skip` channels, so that they lie on the lines of the tensor they were laid out for; the first and the last may reach over the
+// row's ends, where only what is inside is touched, and tensors with other lines (halves of odd rows, bytes) are taken channel by channel.
+template <int NV, bool LINES>
 struct Row {
-    int n, tid, nt;
-    __device__ __forceinline__ int at(int v, int j) const { return VEC ? (v * nt + tid) * kGroup + j : (v * kGroup + j) * nt + tid; }
+    int n, tid, nt, skip;
+    __device__ __forceinline__ int at(int v, int j = 0) const { return (v * nt + tid) * kGroup + j - (LINES ? 0 : skip); }
+    __device__ __forceinline__ bool any(int v) const { return at(v) < n; }
+    __device__ __forceinline__ bool whole(int v) const { return LINES ? any(v) : at(v) >= 0 && at(v) + kGroup <= n; }
+    __device__ __forceinline__ bool inside(int v, int j) const { return LINES ? any(v) : at(v, j) >= 0 && at(v, j) < n; }
+    // The groups lie on lines of the tensor whose row begins at p.
+    template <typename T> __device__ __forceinline__ bool lined(const T *p) const { return LINES || ((reinterpret_cast<uintptr_t>(p) - skip * sizeof(T)) & 15) == 0; }
+    // Lays the groups out on the lines of the row at p.
+    template <typename T> __device__ __forceinline__ void lay_out(const T *p) { skip = LINES ? 0 : static_cast<int>((reinterpret_cast<uintptr_t>(p) & 15) / sizeof(T)); }
 
-    template <typename T> __device__ __forceinline__ void load(const T *p, Held<T, VEC> (&held)[NV]) const {
+    template <typename T> __device__ __forceinline__ Raw<T> group(const T *p, int v, bool on_lines) const {
+        Raw<T> r{};
+        if (whole(v) && on_lines) return ld8(p + at(v));
+        if constexpr (!LINES) {
+            T e[kGroup];
+            if (whole(v)) {
 #pragma unroll
-        for (int v = 0; v < NV; ++v) {
-            held[v] = Held<T, VEC>{};
-            if constexpr (VEC) {
-                if (at(v, 0) < n) held[v] = ld8(p + at(v, 0));
+                for (int j = 0; j < kGroup; ++j) e[j] = p[at(v) + j];
             } else {
-                float f[kGroup] = {};
 #pragma unroll
-                for (int j = 0; j < kGroup; ++j)
-                    if (at(v, j) < n) f[j] = to_float(p[at(v, j)]);
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-                    held[v].v[i] = make_uint4(__float_as_uint(f[4 * i]), __float_as_uint(f[4 * i + 1]), __float_as_uint(f[4 * i + 2]), __float_as_uint(f[4 * i + 3]));
+                for (int j = 0; j < kGroup; ++j) e[j] = inside(v, j) ? p[at(v, j)] : from_float<T>(0.f);
             }
+            __builtin_memcpy(&r, e, sizeof(e));
         }
+        return r;
     }
-    // f(channel value, constant) over the thread's channels; nothing where the constant vector is not given.
-    template <typename F> __device__ __forceinline__ void with(const float *p, float (&f)[NV][8], F apply) const {
+    template <typename T> __device__ __forceinline__ void load(const T *p, Raw<T> (&held)[NV]) const {
+        const bool on_lines = lined(p);
+#pragma unroll
+        for (int v = 0; v < NV; ++v) held[v] = group(p, v, on_lines);
+    }
+    // f(channel value, constant) over the thread's channels; nothing where the constant vector is not given.  A vector is kept four
+    // times, `stride` floats apart and each a float further along, so that the groups of any row lie on 16-byte lines of one of them.
+    template <typename F> __device__ __forceinline__ void with(const float *p, int stride, float (&f)[NV][8], F apply) const {
         if (!p) return;
+        const float *q = LINES ? p : p + (skip & 3) * stride + (skip & 3);
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
-            if constexpr (VEC) {
-                if (at(v, 0) < n) {
-                    const float4 a = __ldg(reinterpret_cast<const float4 *>(p + at(v, 0))), b = __ldg(reinterpret_cast<const float4 *>(p + at(v, 0)) + 1);
-                    const float w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+            if (whole(v)) {
+                const float4 a = __ldg(reinterpret_cast<const float4 *>(q + at(v))), b = __ldg(reinterpret_cast<const float4 *>(q + at(v)) + 1);
+                const float w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
 #pragma unroll
-                    for (int j = 0; j < kGroup; ++j) f[v][j] = apply(f[v][j], w[j]);
-                }
-            } else {
+                for (int j = 0; j < kGroup; ++j) f[v][j] = apply(f[v][j], w[j]);
+            } else if (!LINES) {
 #pragma unroll
                 for (int j = 0; j < kGroup; ++j)
-                    if (at(v, j) < n) f[v][j] = apply(f[v][j], __ldg(p + at(v, j)));
+                    if (inside(v, j)) f[v][j] = apply(f[v][j], __ldg(p + at(v, j)));
             }
         }
     }
     template <typename T> __device__ __forceinline__ void store(T *p, const float (&f)[NV][8]) const {
+        const bool on_lines = lined(p);
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
-            if constexpr (VEC) {
-                if (at(v, 0) < n) st8(p + at(v, 0), f[v]);
-            } else {
+            if (whole(v) && on_lines) {
+                st8(p + at(v), f[v]);
+            } else if (!LINES) {
+                if (whole(v)) {
 #pragma unroll
-                for (int j = 0; j < kGroup; ++j)
-                    if (at(v, j) < n) p[at(v, j)] = from_float<T>(f[v][j]);
+                    for (int j = 0; j < kGroup; ++j) p[at(v) + j] = from_float<T>(f[v][j]);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < kGroup; ++j)
+                        if (inside(v, j)) p[at(v, j)] = from_float<T>(f[v][j]);
+                }
             }
         }
     }
     __device__ __forceinline__ void store_bytes(int8_t *p, const float (&f)[NV][8], float inv) const {
+        const bool words = LINES || ((reinterpret_cast<uintptr_t>(p) - skip) & 7) == 0;
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
-            if constexpr (VEC) {
-                if (at(v, 0) < n) *reinterpret_cast<uint2 *>(p + at(v, 0)) = make_uint2(pack4_s8(f[v], inv), pack4_s8(f[v] + 4, inv));
-            } else {
+            if (whole(v) && words) {
+                *reinterpret_cast<uint2 *>(p + at(v)) = make_uint2(pack4_s8(f[v], inv), pack4_s8(f[v] + 4, inv));
+            } else if (!LINES) {
 #pragma unroll
                 for (int j = 0; j < kGroup; ++j)
-                    if (at(v, j) < n) p[at(v, j)] = static_cast<int8_t>(quantise(f[v][j], inv));
+                    if (inside(v, j)) p[at(v, j)] = static_cast<int8_t>(quantise(f[v][j], inv));
             }
         }
     }
@@ -211,9 +227,9 @@ __device__ __forceinline__ void multiply(float (&f)[NV][8], float by) {
 
 // f = norm(f).  Channels past the row's end are 0 before and after.  With `largest` the bits of the largest magnitude of the result
 // come back too; for an RMS norm without a bias they ride on the sum of squares, since max |f r w| = r max |f w|.
-template <int NV, bool VEC>
-__device__ __forceinline__ void norm_row(const Row<NV, VEC> &row, float (&f)[NV][8], int c, int kind, float eps, const float *weight, const float *bias, Reduce &reduce,
-                                         uint32_t *largest) {
+template <int NV, bool LINES>
+__device__ __forceinline__ void norm_row(const Row<NV, LINES> &row, float (&f)[NV][8], int c, int kind, float eps, const float *weight, const float *bias, int stride,
+                                         Reduce &reduce, uint32_t *largest) {
     const auto times = [](float a, float w) { return a * w; };
     if (kind != ENN_B200_NORM_NONE) {
         const float over = 1.f / static_cast<float>(c);
@@ -227,11 +243,11 @@ __device__ __forceinline__ void norm_row(const Row<NV, VEC> &row, float (&f)[NV]
 #pragma unroll
             for (int v = 0; v < NV; ++v)
 #pragma unroll
-                for (int j = 0; j < kGroup; ++j) f[v][j] = row.at(v, VEC ? 0 : j) < row.n ? f[v][j] - mean : 0.f;
+                for (int j = 0; j < kGroup; ++j) f[v][j] = row.inside(v, j) ? f[v][j] - mean : 0.f;
         }
         float s = sum_of_squares(f);
         if (largest && kind == ENN_B200_NORM_RMS && !bias) {
-            row.with(weight, f, times);
+            row.with(weight, stride, f, times);
             uint32_t m = largest_of(f);
             reduce.both(s, m);
             const float r = rsqrtf(fmaf(s, over, eps));
@@ -240,15 +256,15 @@ __device__ __forceinline__ void norm_row(const Row<NV, VEC> &row, float (&f)[NV]
             return;
         }
         multiply(f, rsqrtf(fmaf(reduce.sum(s), over, eps)));
-        row.with(weight, f, times);
-        row.with(bias, f, [](float a, float b) { return a + b; });
+        row.with(weight, stride, f, times);
+        row.with(bias, stride, f, [](float a, float b) { return a + b; });
     }
     if (largest) *largest = reduce.largest(largest_of(f));
 }
 
 // Threads a block has at most: what the registers of NV groups a thread allow.
-constexpr int max_threads(int nv) { return nv == 1 ? 1024 : (nv == 4 ? 256 : 512); }
-// Blocks of that size an SM is to hold: 64 registers a thread, 80 with four groups, 128 with eight.
+constexpr int max_threads(int nv) { return nv == 1 ? 1024 : (nv == 2 ? 512 : (nv == 4 ? 256 : 544)); }
+// Blocks of that size an SM is to hold: 64 registers a thread, 80 with four groups, 120 with eight.
 constexpr int min_blocks(int nv) { return nv == 4 ? 3 : (nv == 2 ? 2 : 1); }
 
 // A thread's own ring in shared memory: `depth` rows ahead, each with `streams` tensors, filled by asynchronous copies.  A thread reads
@@ -260,24 +276,28 @@ struct Ahead {
     uint32_t piece;                                    // bytes from piece to piece: 16 for each thread of the block
     int streams, depth, slot;
     __device__ __forceinline__ uint32_t at(int s, int stream, int v, int i) const { return base + static_cast<uint32_t>(((s * streams + stream) * NV + v) * kPieces + i) * piece; }
-    __device__ __forceinline__ void fetch(const Row<NV, true> &row, int s, int stream, const T *p) const {
+    template <bool LINES> __device__ __forceinline__ void fetch(const Row<NV, LINES> &row, int s, int stream, const T *p) const {
+        if (!row.lined(p)) return;
 #pragma unroll
         for (int v = 0; v < NV; ++v)
-            if (row.at(v, 0) < row.n)
+            if (row.whole(v))
 #pragma unroll
                 for (int i = 0; i < kPieces; ++i)
-                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at(s, stream, v, i)), "l"(reinterpret_cast<const uint4 *>(p + row.at(v, 0)) + i) : "memory");
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at(s, stream, v, i)), "l"(reinterpret_cast<const uint4 *>(p + row.at(v)) + i) : "memory");
     }
-    __device__ __forceinline__ void read(const Row<NV, true> &row, int stream, Raw<T> (&held)[NV]) const {
+    template <bool LINES> __device__ __forceinline__ void read(const Row<NV, LINES> &row, int stream, const T *p, Raw<T> (&held)[NV]) const {
+        const bool copied = row.lined(p);
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
-            held[v] = Raw<T>{};
-            if (row.at(v, 0) < row.n)
+            if (row.whole(v) && copied) {
 #pragma unroll
                 for (int i = 0; i < kPieces; ++i) {
                     uint4 &q = held[v].v[i];
                     asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(q.x), "=r"(q.y), "=r"(q.z), "=r"(q.w) : "r"(at(slot, stream, v, i)) : "memory");
                 }
+            } else {
+                held[v] = row.any(v) ? row.group(p, v, false) : Raw<T>{};
+            }
         }
     }
 };
@@ -292,50 +312,47 @@ __device__ __forceinline__ void ahead_wait(int pending) {
 constexpr int kMaxDepth = 4;
 constexpr int kRingBytes = 216 * 1024;
 
-template <typename T, int NV, bool VEC>
+template <typename T, int NV, bool LINES>
 __global__ void __launch_bounds__(max_threads(NV), min_blocks(NV)) token_norm_kernel(NormParams p, int32_t rows, int32_t out_dtype, int32_t depth, const T *x,
                                                                                        const T *residual, const T *gate, T *stream, void *out, float *scale) {
     extern __shared__ __align__(16) uint8_t ring[];
     __shared__ float2 scratch[2][32];
     const int64_t step = static_cast<int64_t>(gridDim.x) * blockDim.y;
-    Row<NV, VEC> row{p.c, static_cast<int>(threadIdx.x), static_cast<int>(blockDim.x)};
+    Row<NV, LINES> row{p.c, static_cast<int>(threadIdx.x), static_cast<int>(blockDim.x), 0};
     Reduce reduce{scratch, row.nt, 0};
     pdl_wait();
     pdl_trigger();
     const int64_t first = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
-    [[maybe_unused]] Ahead<T, NV> ahead{};
-    if constexpr (VEC) {
-        const uint32_t threads = blockDim.x * blockDim.y;
-        ahead = Ahead<T, NV>{smem_u32(ring) + 16 * (threadIdx.y * blockDim.x + threadIdx.x), 16 * threads, 1 + (residual != nullptr) + (gate != nullptr), depth, 0};
-    }
+    const uint32_t threads = blockDim.x * blockDim.y;
+    Ahead<T, NV> ahead{smem_u32(ring) + 16 * (threadIdx.y * blockDim.x + threadIdx.x), 16 * threads, 1 + (residual != nullptr) + (gate != nullptr), depth, 0};
     auto fetch = [&](int s, int64_t t) {
-        if constexpr (VEC) {
-            if (t < rows) {
-                ahead.fetch(row, s, 0, x + t * p.c);
-                if (residual) ahead.fetch(row, s, 1, residual + t * p.c);
-                if (gate) ahead.fetch(row, s, ahead.streams - 1, gate + t / p.gate_tokens * p.c);
-            }
-            ahead_commit();
+        if (depth == 0) return;
+        if (t < rows) {
+            Row<NV, LINES> r = row;
+            r.lay_out(x + t * p.c);
+            ahead.fetch(r, s, 0, x + t * p.c);
+            if (residual) ahead.fetch(r, s, 1, residual + t * p.c);
+            if (gate) ahead.fetch(r, s, ahead.streams - 1, gate + t / p.gate_tokens * p.c);
         }
+        ahead_commit();
     };
-    // Tensor `which` of row t, from the ring or from memory.
     auto take = [&](int which, const T *p_row, float (&f)[NV][8]) {
-        Held<T, VEC> held[NV];
-        if constexpr (VEC) ahead.read(row, which, held);
+        Raw<T> held[NV];
+        if (depth) ahead.read(row, which, p_row, held);
         else row.load(p_row, held);
 #pragma unroll
         for (int v = 0; v < NV; ++v) widen(held[v], f[v]);
     };
-    if constexpr (VEC)
-        for (int s = 0; s < depth; ++s) fetch(s, first + s * step);
+    for (int s = 0; s < depth; ++s) fetch(s, first + s * step);
     for (int64_t t = first; t < rows; t += step) {      // t is the same for a whole warp, and for the whole block where a row has several warps
         float f[NV][8];
-        if constexpr (VEC) ahead_wait(depth - 1);
+        row.lay_out(x + t * p.c);
+        if (depth) ahead_wait(depth - 1);
         take(0, x + t * p.c, f);
-        norm_row(row, f, p.c, p.post_norm, p.post_eps, p.post_weight, p.post_bias, reduce, nullptr);
+        norm_row(row, f, p.c, p.post_norm, p.post_eps, p.post_weight, p.post_bias, p.stride, reduce, nullptr);
         if (gate) {
             float g[NV][8];
-            take(VEC ? ahead.streams - 1 : 0, gate + t / p.gate_tokens * p.c, g);
+            take(ahead.streams - 1, gate + t / p.gate_tokens * p.c, g);
 #pragma unroll
             for (int v = 0; v < NV; ++v)
 #pragma unroll
@@ -351,17 +368,15 @@ __global__ void __launch_bounds__(max_threads(NV), min_blocks(NV)) token_norm_ke
         } else if (p.residual_scale != 1.f) {
             multiply(f, p.residual_scale);
         }
-        if constexpr (VEC) {
-            fetch(ahead.slot, t + depth * step);        // this row's memory has been read
-            if (++ahead.slot == depth) ahead.slot = 0;
-        }
+        fetch(ahead.slot, t + depth * step);        // this row's memory has been read
+        if (++ahead.slot >= depth) ahead.slot = 0;
         if (residual) row.store(stream + t * p.c, f);
         if (out_dtype != ENN_B200_S8) {
-            norm_row(row, f, p.c, p.norm, p.eps, p.weight, p.bias, reduce, nullptr);
+            norm_row(row, f, p.c, p.norm, p.eps, p.weight, p.bias, p.stride, reduce, nullptr);
             row.store_as(out_dtype, out, t * p.c, f);
         } else {
             uint32_t largest;
-            norm_row(row, f, p.c, p.norm, p.eps, p.weight, p.bias, reduce, &largest);
+            norm_row(row, f, p.c, p.norm, p.eps, p.weight, p.bias, p.stride, reduce, &largest);
             const RowScale rs = row_scale(largest);
             int8_t *q = static_cast<int8_t *>(out) + t * p.pitch;
             row.store_bytes(q, f, rs.inv);
@@ -398,9 +413,9 @@ __device__ __forceinline__ float gate_act(float g) {
 }
 
 // f = act(gates) * values of the thread's channels.
-template <typename T, int NV, bool VEC>
-__device__ __forceinline__ void gate_row(const Row<NV, VEC> &row, const T *gates, const T *values, int act, float (&f)[NV][8]) {
-    Held<T, VEC> rg[NV], ru[NV];
+template <typename T, int NV, bool LINES>
+__device__ __forceinline__ void gate_row(const Row<NV, LINES> &row, const T *gates, const T *values, int act, float (&f)[NV][8]) {
+    Raw<T> rg[NV], ru[NV];
     row.load(gates, rg);
     row.load(values, ru);
     auto apply = [&](auto which) {
@@ -424,14 +439,14 @@ __device__ __forceinline__ void gate_row(const Row<NV, VEC> &row, const T *gates
 
 // Grid: rows x segments of `seg` channels.  Floats leave at once.  Bytes need the row's largest magnitude first: the
 // segments of a row are then the CTAs of a cluster, which tell each other theirs.
-template <typename T, int NV, bool VEC>
+template <typename T, int NV, bool LINES>
 __global__ void __launch_bounds__(max_threads(NV)) token_gate_kernel(GateParams p, int32_t rows, int32_t seg, int32_t out_dtype, const T *gates, const T *values,
                                                                  void *out, float *scale) {
     __shared__ float2 scratch[2][32];
     __shared__ uint32_t of_cluster[8];
     const int64_t t = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
     const int32_t segs = static_cast<int32_t>(gridDim.y), rank = static_cast<int32_t>(blockIdx.y), c0 = rank * seg;
-    Row<NV, VEC> row{min(seg, p.c - c0), static_cast<int>(threadIdx.x), static_cast<int>(blockDim.x)};
+    Row<NV, LINES> row{min(seg, p.c - c0), static_cast<int>(threadIdx.x), static_cast<int>(blockDim.x), 0};
     // Seen by the others of the cluster before they write here: waited for below.
     const bool clustered = segs > 1 && out_dtype == ENN_B200_S8;
     if (clustered) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
@@ -439,6 +454,7 @@ __global__ void __launch_bounds__(max_threads(NV)) token_gate_kernel(GateParams 
     pdl_trigger();
     if (t >= rows) return;      // a whole warp, and then the block has no barrier
     float f[NV][8];
+    row.lay_out(gates + t * p.in_stride + c0);
     gate_row(row, gates + t * p.in_stride + c0, values + t * p.in_stride + c0, p.act, f);
     if (out_dtype != ENN_B200_S8) {
         row.store_as(out_dtype, out, t * p.c + c0, f);
@@ -468,12 +484,12 @@ bool aligned(const void *p, size_t to) { return reinterpret_cast<uintptr_t>(p) %
 struct Shape {
     int nt, nv, per_block;
 };
-Shape row_shape(int n, bool vec, bool spread) {
-    const int groups = (n + kGroup - 1) / kGroup;
+Shape row_shape(int n, bool lines, bool spread) {
+    const int groups = (n + (lines ? 0 : kGroup - 1) + kGroup - 1) / kGroup;      // one more where they are shifted
     auto threads = [&](int nv) { return ((groups + nv - 1) / nv + 31) / 32 * 32; };
     Shape s;
-    if (groups <= 32 || ((spread || !vec) && groups <= 1024)) s.nv = 1;
-    else if (groups <= 64 || (!vec && groups <= 1024)) s.nv = 2;
+    if (groups <= 32 || (spread && groups <= 1024)) s.nv = 1;
+    else if (groups <= 64) s.nv = 2;
     else s.nv = groups <= 1024 ? 4 : 8;
     s.nt = threads(s.nv);
     s.per_block = s.nt == 32 ? 8 : 1;
@@ -481,7 +497,7 @@ Shape row_shape(int n, bool vec, bool spread) {
 }
 
 template <typename F>
-cudaError_t with_shape(int nv, bool vec, F f) {
+cudaError_t with_shape(int nv, bool lines, F f) {
     auto groups = [&](auto v) {
         switch (nv) {
             case 1: return f(std::integral_constant<int, 1>{}, v);
@@ -490,7 +506,7 @@ cudaError_t with_shape(int nv, bool vec, F f) {
             default: return f(std::integral_constant<int, 8>{}, v);
         }
     };
-    return vec ? groups(std::true_type{}) : groups(std::false_type{});
+    return lines ? groups(std::true_type{}) : groups(std::false_type{});
 }
 
 template <typename T>
@@ -506,20 +522,20 @@ cudaError_t norm_typed(const enn_b200_op *op, int32_t rows, const void *const *i
     float *scale = t.out_dtype == ENN_B200_S8 ? static_cast<float *>(outs[o++]) : nullptr;
     const bool lines = p.c % kGroup == 0 && aligned(x, 16) && aligned(residual, 16) && aligned(gate, 16) && aligned(stream, 16) && aligned(y, scale ? 8 : 16);
     const Shape s = row_shape(p.c, lines, rows <= 2 * op->ctx->sm_count);
-    // As many blocks as an SM holds, each taking rows in turn, and rings of up to four rows in what shared memory that leaves them.
+    // As many blocks as an SM holds, each taking rows in turn, and rings of up to four rows in what shared memory
+    // that leaves them; the widest rows of 32-bit types do without.
     const int threads = s.nt * s.per_block;
     const int blocks = std::max(1, max_threads(s.nv) * min_blocks(s.nv) / threads);
     const int ahead_bytes = threads * s.nv * kGroup * static_cast<int>(sizeof(T)) * (1 + (residual != nullptr) + (gate != nullptr));
-    const int depth = std::min(kMaxDepth, std::max(1, kRingBytes / blocks / ahead_bytes));
-    const bool vec = lines && ahead_bytes <= kRingBytes;
+    const int depth = ahead_bytes > kRingBytes ? 0 : std::min(kMaxDepth, std::max(1, kRingBytes / blocks / ahead_bytes));
     const int64_t want = (static_cast<int64_t>(rows) + s.per_block - 1) / s.per_block, most = static_cast<int64_t>(op->ctx->launch_sms()) * blocks;
     const dim3 grid(static_cast<unsigned>(std::min(want, most))), block(static_cast<unsigned>(s.nt), static_cast<unsigned>(s.per_block));
-    return with_shape(s.nv, vec, [&](auto nv, auto v) {
+    return with_shape(s.nv, lines, [&](auto nv, auto v) {
         constexpr auto kernel = token_norm_kernel<T, decltype(nv)::value, decltype(v)::value>;
         static PerDeviceInit once;
         const cudaError_t e = once.run(op->ctx->device, [&] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBytes); });
         if (e != cudaSuccess) return e;
-        return launch_pdl(kernel, grid, block, vec ? static_cast<size_t>(depth) * ahead_bytes : 0, op->ctx->stream, p, rows, t.out_dtype, depth, x, residual, gate, stream, y, scale);
+        return launch_pdl(kernel, grid, block, static_cast<size_t>(depth) * ahead_bytes, op->ctx->stream, p, rows, t.out_dtype, depth, x, residual, gate, stream, y, scale);
     });
 }
 
@@ -529,7 +545,7 @@ cudaError_t gate_typed(const enn_b200_op *op, int32_t rows, const void *const *i
     const GateParams &p = t.gate;
     const T *g = static_cast<const T *>(ins[0]), *u = t.packed ? g + p.c : static_cast<const T *>(ins[1]);
     const bool bytes = t.out_dtype == ENN_B200_S8;
-    const bool vec = p.c % kGroup == 0 && aligned(g, 16) && aligned(u, 16) && aligned(outs[0], bytes ? 8 : 16);
+    const bool lines = p.c % kGroup == 0 && aligned(g, 16) && aligned(u, 16) && aligned(outs[0], bytes ? 8 : 16);
     // Segments: of up to 8192 channels; of bytes up to eight of them, more where the rows alone do not occupy the device.
     int segs = 1;
     if (!bytes) segs = (p.c + 8191) / 8192;
@@ -537,7 +553,7 @@ cudaError_t gate_typed(const enn_b200_op *op, int32_t rows, const void *const *i
         while (segs < 8 && (p.c > 8192 * segs || (static_cast<int64_t>(rows) * segs * 2 <= 2 * op->ctx->sm_count && p.c >= 2048 * segs))) segs *= 2;
     const int seg = segs == 1 ? p.c : ((p.c + segs - 1) / segs + kGroup - 1) / kGroup * kGroup;
     if (!bytes) segs = (p.c + seg - 1) / seg;
-    const Shape s = row_shape(seg, vec, static_cast<int64_t>(rows) * segs <= 2 * op->ctx->sm_count);
+    const Shape s = row_shape(seg, lines, static_cast<int64_t>(rows) * segs <= 2 * op->ctx->sm_count);
     const int per_block = segs > 1 && bytes ? 1 : s.per_block;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(static_cast<unsigned>((static_cast<int64_t>(rows) + per_block - 1) / per_block), static_cast<unsigned>(segs));
@@ -551,7 +567,7 @@ cudaError_t gate_typed(const enn_b200_op *op, int32_t rows, const void *const *i
     attr[1].val.clusterDim.y = static_cast<unsigned>(segs);
     cfg.attrs = attr;
     cfg.numAttrs = bytes && segs > 1 ? 2 : 1;
-    return with_shape(s.nv, vec, [&](auto nv, auto v) {
+    return with_shape(s.nv, lines, [&](auto nv, auto v) {
         return cudaLaunchKernelEx(&cfg, token_gate_kernel<T, decltype(nv)::value, decltype(v)::value>, p, rows, seg, t.out_dtype, g, u, outs[0],
                                   bytes ? static_cast<float *>(outs[1]) : nullptr);
     });

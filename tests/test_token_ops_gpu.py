@@ -352,6 +352,36 @@ def test_token_norm_fewer_rows_than_prepared(enn, ctx, rows):
         run_norm(enn, ctx, norm_case(40, 520, "bf16", out, "rms", "rms", True, 3), rows=rows)
 
 
+@pytest.mark.parametrize("io,out", [("bf16", "bf16"), ("f16", "s8"), ("f32", "f32"), ("bf16", "f32"), ("f32", "s8")])
+@pytest.mark.parametrize("m,c", [(700, 4097), (900, 1001), (3000, 67), (400, 6150), (300, 9), (650, 2044), (310, 12301)])
+def test_token_norm_odd_widths_many_rows(enn, ctx, m, c, io, out):
+    run_norm(enn, ctx, norm_case(m, c, io, out, "layer", "rms", True, 50))
+    run_norm(enn, ctx, norm_case(m, c, io, out, "rms", "none", False))
+
+
+@pytest.mark.parametrize("x_off,r_off,g_off,h_off,y_off", [(1, 0, 0, 0, 0), (0, 3, 0, 0, 0), (5, 5, 5, 5, 5), (2, 2, 1, 2, 7), (0, 0, 0, 4, 0), (0, 0, 0, 0, 1)])
+def test_token_norm_tensors_on_different_lines(enn, ctx, x_off, r_off, g_off, h_off, y_off):
+    """Every tensor at an address of its own, rows of odd and even widths."""
+    for m, c, io, out in ((400, 515, "bf16", "bf16"), (30, 1024, "f16", "s8"), (310, 4096, "bf16", "s8"), (3, 32768, "f32", "f16")):
+        place = lambda t, off: torch.zeros(t.numel() + 16, dtype=t.dtype, device="cuda")[off:off + t.numel()].view(t.shape).copy_(t)      # noqa: E731
+        x, r, g = place(rand(1, m, c).to(TYPES[io]), x_off), place(rand(2, m, c).to(TYPES[io]), r_off), place(rand(3, -(-m // 7), c).to(TYPES[io]), g_off)
+        vectors = tuple(1 + 0.3 * rand(k, c) for k in range(4))
+        torch.cuda.synchronize()
+        d = enn.TokenNormDesc(m=m, c=c, norm=enn.NORM_LAYER, post_norm=enn.NORM_LAYER, residual=1, gate_tokens=7, io_dtype=code(enn, io), out_dtype=code(enn, out), eps=1e-6,
+                              post_eps=1e-6, residual_scale=0.5)
+        op = enn.token_norm(ctx, d, *[v.data_ptr() for v in vectors])
+        h = guarded(m, c, TYPES[io], h_off)
+        outs = [h, guarded(m, enn.token_pitch(c), torch.int8, y_off), guarded(m, 1, torch.float32)] if out == "s8" else [h, guarded(m, c, TYPES[out], y_off)]
+        execute(op, m, [x, r, g], outs)
+        op.release()
+        stream, (y, err) = norm_reference(norm_case(m, c, io, out, "layer", "layer", True, 7), x, r, g, vectors, 0.5, float(np.float32(1e-6)))
+        check_close(h[:m], *stream, io)
+        if out == "s8":
+            check_bytes(outs[1][:m], outs[2][:m, 0], y, err, c)
+        else:
+            check_close(outs[1][:m], y, err, out)
+
+
 def test_token_norm_many_rows(enn, ctx):
     run_norm(enn, ctx, norm_case(5000, 72, "f32", "s8", "layer", "none", True, 64))
     run_norm(enn, ctx, norm_case(3000, 1536, "bf16", "bf16", "rms", "rms", True))
@@ -475,6 +505,14 @@ def test_token_gate_activations(enn, ctx, act, out, packed):
 @pytest.mark.parametrize("out", ["bf16", "s8"])
 def test_token_gate_widest_rows(enn, ctx, c, out):
     run_gate(enn, ctx, 2, c, "bf16", out, "silu", True)
+
+
+@pytest.mark.parametrize("out", ["bf16", "s8"])
+@pytest.mark.parametrize("packed", [True, False])
+@pytest.mark.parametrize("m,c", [(700, 4099), (900, 1001), (2500, 67), (300, 9), (650, 2044), (40, 8193), (5, 40001)])
+def test_token_gate_odd_widths_many_rows(enn, ctx, m, c, packed, out):
+    run_gate(enn, ctx, m, c, "bf16", out, "silu", packed)
+    run_gate(enn, ctx, min(m, 100), c, "f32", out, "gelu_tanh", packed)
 
 
 def test_token_gate_many_rows(enn, ctx):
