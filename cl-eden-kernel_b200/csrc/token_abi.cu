@@ -62,15 +62,18 @@ struct Building {
         e = cudaMemcpy2DAsync(*dst, pitch, src, width, width, height, cudaMemcpyDefault, op->ctx->stream);
         return e == cudaSuccess ? cudaStreamSynchronize(op->ctx->stream) : e;
     }
-    // `copies` times, copy i shifted by i floats within `stride`.
+    // `copies` times, copy i shifted by i floats within `stride`, zeros around each.
     cudaError_t vector(const float *src, int32_t n, const float **dst, int copies = 1, int32_t stride = 0) {
         if (!src) return cudaSuccess;
         op->info.algorithmic_bytes += int64_t{4} * n;
         const size_t bytes = sizeof(float) * static_cast<size_t>(n);
         float *d = nullptr;
-        cudaError_t e = cudaMalloc(&d, sizeof(float) * static_cast<size_t>(stride) * (copies - 1) + bytes + sizeof(float) * (copies - 1));
+        const size_t around = copies > 1 ? 16 : 0, all = bytes + sizeof(float) * (static_cast<size_t>(stride) * (copies - 1) + copies + 2 * around);
+        cudaError_t e = cudaMalloc(&d, all);
         if (e != cudaSuccess) return e;
         op->owned.push_back(d);
+        e = cudaMemsetAsync(d, 0, all, op->ctx->stream);
+        d += around;
         for (int i = 0; i < copies && e == cudaSuccess; ++i)
             e = cudaMemcpyAsync(d + static_cast<size_t>(i) * stride + i, src, bytes, cudaMemcpyDefault, op->ctx->stream);
         *dst = d;
@@ -155,7 +158,7 @@ int32_t enn_b200_token_norm_prepare(enn_b200_context *ctx, const enn_b200_token_
     p.gate_tokens = d->gate_tokens;
     p.eps = d->eps; p.post_eps = d->post_eps; p.residual_scale = d->residual_scale;
     p.pitch = token_pitch(d->c);
-    p.stride = (d->c + 3) / 4 * 4 + 4;
+    p.stride = (d->c + 3) / 4 * 4 + 16;
     cudaError_t e = b.vector(weight, d->c, &p.weight, 4, p.stride);
     if (e == cudaSuccess) e = b.vector(bias, d->c, &p.bias, 4, p.stride);
     if (e == cudaSuccess) e = b.vector(post_weight, d->c, &p.post_weight, 4, p.stride);

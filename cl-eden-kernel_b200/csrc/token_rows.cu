@@ -76,52 +76,68 @@ __device__ __forceinline__ uint32_t pack4_s8(const float *f, float inv) {
 template <int NV, bool LINES>
 struct Row {
     int n, tid, nt, skip;
+    int low, high;      // channels, counted from the row's first, that are the tensor's: those of its neighbours count
     __device__ __forceinline__ int at(int v, int j = 0) const { return (v * nt + tid) * kGroup + j - (LINES ? 0 : skip); }
     __device__ __forceinline__ bool any(int v) const { return at(v) < n; }
     __device__ __forceinline__ bool whole(int v) const { return LINES ? any(v) : at(v) >= 0 && at(v) + kGroup <= n; }
     __device__ __forceinline__ bool inside(int v, int j) const { return LINES ? any(v) : at(v, j) >= 0 && at(v, j) < n; }
+    // The group's line may be read as a whole.
+    __device__ __forceinline__ bool readable(int v) const { return LINES ? any(v) : any(v) && at(v) >= low && at(v) + kGroup <= high; }
+    // Nothing counts outside the row.
+    __device__ __forceinline__ void clear_outside(int v, float (&f)[8]) const {
+        if (LINES || whole(v)) return;
+#pragma unroll
+        for (int j = 0; j < kGroup; ++j) f[j] = inside(v, j) ? f[j] : 0.f;
+    }
     // The groups lie on lines of the tensor whose row begins at p.
     template <typename T> __device__ __forceinline__ bool lined(const T *p) const { return LINES || ((reinterpret_cast<uintptr_t>(p) - skip * sizeof(T)) & 15) == 0; }
     // Lays the groups out on the lines of the row at p.
-    template <typename T> __device__ __forceinline__ void lay_out(const T *p) { skip = LINES ? 0 : static_cast<int>((reinterpret_cast<uintptr_t>(p) & 15) / sizeof(T)); }
-
-    template <typename T> __device__ __forceinline__ Raw<T> group(const T *p, int v, bool on_lines) const {
-        Raw<T> r{};
-        if (whole(v) && on_lines) return ld8(p + at(v));
-        if constexpr (!LINES) {
-            T e[kGroup];
-            if (whole(v)) {
+    template <typename T> __device__ __forceinline__ void lay_out(const T *p) {
+        if (!LINES) skip = static_cast<int>((reinterpret_cast<uintptr_t>(p) & 15) / sizeof(T));
+    }
+    // Channels of the tensor before the row's first and after its last.  (Where the stream is updated in place, another block may be
+    // writing a neighbour's channels on a shared line: what is read of them is not used.)
+    __device__ __forceinline__ void bound(int64_t before, int64_t after) {
+        if (LINES) return;
+        low = -static_cast<int>(min(static_cast<int64_t>(kGroup), before));
+        high = n + static_cast<int>(min(static_cast<int64_t>(kGroup), after));
+    }
+    // Channel by channel, 0 outside.
+    template <typename T> __device__ __forceinline__ Raw<T> gather(const T *p, int v) const {
+        Raw<T> r;
+        T e[kGroup];
+        if (whole(v)) {
 #pragma unroll
-                for (int j = 0; j < kGroup; ++j) e[j] = p[at(v) + j];
-            } else {
+            for (int j = 0; j < kGroup; ++j) e[j] = p[at(v) + j];
+        } else {
 #pragma unroll
-                for (int j = 0; j < kGroup; ++j) e[j] = inside(v, j) ? p[at(v, j)] : from_float<T>(0.f);
-            }
-            __builtin_memcpy(&r, e, sizeof(e));
+            for (int j = 0; j < kGroup; ++j) e[j] = inside(v, j) ? p[at(v, j)] : from_float<T>(0.f);
         }
+        __builtin_memcpy(&r, e, sizeof(e));
         return r;
     }
+    // Past the row's ends what lies there; nothing where the thread has no channels.
     template <typename T> __device__ __forceinline__ void load(const T *p, Raw<T> (&held)[NV]) const {
         const bool on_lines = lined(p);
 #pragma unroll
-        for (int v = 0; v < NV; ++v) held[v] = group(p, v, on_lines);
+        for (int v = 0; v < NV; ++v) {
+            held[v] = Raw<T>{};
+            if (on_lines && readable(v)) held[v] = ld8(p + at(v));
+            else if (!LINES && any(v)) held[v] = gather(p, v);
+        }
     }
     // f(channel value, constant) over the thread's channels; nothing where the constant vector is not given.  A vector is kept four
-    // times, `stride` floats apart and each a float further along, so that the groups of any row lie on 16-byte lines of one of them.
+    // times, `stride` floats apart, each a float further along and zeros around it, so that the groups of any row lie on 16-byte lines of one.
     template <typename F> __device__ __forceinline__ void with(const float *p, int stride, float (&f)[NV][8], F apply) const {
         if (!p) return;
         const float *q = LINES ? p : p + (skip & 3) * stride + (skip & 3);
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
-            if (whole(v)) {
+            if (any(v)) {
                 const float4 a = __ldg(reinterpret_cast<const float4 *>(q + at(v))), b = __ldg(reinterpret_cast<const float4 *>(q + at(v)) + 1);
                 const float w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
 #pragma unroll
                 for (int j = 0; j < kGroup; ++j) f[v][j] = apply(f[v][j], w[j]);
-            } else if (!LINES) {
-#pragma unroll
-                for (int j = 0; j < kGroup; ++j)
-                    if (inside(v, j)) f[v][j] = apply(f[v][j], __ldg(p + at(v, j)));
             }
         }
     }
@@ -150,9 +166,14 @@ struct Row {
             if (whole(v) && words) {
                 *reinterpret_cast<uint2 *>(p + at(v)) = make_uint2(pack4_s8(f[v], inv), pack4_s8(f[v] + 4, inv));
             } else if (!LINES) {
+                if (whole(v)) {
 #pragma unroll
-                for (int j = 0; j < kGroup; ++j)
-                    if (inside(v, j)) p[at(v, j)] = static_cast<int8_t>(quantise(f[v][j], inv));
+                    for (int j = 0; j < kGroup; ++j) p[at(v) + j] = static_cast<int8_t>(quantise(f[v][j], inv));
+                } else {
+#pragma unroll
+                    for (int j = 0; j < kGroup; ++j)
+                        if (inside(v, j)) p[at(v, j)] = static_cast<int8_t>(quantise(f[v][j], inv));
+                }
             }
         }
     }
@@ -280,7 +301,7 @@ struct Ahead {
         if (!row.lined(p)) return;
 #pragma unroll
         for (int v = 0; v < NV; ++v)
-            if (row.whole(v))
+            if (row.readable(v))
 #pragma unroll
                 for (int i = 0; i < kPieces; ++i)
                     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at(s, stream, v, i)), "l"(reinterpret_cast<const uint4 *>(p + row.at(v)) + i) : "memory");
@@ -289,14 +310,15 @@ struct Ahead {
         const bool copied = row.lined(p);
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
-            if (row.whole(v) && copied) {
+            if (row.readable(v) && copied) {
 #pragma unroll
                 for (int i = 0; i < kPieces; ++i) {
                     uint4 &q = held[v].v[i];
                     asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(q.x), "=r"(q.y), "=r"(q.z), "=r"(q.w) : "r"(at(slot, stream, v, i)) : "memory");
                 }
             } else {
-                held[v] = row.any(v) ? row.group(p, v, false) : Raw<T>{};
+                held[v] = Raw<T>{};
+                if (!LINES && row.any(v)) held[v] = row.gather(p, v);
             }
         }
     }
@@ -318,7 +340,8 @@ __global__ void __launch_bounds__(max_threads(NV), min_blocks(NV)) token_norm_ke
     extern __shared__ __align__(16) uint8_t ring[];
     __shared__ float2 scratch[2][32];
     const int64_t step = static_cast<int64_t>(gridDim.x) * blockDim.y;
-    Row<NV, LINES> row{p.c, static_cast<int>(threadIdx.x), static_cast<int>(blockDim.x), 0};
+    Row<NV, LINES> row{p.c, static_cast<int>(threadIdx.x), static_cast<int>(blockDim.x), 0, 0, p.c};
+    const int64_t gate_rows = gate ? (rows - 1) / p.gate_tokens + 1 : 0;
     Reduce reduce{scratch, row.nt, 0};
     pdl_wait();
     pdl_trigger();
@@ -330,29 +353,41 @@ __global__ void __launch_bounds__(max_threads(NV), min_blocks(NV)) token_norm_ke
         if (t < rows) {
             Row<NV, LINES> r = row;
             r.lay_out(x + t * p.c);
+            r.bound(t * p.c, (rows - 1 - t) * p.c);
             ahead.fetch(r, s, 0, x + t * p.c);
             if (residual) ahead.fetch(r, s, 1, residual + t * p.c);
-            if (gate) ahead.fetch(r, s, ahead.streams - 1, gate + t / p.gate_tokens * p.c);
+            if (gate) {
+                const int64_t tg = t / p.gate_tokens;
+                r.bound(tg * p.c, (gate_rows - 1 - tg) * p.c);
+                ahead.fetch(r, s, ahead.streams - 1, gate + tg * p.c);
+            }
         }
         ahead_commit();
     };
-    auto take = [&](int which, const T *p_row, float (&f)[NV][8]) {
+    auto take = [&](const Row<NV, LINES> &r, int which, const T *p_row, float (&f)[NV][8]) {
         Raw<T> held[NV];
-        if (depth) ahead.read(row, which, p_row, held);
-        else row.load(p_row, held);
+        if (depth) ahead.read(r, which, p_row, held);
+        else r.load(p_row, held);
 #pragma unroll
-        for (int v = 0; v < NV; ++v) widen(held[v], f[v]);
+        for (int v = 0; v < NV; ++v) {
+            widen(held[v], f[v]);
+            r.clear_outside(v, f[v]);
+        }
     };
     for (int s = 0; s < depth; ++s) fetch(s, first + s * step);
     for (int64_t t = first; t < rows; t += step) {      // t is the same for a whole warp, and for the whole block where a row has several warps
         float f[NV][8];
         row.lay_out(x + t * p.c);
+        row.bound(t * p.c, (rows - 1 - t) * p.c);
         if (depth) ahead_wait(depth - 1);
-        take(0, x + t * p.c, f);
+        take(row, 0, x + t * p.c, f);
         norm_row(row, f, p.c, p.post_norm, p.post_eps, p.post_weight, p.post_bias, p.stride, reduce, nullptr);
         if (gate) {
             float g[NV][8];
-            take(ahead.streams - 1, gate + t / p.gate_tokens * p.c, g);
+            const int64_t tg = t / p.gate_tokens;
+            Row<NV, LINES> r = row;
+            r.bound(tg * p.c, (gate_rows - 1 - tg) * p.c);
+            take(r, ahead.streams - 1, gate + tg * p.c, g);
 #pragma unroll
             for (int v = 0; v < NV; ++v)
 #pragma unroll
@@ -360,7 +395,7 @@ __global__ void __launch_bounds__(max_threads(NV), min_blocks(NV)) token_norm_ke
         }
         if (residual) {
             float r[NV][8];
-            take(1, residual + t * p.c, r);
+            take(row, 1, residual + t * p.c, r);
 #pragma unroll
             for (int v = 0; v < NV; ++v)
 #pragma unroll
@@ -424,6 +459,8 @@ __device__ __forceinline__ void gate_row(const Row<NV, LINES> &row, const T *gat
             float g[8], u[8];
             widen(rg[v], g);
             widen(ru[v], u);
+            row.clear_outside(v, u);
+            row.clear_outside(v, g);
 #pragma unroll
             for (int j = 0; j < kGroup; ++j) f[v][j] = gate_act<decltype(which)::value>(g[j]) * u[j];
         }
@@ -446,7 +483,7 @@ __global__ void __launch_bounds__(max_threads(NV)) token_gate_kernel(GateParams 
     __shared__ uint32_t of_cluster[8];
     const int64_t t = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
     const int32_t segs = static_cast<int32_t>(gridDim.y), rank = static_cast<int32_t>(blockIdx.y), c0 = rank * seg;
-    Row<NV, LINES> row{min(seg, p.c - c0), static_cast<int>(threadIdx.x), static_cast<int>(blockDim.x), 0};
+    Row<NV, LINES> row{min(seg, p.c - c0), static_cast<int>(threadIdx.x), static_cast<int>(blockDim.x), 0, 0, 0};
     // Seen by the others of the cluster before they write here: waited for below.
     const bool clustered = segs > 1 && out_dtype == ENN_B200_S8;
     if (clustered) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
@@ -455,6 +492,7 @@ __global__ void __launch_bounds__(max_threads(NV)) token_gate_kernel(GateParams 
     if (t >= rows) return;      // a whole warp, and then the block has no barrier
     float f[NV][8];
     row.lay_out(gates + t * p.in_stride + c0);
+    row.bound(t * p.in_stride + c0, (rows - 1 - t) * p.in_stride + (p.c - c0 - row.n));      // of the gates or of the values, whichever is less
     gate_row(row, gates + t * p.in_stride + c0, values + t * p.in_stride + c0, p.act, f);
     if (out_dtype != ENN_B200_S8) {
         row.store_as(out_dtype, out, t * p.c + c0, f);
