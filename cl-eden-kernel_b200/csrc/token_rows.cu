@@ -85,9 +85,11 @@ struct Row {
     __device__ __forceinline__ bool readable(int v) const { return LINES ? any(v) : any(v) && at(v) >= low && at(v) + kGroup <= high; }
     // Nothing counts outside the row.
     __device__ __forceinline__ void clear_outside(int v, float (&f)[8]) const {
-        if (LINES || whole(v)) return;
+        if constexpr (!LINES) {
+            if (whole(v)) return;
 #pragma unroll
-        for (int j = 0; j < kGroup; ++j) f[j] = inside(v, j) ? f[j] : 0.f;
+            for (int j = 0; j < kGroup; ++j) f[j] = inside(v, j) ? f[j] : 0.f;
+        }
     }
     // The groups lie on lines of the tensor whose row begins at p.
     template <typename T> __device__ __forceinline__ bool lined(const T *p) const { return LINES || ((reinterpret_cast<uintptr_t>(p) - skip * sizeof(T)) & 15) == 0; }
@@ -99,21 +101,35 @@ struct Row {
     // writing a neighbour's channels on a shared line: what is read of them is not used.)
     __device__ __forceinline__ void bound(int64_t before, int64_t after) {
         if (LINES) return;
-        low = -static_cast<int>(min(static_cast<int64_t>(kGroup), before));
-        high = n + static_cast<int>(min(static_cast<int64_t>(kGroup), after));
+        low = -static_cast<int>(min(static_cast<int64_t>(2 * kGroup), before));
+        high = n + static_cast<int>(min(static_cast<int64_t>(2 * kGroup), after));
     }
-    // Channel by channel, 0 outside.
-    template <typename T> __device__ __forceinline__ Raw<T> gather(const T *p, int v) const {
+    // A group that lies across lines: put together from those, or channel by channel (0 outside) where they are not the tensor's.
+    template <typename T> __device__ __forceinline__ Raw<T> across(const T *p, int v) const {
+        constexpr int W = static_cast<int>(sizeof(T)) * 2, L = W / 4 + 1;      // words of a group, lines it touches
+        const int off = static_cast<int>(reinterpret_cast<uintptr_t>(p + at(v)) & 15), before = off / static_cast<int>(sizeof(T));
         Raw<T> r;
-        T e[kGroup];
-        if (whole(v)) {
+        if (at(v) - before >= low && at(v) - before + L * 16 / static_cast<int>(sizeof(T)) <= high) {
+            uint32_t w[4 * L];
 #pragma unroll
-            for (int j = 0; j < kGroup; ++j) e[j] = p[at(v) + j];
+            for (int i = 0; i < L; ++i) {
+                const uint4 q = ld_stream(reinterpret_cast<const uint4 *>(p + at(v) - before) + i);
+                w[4 * i] = q.x; w[4 * i + 1] = q.y; w[4 * i + 2] = q.z; w[4 * i + 3] = q.w;
+            }
+#pragma unroll
+            for (int i = 0; i < 4 * L - 2; ++i) w[i] = off & 8 ? w[i + 2] : w[i];
+#pragma unroll
+            for (int i = 0; i < 4 * L - 3; ++i) w[i] = off & 4 ? w[i + 1] : w[i];
+            uint32_t out[W];
+#pragma unroll
+            for (int i = 0; i < W; ++i) out[i] = sizeof(T) == 2 ? __funnelshift_r(w[i], w[i + 1], off & 2 ? 16 : 0) : w[i];
+            __builtin_memcpy(&r, out, sizeof(out));
         } else {
+            T e[kGroup];
 #pragma unroll
             for (int j = 0; j < kGroup; ++j) e[j] = inside(v, j) ? p[at(v, j)] : from_float<T>(0.f);
+            __builtin_memcpy(&r, e, sizeof(e));
         }
-        __builtin_memcpy(&r, e, sizeof(e));
         return r;
     }
     // Past the row's ends what lies there; nothing where the thread has no channels.
@@ -123,7 +139,7 @@ struct Row {
         for (int v = 0; v < NV; ++v) {
             held[v] = Raw<T>{};
             if (on_lines && readable(v)) held[v] = ld8(p + at(v));
-            else if (!LINES && any(v)) held[v] = gather(p, v);
+            else if (!LINES && any(v)) held[v] = across(p, v);
         }
     }
     // f(channel value, constant) over the thread's channels; nothing where the constant vector is not given.  A vector is kept four
@@ -318,7 +334,7 @@ struct Ahead {
                 }
             } else {
                 held[v] = Raw<T>{};
-                if (!LINES && row.any(v)) held[v] = row.gather(p, v);
+                if (!LINES && row.any(v)) held[v] = row.across(p, v);
             }
         }
     }
@@ -491,7 +507,10 @@ __global__ void __launch_bounds__(max_threads(NV)) token_gate_kernel(GateParams 
     pdl_trigger();
     if (t >= rows) return;      // a whole warp, and then the block has no barrier
     float f[NV][8];
-    row.lay_out(gates + t * p.in_stride + c0);
+    // Groups on the lines of the results, which are stored as a whole; gates and values are put together where theirs are others.
+    if (out_dtype == ENN_B200_S8) row.skip = static_cast<int>(reinterpret_cast<uintptr_t>(static_cast<int8_t *>(out) + t * p.pitch + c0) & 7);
+    else if (out_dtype == ENN_B200_F32) row.lay_out(static_cast<float *>(out) + t * p.c + c0);
+    else row.lay_out(static_cast<uint16_t *>(out) + t * p.c + c0);
     row.bound(t * p.in_stride + c0, (rows - 1 - t) * p.in_stride + (p.c - c0 - row.n));      // of the gates or of the values, whichever is less
     gate_row(row, gates + t * p.in_stride + c0, values + t * p.in_stride + c0, p.act, f);
     if (out_dtype != ENN_B200_S8) {
@@ -527,7 +546,7 @@ Shape row_shape(int n, bool lines, bool spread) {
     auto threads = [&](int nv) { return ((groups + nv - 1) / nv + 31) / 32 * 32; };
     Shape s;
     if (groups <= 32 || (spread && groups <= 1024)) s.nv = 1;
-    else if (groups <= 64) s.nv = 2;
+    else if (groups <= 64 || (!lines && groups <= 1024)) s.nv = 2;      // (the code for shifted groups is long: four of them overflow the instruction cache)
     else s.nv = groups <= 1024 ? 4 : 8;
     s.nt = threads(s.nv);
     s.per_block = s.nt == 32 ? 8 : 1;
