@@ -348,7 +348,8 @@ __device__ __forceinline__ void ahead_wait(int pending) {
     else asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 constexpr int kMaxDepth = 4;
-constexpr int kRingBytes = 216 * 1024;
+constexpr int kRingBytes = 216 * 1024;      // at most
+constexpr int kRingShare = 112 * 1024;      // of an SM: what they take, L1 lacks for the constant vectors (8192x5120: 65 us with all of it, 61 us so)
 
 template <typename T, int NV, bool LINES>
 __global__ void __launch_bounds__(max_threads(NV), min_blocks(NV)) token_norm_kernel(NormParams p, int32_t rows, int32_t out_dtype, int32_t depth, const T *x,
@@ -584,7 +585,7 @@ cudaError_t norm_typed(const enn_b200_op *op, int32_t rows, const void *const *i
     const int threads = s.nt * s.per_block;
     const int blocks = std::max(1, max_threads(s.nv) * min_blocks(s.nv) / threads);
     const int ahead_bytes = threads * s.nv * kGroup * static_cast<int>(sizeof(T)) * (1 + (residual != nullptr) + (gate != nullptr));
-    const int depth = ahead_bytes > kRingBytes ? 0 : std::min(kMaxDepth, std::max(1, kRingBytes / blocks / ahead_bytes));
+    const int depth = ahead_bytes > kRingBytes ? 0 : std::min(kMaxDepth, std::max(1, kRingShare / blocks / ahead_bytes));
     const int64_t want = (static_cast<int64_t>(rows) + s.per_block - 1) / s.per_block, most = static_cast<int64_t>(op->ctx->launch_sms()) * blocks;
     const dim3 grid(static_cast<unsigned>(std::min(want, most))), block(static_cast<unsigned>(s.nt), static_cast<unsigned>(s.per_block));
     return with_shape(s.nv, lines, [&](auto nv, auto v) {
