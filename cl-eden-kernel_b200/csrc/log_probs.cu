@@ -11,6 +11,7 @@
 #include <math_constants.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "per_device.h"
 #include "tc_common.cuh"
@@ -19,13 +20,16 @@
 namespace enn_b200 {
 namespace {
 
-constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kMaxTop = ENN_B200_LOG_PROBS_MAX_TOP;
 constexpr int kMaxSegments = 8;
 constexpr int kChunk = 4;               // 16-byte pieces a thread works on at a time
-constexpr int kDepth = 3;               // chunks a thread asks for ahead
-constexpr int kBlocks = 3;              // CTAs an SM is to hold
+constexpr int kDepth = 2;               // chunks a thread asks for ahead
 constexpr int kCandidates = 1024;
+// Threads of a CTA: kLong, or kShort for many short rows, whose time is that of the reductions and of the search, one step after the
+// other: more rows side by side.  And the CTAs an SM is to hold.
+constexpr int kLong = 256, kShort = 64;
+constexpr int kShortBytes = 16384;       // of a short row
+constexpr int blocks_of(int threads) { return threads == kLong ? 3 : 8; }
 constexpr int kLookers = 8;             // threads that look at one thread's logits again
 constexpr float kNothing = -1e4f;       // 2^-10000 is 0; keeps the products d 2^d away from infinity times 0
 constexpr float kSlack = 20.f;
@@ -193,7 +197,9 @@ __device__ __forceinline__ void take_largest(const uint64_t *lists, int n_lists,
     }
 }
 
+template <int kThreads>
 struct Shared {
+    static constexpr int kWarps = kThreads / 32;
     float part[3][kWarps];
     uint64_t of_warp[kWarps];
     uint64_t firsts[kWarps * (kMaxTop / kWarps + 2)], bound;
@@ -214,8 +220,9 @@ __device__ __forceinline__ V warp_join(V v, F join) {
 }
 
 // Round by round over the whole segment: for rows with NaN or +inf, and where more candidates turn up than there is room for.
-template <typename T>
-__device__ __noinline__ void largest_by_rounds(const Segment<T> &seg, int top, Shared &sh) {
+template <int kThreads, typename T>
+__device__ __noinline__ void largest_by_rounds(const Segment<T> &seg, int top, Shared<kThreads> &sh) {
+    constexpr int kWarps = kThreads / 32;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     uint64_t below = ~0ull;
     for (int r = 0; r < top; ++r) {
@@ -241,8 +248,8 @@ __device__ __noinline__ void largest_by_rounds(const Segment<T> &seg, int top, S
 
 // The logits of the threads whose maximum reaches `least`, as far as they reach it themselves, into sh.candidates.  `mine`: a key of the
 // thread's maximum.  Returns their number, which may be above what there is room for.
-template <typename T>
-__device__ __forceinline__ int collect(const Segment<T> &seg, uint64_t mine, uint64_t least, Shared &sh) {
+template <int kThreads, typename T>
+__device__ __forceinline__ int collect(const Segment<T> &seg, uint64_t mine, uint64_t least, Shared<kThreads> &sh) {
     if (threadIdx.x == 0) sh.n_candidates = sh.n_lookups = 0;
     __syncthreads();
     if (mine && mine >= least) sh.lookups[atomicAdd(&sh.n_lookups, 1)] = threadIdx.x;
@@ -269,7 +276,9 @@ __device__ __forceinline__ int collect(const Segment<T> &seg, uint64_t mine, uin
 
 // A key that `top` of the keys `mine` of the threads reach, 0 if fewer of them have one: the top-th largest among the first few of every
 // warp, two more than would do, so that hardly more threads than `top` reach it.
-__device__ __forceinline__ uint64_t reached_by(uint64_t mine, int top, Shared &sh) {
+template <int kThreads>
+__device__ __forceinline__ uint64_t reached_by(uint64_t mine, int top, Shared<kThreads> &sh) {
+    constexpr int kWarps = kThreads / 32;
     const int rounds = min(top, (top + kWarps - 1) / kWarps + 2), n = rounds * kWarps;
     __syncthreads();
     for (int r = 0; r < rounds; ++r) {
@@ -281,7 +290,7 @@ __device__ __forceinline__ uint64_t reached_by(uint64_t mine, int top, Shared &s
         }
     }
     __syncthreads();
-    if (static_cast<int>(threadIdx.x) < n) {
+    if (static_cast<int>(threadIdx.x) < n) {      // at most 36 keys
         const uint64_t k = sh.firsts[threadIdx.x];
         int place = 0;
         for (int j = 0; j < n; ++j) {
@@ -295,8 +304,8 @@ __device__ __forceinline__ uint64_t reached_by(uint64_t mine, int top, Shared &s
 }
 
 // sh.sorted[0 .. top): the largest keys of a segment without NaN.  `best`: the thread's largest logit.
-template <typename T>
-__device__ __forceinline__ void largest_of_segment(const Segment<T> &seg, float best, int top, Shared &sh) {
+template <int kThreads, typename T>
+__device__ __forceinline__ void largest_of_segment(const Segment<T> &seg, float best, int top, Shared<kThreads> &sh) {
     const bool has = static_cast<int32_t>(threadIdx.x) < seg.pieces;
     // By value first: all that equal the bound are candidates.
     uint64_t mine = has ? order_key(best, -1) : 0;
@@ -332,11 +341,12 @@ __device__ __forceinline__ void largest_of_segment(const Segment<T> &seg, float 
 
 // Grid: rows x segments, the segments of a row being a cluster.  Where rows have one segment a CTA takes several of them, and the copies
 // of the next row's first chunks are under way while the alternatives of this one are sorted out.
-template <typename T>
-__global__ void __launch_bounds__(kThreads, kBlocks) log_probs_kernel(LogProbsParams p, int32_t rows, int32_t seg_size, const T *logits, const int32_t *ids, float *given,
+template <typename T, int kThreads>
+__global__ void __launch_bounds__(kThreads, blocks_of(kThreads)) log_probs_kernel(LogProbsParams p, int32_t rows, int32_t seg_size, const T *logits, const int32_t *ids, float *given,
                                                                       float *entropy, int32_t *top_ids, float *top) {
     extern __shared__ __align__(16) uint8_t ring[];      // [kDepth][kChunk][kThreads] pieces: a thread reads what it copied itself
-    __shared__ Shared sh;
+    __shared__ Shared<kThreads> sh;
+    constexpr int kWarps = kThreads / 32;
     constexpr int E = Segment<T>::E;
     constexpr int kStep = kThreads * kChunk;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -521,28 +531,33 @@ cudaError_t launch_typed(const enn_b200_op *op, int32_t rows, const void *const 
     int32_t *top_ids = p.top ? static_cast<int32_t *>(outs[o++]) : nullptr;
     float *top = p.top ? static_cast<float *>(outs[o++]) : nullptr;
     // Segments while the device has room for them and a segment keeps a chunk for every thread.
-    const int64_t slots = static_cast<int64_t>(kBlocks) * op->ctx->sm_count;
+    const int64_t sms = op->ctx->sm_count;
     int segs = 1;
-    while (segs < kMaxSegments && static_cast<int64_t>(rows) * segs * 2 <= slots && p.vocab / (segs * 2) >= 4096) segs *= 2;
+    while (segs < kMaxSegments && static_cast<int64_t>(rows) * segs * 2 <= blocks_of(kLong) * sms && p.vocab / (segs * 2) >= 4096) segs *= 2;
     const int32_t seg_size = (p.vocab + segs - 1) / segs;
-    static PerDeviceInit once;
-    constexpr int kRing = kDepth * kChunk * kThreads * 16;
-    const cudaError_t e = once.run(op->ctx->device, [] { return cudaFuncSetAttribute(log_probs_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRing); });
-    if (e != cudaSuccess) return e;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(static_cast<unsigned>(segs > 1 ? rows : std::min<int64_t>(rows, slots)), static_cast<unsigned>(segs));
-    cfg.dynamicSmemBytes = kRing;
-    cfg.blockDim = dim3(kThreads);
-    cfg.stream = op->ctx->stream;
-    cudaLaunchAttribute attr[2] = {};
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = attr[1].val.clusterDim.z = 1;
-    attr[1].val.clusterDim.y = static_cast<unsigned>(segs);
-    cfg.attrs = attr;
-    cfg.numAttrs = segs > 1 ? 2 : 1;
-    return cudaLaunchKernelEx(&cfg, log_probs_kernel<T>, p, rows, seg_size, static_cast<const T *>(ins[0]), ids, given, entropy, top_ids, top);
+    const auto run = [&](auto threads) {
+        constexpr int kThreads = decltype(threads)::value, kRing = kDepth * kChunk * kThreads * 16;
+        constexpr auto kernel = log_probs_kernel<T, kThreads>;
+        static PerDeviceInit once;
+        const cudaError_t e = once.run(op->ctx->device, [&] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRing); });
+        if (e != cudaSuccess) return e;
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3(static_cast<unsigned>(segs > 1 ? rows : std::min<int64_t>(rows, blocks_of(kThreads) * sms)), static_cast<unsigned>(segs));
+        cfg.blockDim = dim3(kThreads);
+        cfg.dynamicSmemBytes = kRing;
+        cfg.stream = op->ctx->stream;
+        cudaLaunchAttribute attr[2] = {};
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
+        attr[1].id = cudaLaunchAttributeClusterDimension;
+        attr[1].val.clusterDim.x = attr[1].val.clusterDim.z = 1;
+        attr[1].val.clusterDim.y = static_cast<unsigned>(segs);
+        cfg.attrs = attr;
+        cfg.numAttrs = segs > 1 ? 2 : 1;
+        return cudaLaunchKernelEx(&cfg, kernel, p, rows, seg_size, static_cast<const T *>(ins[0]), ids, given, entropy, top_ids, top);
+    };
+    if (rows > blocks_of(kLong) * sms && p.vocab * static_cast<int64_t>(sizeof(T)) <= kShortBytes) return run(std::integral_constant<int, kShort>{});
+    return run(std::integral_constant<int, kLong>{});
 }
 
 }  // namespace

@@ -491,10 +491,12 @@ __device__ __forceinline__ void gate_row(const Row<NV, LINES> &row, const T *gat
     }
 }
 
+constexpr int gate_threads(int nv) { return nv == 4 ? 512 : max_threads(nv); }
+
 // Grid: rows x segments of `seg` channels.  Floats leave at once.  Bytes need the row's largest magnitude first: the
 // segments of a row are then the CTAs of a cluster, which tell each other theirs.
 template <typename T, int NV, bool LINES>
-__global__ void __launch_bounds__(max_threads(NV)) token_gate_kernel(GateParams p, int32_t rows, int32_t seg, int32_t out_dtype, const T *gates, const T *values,
+__global__ void __launch_bounds__(gate_threads(NV)) token_gate_kernel(GateParams p, int32_t rows, int32_t seg, int32_t out_dtype, const T *gates, const T *values,
                                                                  void *out, float *scale) {
     __shared__ float2 scratch[2][32];
     __shared__ uint32_t of_cluster[8];
@@ -538,17 +540,18 @@ __global__ void __launch_bounds__(max_threads(NV)) token_gate_kernel(GateParams 
 bool aligned(const void *p, size_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
 
 // Threads of a row and groups per thread for `n` channels.  `spread`: as many threads as there are groups (few rows: latency), else
-// four groups each (many rows: what a row costs whatever its length, reductions and addresses, is shared by more channels).
+// four groups each (many rows: what a row costs whatever its length, reductions and addresses, is shared by more channels), up to
+// `most_by_four` threads.
 struct Shape {
     int nt, nv, per_block;
 };
-Shape row_shape(int n, bool lines, bool spread) {
+Shape row_shape(int n, bool lines, bool spread, int most_by_four) {
     const int groups = (n + (lines ? 0 : kGroup - 1) + kGroup - 1) / kGroup;      // one more where they are shifted
     auto threads = [&](int nv) { return ((groups + nv - 1) / nv + 31) / 32 * 32; };
     Shape s;
     if (groups <= 32 || (spread && groups <= 1024)) s.nv = 1;
     else if (groups <= 64 || (!lines && groups <= 1024)) s.nv = 2;      // (the code for shifted groups is long: four of them overflow the instruction cache)
-    else s.nv = groups <= 1024 ? 4 : 8;
+    else s.nv = groups <= 4 * most_by_four ? 4 : 8;
     s.nt = threads(s.nv);
     s.per_block = s.nt == 32 ? 8 : 1;
     return s;
@@ -579,7 +582,7 @@ cudaError_t norm_typed(const enn_b200_op *op, int32_t rows, const void *const *i
     void *y = outs[o++];
     float *scale = t.out_dtype == ENN_B200_S8 ? static_cast<float *>(outs[o++]) : nullptr;
     const bool lines = p.c % kGroup == 0 && aligned(x, 16) && aligned(residual, 16) && aligned(gate, 16) && aligned(stream, 16) && aligned(y, scale ? 8 : 16);
-    const Shape s = row_shape(p.c, lines, rows <= 2 * op->ctx->sm_count);
+    const Shape s = row_shape(p.c, lines, rows <= 2 * op->ctx->sm_count, max_threads(4));
     // As many blocks as an SM holds, each taking rows in turn, and rings of up to four rows in what shared memory
     // that leaves them; the widest rows of 32-bit types do without.
     const int threads = s.nt * s.per_block;
@@ -608,10 +611,10 @@ cudaError_t gate_typed(const enn_b200_op *op, int32_t rows, const void *const *i
     int segs = 1;
     if (!bytes) segs = (p.c + 8191) / 8192;
     else
-        while (segs < 8 && (p.c > 8192 * segs || (static_cast<int64_t>(rows) * segs * 2 <= 2 * op->ctx->sm_count && p.c >= 2048 * segs))) segs *= 2;
+        while (segs < 8 && (p.c > 16384 * segs || (static_cast<int64_t>(rows) * segs * 2 <= 2 * op->ctx->sm_count && p.c >= 2048 * segs))) segs *= 2;
     const int seg = segs == 1 ? p.c : ((p.c + segs - 1) / segs + kGroup - 1) / kGroup * kGroup;
     if (!bytes) segs = (p.c + seg - 1) / seg;
-    const Shape s = row_shape(seg, lines, static_cast<int64_t>(rows) * segs <= 2 * op->ctx->sm_count);
+    const Shape s = row_shape(seg, lines, static_cast<int64_t>(rows) * segs <= 2 * op->ctx->sm_count, gate_threads(4));
     const int per_block = segs > 1 && bytes ? 1 : s.per_block;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(static_cast<unsigned>((static_cast<int64_t>(rows) + per_block - 1) / per_block), static_cast<unsigned>(segs));
