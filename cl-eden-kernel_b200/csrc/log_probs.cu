@@ -531,7 +531,7 @@ cudaError_t launch_typed(const enn_b200_op *op, int32_t rows, const void *const 
     int32_t *top_ids = p.top ? static_cast<int32_t *>(outs[o++]) : nullptr;
     float *top = p.top ? static_cast<float *>(outs[o++]) : nullptr;
     // Segments while the device has room for them and a segment keeps a chunk for every thread.
-    const int64_t sms = op->ctx->sm_count;
+    const int64_t sms = op->token->sms;
     int segs = 1;
     while (segs < kMaxSegments && static_cast<int64_t>(rows) * segs * 2 <= blocks_of(kLong) * sms && p.vocab / (segs * 2) >= 4096) segs *= 2;
     const int32_t seg_size = (p.vocab + segs - 1) / segs;

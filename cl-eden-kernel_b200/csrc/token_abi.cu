@@ -12,6 +12,11 @@ int32_t tfail(enn_b200_context *ctx, int32_t st, const char *msg) {
     return st;
 }
 
+int32_t cfail(enn_b200_context *ctx, cudaError_t e) {
+    if (ctx) ctx->last_error = std::string("token operator: ") + cudaGetErrorString(e);
+    return ENN_B200_CUDA_FAILURE;
+}
+
 // The device of the context for the length of a call; the caller's current device is put back.
 class OnDevice {
   public:
@@ -46,6 +51,7 @@ struct Building {
         op->token = new (std::nothrow) TokenState();
         if (!op->token) return false;
         op->token->call = call;
+        op->token->sms = ctx->launch_sms();
         for (int i = 0; i < call.n_in; ++i) op->info.in_bytes += call.in_bytes[i];
         for (int o = 0; o < call.n_out; ++o) op->info.out_bytes += call.out_bytes[o];
         op->info.algorithmic_bytes = op->info.in_bytes + op->info.out_bytes;
@@ -53,14 +59,21 @@ struct Building {
         op->info.out_h = op->info.out_w = 1;
         return true;
     }
-    // `width` bytes of each of `height` rows, from host or device memory, into an allocation of the operator with `pitch` bytes per row.
-    cudaError_t constant(const void *src, size_t width, size_t height, size_t pitch, void **dst) {
-        cudaError_t e = cudaMalloc(dst, height * pitch);
+    // `width` bytes of each of `height` rows, from host or device memory, into an allocation of the operator with `pitch` bytes per row,
+    // zeros beyond the width.  (A two-dimensional copy of odd widths takes milliseconds for a few thousand rows.)
+    cudaError_t rows(const void *src, int32_t width, int32_t height, int64_t pitch, void **dst) {
+        const size_t bytes = static_cast<size_t>(width) * height;
+        cudaError_t e = cudaMalloc(dst, static_cast<size_t>(pitch) * height);
         if (e != cudaSuccess) return e;
         op->owned.push_back(*dst);
-        if (width != pitch && (e = cudaMemsetAsync(*dst, 0, height * pitch, op->ctx->stream)) != cudaSuccess) return e;
-        e = cudaMemcpy2DAsync(*dst, pitch, src, width, width, height, cudaMemcpyDefault, op->ctx->stream);
-        return e == cudaSuccess ? cudaStreamSynchronize(op->ctx->stream) : e;
+        if (width == pitch) return cudaMemcpyAsync(*dst, src, bytes, cudaMemcpyDefault, op->ctx->stream);
+        void *dense = nullptr;
+        if ((e = cudaMalloc(&dense, bytes)) != cudaSuccess) return e;
+        e = cudaMemcpyAsync(dense, src, bytes, cudaMemcpyDefault, op->ctx->stream);
+        if (e == cudaSuccess) e = launch_pad_rows(dense, width, height, pitch, *dst, op->ctx->stream);
+        const cudaError_t done = cudaStreamSynchronize(op->ctx->stream);
+        cudaFree(dense);
+        return e == cudaSuccess ? done : e;
     }
     // `copies` times, copy i shifted by i floats within `stride`, zeros around each.
     cudaError_t vector(const float *src, int32_t n, const float **dst, int copies = 1, int32_t stride = 0) {
@@ -77,19 +90,17 @@ struct Building {
         for (int i = 0; i < copies && e == cudaSuccess; ++i)
             e = cudaMemcpyAsync(d + static_cast<size_t>(i) * stride + i, src, bytes, cudaMemcpyDefault, op->ctx->stream);
         *dst = d;
-        return e == cudaSuccess ? cudaStreamSynchronize(op->ctx->stream) : e;
+        return e;
     }
+    // Hands the operator out once its constants have arrived: their sources may go then.
     int32_t finish(enn_b200_op **out) {
+        const cudaError_t e = op->owned.empty() ? cudaSuccess : cudaStreamSynchronize(op->ctx->stream);
+        if (e != cudaSuccess) return cfail(op->ctx, e);
         *out = op;
         op = nullptr;
         return ENN_B200_SUCCESS;
     }
 };
-
-int32_t cfail(enn_b200_context *ctx, cudaError_t e) {
-    if (ctx) ctx->last_error = std::string("token operator: ") + cudaGetErrorString(e);
-    return ENN_B200_CUDA_FAILURE;
-}
 
 }  // namespace
 
@@ -123,7 +134,7 @@ int32_t enn_b200_token_fc_prepare(enn_b200_context *ctx, const enn_b200_token_fc
     t.fc.in_pitch = d->in_pitch ? d->in_pitch : token_pitch(d->k);
     t.fc.w_pitch = token_pitch(d->k);
     void *w = nullptr;
-    cudaError_t e = b.constant(weights, static_cast<size_t>(d->k), static_cast<size_t>(d->n), static_cast<size_t>(t.fc.w_pitch), &w);
+    cudaError_t e = b.rows(weights, d->k, d->n, t.fc.w_pitch, &w);
     t.fc.w = static_cast<const int8_t *>(w);
     if (e == cudaSuccess) e = b.vector(channel_scales, d->n, &t.fc.channel_scale);
     if (e == cudaSuccess) e = b.vector(bias, d->n, &t.fc.bias);

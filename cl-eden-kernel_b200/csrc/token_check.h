@@ -28,6 +28,8 @@ struct TokenCall {
     }
 };
 
+constexpr int32_t kMostRows = 1 << 30;
+
 inline int32_t float_size(int32_t dtype) {
     return dtype == ENN_B200_F32 ? 4 : (dtype == ENN_B200_F16 || dtype == ENN_B200_BF16 ? 2 : 0);
 }
@@ -36,7 +38,7 @@ inline int64_t token_pitch(int32_t c) { return (static_cast<int64_t>(c) + 15) & 
 
 // The check_* return null and fill `call`, or what is wrong with the descriptor.
 inline const char *check_token_fc(const enn_b200_token_fc_desc &d, TokenCall *call) {
-    if (d.m < 0 || d.k <= 0 || d.n <= 0 || d.n > (1 << 21)) return "token_fc: bad shape (n is 1 .. 2^21)";
+    if (d.m < 0 || d.m > kMostRows || d.k <= 0 || d.n <= 0 || d.n > (1 << 21)) return "token_fc: bad shape (n is 1 .. 2^21)";
     if (d.k >= 131072) return "token_fc: k must be below 131072 (sums of products are 32-bit)";
     const int32_t e = float_size(d.out_dtype);
     if (!e) return "token_fc: out_dtype must be F32, F16 or BF16";
@@ -62,7 +64,7 @@ inline bool token_out(TokenCall *call, int32_t m, int32_t c, int32_t dtype) {
 }
 
 inline const char *check_token_norm(const enn_b200_token_norm_desc &d, TokenCall *call) {
-    if (d.m < 0 || d.c <= 0) return "token_norm: bad shape";
+    if (d.m < 0 || d.m > kMostRows || d.c <= 0) return "token_norm: bad shape";
     if (d.c > 32768) return "token_norm: c must be at most 32768";
     if (d.norm < ENN_B200_NORM_NONE || d.norm > ENN_B200_NORM_LAYER || d.post_norm < ENN_B200_NORM_NONE || d.post_norm > ENN_B200_NORM_LAYER)
         return "token_norm: unknown norm";
@@ -82,7 +84,7 @@ inline const char *check_token_norm(const enn_b200_token_norm_desc &d, TokenCall
 }
 
 inline const char *check_token_gate(const enn_b200_token_gate_desc &d, TokenCall *call) {
-    if (d.m < 0 || d.c <= 0) return "token_gate: bad shape";
+    if (d.m < 0 || d.m > kMostRows || d.c <= 0) return "token_gate: bad shape";
     if (d.c > 65536) return "token_gate: c must be at most 65536";
     if (d.act < ENN_B200_GATE_SILU || d.act > ENN_B200_GATE_SIGMOID) return "token_gate: unknown activation";
     const int32_t e = float_size(d.in_dtype);
@@ -95,7 +97,7 @@ inline const char *check_token_gate(const enn_b200_token_gate_desc &d, TokenCall
 }
 
 inline const char *check_log_probs(const enn_b200_log_probs_desc &d, TokenCall *call) {
-    if (d.m < 0 || d.vocab <= 0 || d.vocab > (1 << 24)) return "log_probs: bad shape (vocab is 1 .. 2^24)";
+    if (d.m < 0 || d.m > kMostRows || d.vocab <= 0 || d.vocab > (1 << 24)) return "log_probs: bad shape (vocab is 1 .. 2^24)";
     const int32_t e = float_size(d.in_dtype);
     if (!e) return "log_probs: in_dtype must be F32, F16 or BF16";
     if (d.given < 0 || d.given > 1024) return "log_probs: given must be within 0 .. 1024";

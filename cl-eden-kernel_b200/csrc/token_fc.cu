@@ -541,7 +541,7 @@ cudaError_t launch_tc(enn_b200_op *op, int32_t rows, const void *const *ins, voi
     const auto encode = [&](int32_t box) {
         return encode_2d(ctx, &map_q, ins[0], static_cast<uint64_t>(f.k), static_cast<uint64_t>(rows), static_cast<uint64_t>(f.in_pitch), kBK, static_cast<uint32_t>(box));
     };
-    const int pairs = ctx->launch_sms() / 2;
+    const int pairs = t.sms / 2;
 
     // Large products: pairs of CTAs.  The width of the token tiles is the one whose rounds over the device take least, a tile costing its
     // columns and about as much as kTileCost more.
@@ -576,7 +576,7 @@ cudaError_t launch_tc(enn_b200_op *op, int32_t rows, const void *const *ins, voi
     token_tiles(rows, kTcTokens, 16, &c.m_tiles, &c.bn);
     const int64_t tiles = static_cast<int64_t>((f.n + kChannels - 1) / kChannels) * c.m_tiles;
     c.splits = 1;
-    while (c.splits < kMaxSplits && tiles * c.splits * 2 <= 2 * ctx->launch_sms() && kb_total >= 4 * c.splits) c.splits *= 2;
+    while (c.splits < kMaxSplits && tiles * c.splits * 2 <= 2 * t.sms && kb_total >= 4 * c.splits) c.splits *= 2;
     const int stage_bytes = (kChannels + c.bn) * kBK;
     c.stages = std::min({111 * 1024 / stage_bytes, (kb_total + c.splits - 1) / c.splits, kMaxStages});
     const size_t smem = 1024 + static_cast<size_t>(std::max(c.stages * stage_bytes, c.bn * kChannels * 4));
@@ -600,7 +600,22 @@ cudaError_t launch_typed(enn_b200_op *op, int32_t rows, const void *const *ins, 
                       static_cast<const float *>(ins[1]), static_cast<O *>(outs[0]));
 }
 
+__global__ void pad_rows_kernel(const int8_t *src, int32_t width, int64_t pitch, int64_t total, int8_t *dst) {
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total; i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
+        const int64_t r = i / pitch, c = i - r * pitch;
+        dst[i] = c < width ? src[r * width + c] : int8_t{0};
+    }
+}
+
 }  // namespace
+
+// Dense rows into rows `pitch` bytes apart, zeros beyond the width.
+cudaError_t launch_pad_rows(const void *src, int32_t width, int32_t height, int64_t pitch, void *dst, cudaStream_t stream) {
+    const int64_t total = pitch * height;
+    pad_rows_kernel<<<static_cast<unsigned>(std::min<int64_t>(total / 2048 + 1, 4096)), 256, 0, stream>>>(static_cast<const int8_t *>(src), width, pitch, total,
+                                                                                                           static_cast<int8_t *>(dst));
+    return cudaGetLastError();
+}
 
 // The part of the plan that does not depend on a call: the weights' tensor map and the error word.
 cudaError_t token_fc_plan(enn_b200_op *op) {

@@ -52,6 +52,7 @@ struct TokenFcParams {
 struct TokenState {
     TokenCall call;
     int32_t in_dtype = 0, out_dtype = 0;
+    int32_t sms = 0;        // SMs a launch may occupy (option grid_cap when the operator was prepared)
     bool residual = false, packed = false;
     NormParams norm{};
     GateParams gate{};
@@ -65,6 +66,7 @@ cudaError_t token_gate_launch(const enn_b200_op *op, int32_t rows, const void *c
 cudaError_t log_probs_launch(const enn_b200_op *op, int32_t rows, const void *const *ins, void *const *outs);
 cudaError_t token_fc_launch(enn_b200_op *op, int32_t rows, const void *const *ins, void *const *outs);
 cudaError_t token_fc_plan(enn_b200_op *op);
+cudaError_t launch_pad_rows(const void *src, int32_t width, int32_t height, int64_t pitch, void *dst, cudaStream_t stream);
 
 #ifdef __CUDACC__
 namespace {

@@ -582,14 +582,14 @@ cudaError_t norm_typed(const enn_b200_op *op, int32_t rows, const void *const *i
     void *y = outs[o++];
     float *scale = t.out_dtype == ENN_B200_S8 ? static_cast<float *>(outs[o++]) : nullptr;
     const bool lines = p.c % kGroup == 0 && aligned(x, 16) && aligned(residual, 16) && aligned(gate, 16) && aligned(stream, 16) && aligned(y, scale ? 8 : 16);
-    const Shape s = row_shape(p.c, lines, rows <= 2 * op->ctx->sm_count, max_threads(4));
+    const Shape s = row_shape(p.c, lines, rows <= 2 * op->token->sms, max_threads(4));
     // As many blocks as an SM holds, each taking rows in turn, and rings of up to four rows in what shared memory
     // that leaves them; the widest rows of 32-bit types do without.
     const int threads = s.nt * s.per_block;
     const int blocks = std::max(1, max_threads(s.nv) * min_blocks(s.nv) / threads);
     const int ahead_bytes = threads * s.nv * kGroup * static_cast<int>(sizeof(T)) * (1 + (residual != nullptr) + (gate != nullptr));
     const int depth = ahead_bytes > kRingBytes ? 0 : std::min(kMaxDepth, std::max(1, kRingShare / blocks / ahead_bytes));
-    const int64_t want = (static_cast<int64_t>(rows) + s.per_block - 1) / s.per_block, most = static_cast<int64_t>(op->ctx->launch_sms()) * blocks;
+    const int64_t want = (static_cast<int64_t>(rows) + s.per_block - 1) / s.per_block, most = static_cast<int64_t>(t.sms) * blocks;
     const dim3 grid(static_cast<unsigned>(std::min(want, most))), block(static_cast<unsigned>(s.nt), static_cast<unsigned>(s.per_block));
     return with_shape(s.nv, lines, [&](auto nv, auto v) {
         constexpr auto kernel = token_norm_kernel<T, decltype(nv)::value, decltype(v)::value>;
@@ -607,14 +607,16 @@ cudaError_t gate_typed(const enn_b200_op *op, int32_t rows, const void *const *i
     const T *g = static_cast<const T *>(ins[0]), *u = t.packed ? g + p.c : static_cast<const T *>(ins[1]);
     const bool bytes = t.out_dtype == ENN_B200_S8;
     const bool lines = p.c % kGroup == 0 && aligned(g, 16) && aligned(u, 16) && aligned(outs[0], bytes ? 8 : 16);
-    // Segments: of up to 8192 channels; of bytes up to eight of them, more where the rows alone do not occupy the device.
+    // Segments: of up to 8192 channels.  Of bytes one for up to 16384 channels (the exchange in a cluster costs more than it brings:
+    // 8192x12288 99 us in two, 96 us in one; 2048x24576 53 us in four, 63 us in two), then up to eight, and more where the rows alone do not
+    // occupy the device.
     int segs = 1;
     if (!bytes) segs = (p.c + 8191) / 8192;
     else
-        while (segs < 8 && (p.c > 16384 * segs || (static_cast<int64_t>(rows) * segs * 2 <= 2 * op->ctx->sm_count && p.c >= 2048 * segs))) segs *= 2;
+        while (segs < 8 && (p.c > (segs == 1 ? 16384 : 8192 * segs) || (static_cast<int64_t>(rows) * segs * 2 <= 2 * op->token->sms && p.c >= 2048 * segs))) segs *= 2;
     const int seg = segs == 1 ? p.c : ((p.c + segs - 1) / segs + kGroup - 1) / kGroup * kGroup;
     if (!bytes) segs = (p.c + seg - 1) / seg;
-    const Shape s = row_shape(seg, lines, static_cast<int64_t>(rows) * segs <= 2 * op->ctx->sm_count, gate_threads(4));
+    const Shape s = row_shape(seg, lines, static_cast<int64_t>(rows) * segs <= 2 * op->token->sms, gate_threads(4));
     const int per_block = segs > 1 && bytes ? 1 : s.per_block;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(static_cast<unsigned>((static_cast<int64_t>(rows) + per_block - 1) / per_block), static_cast<unsigned>(segs));

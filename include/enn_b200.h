@@ -165,8 +165,8 @@ typedef struct enn_b200_resize_desc {
 
 /* ---- token operators: what runs around an 8-bit product whose activations are quantised row by row at run time, as in
  *      the blocks of a language model served in 8-bit integers.  No counterpart in the reference.  A row is a token; an
- *      operator is prepared once for up to `m` rows and enn_b200_op_execute_rows runs it on 0 .. m of them (1 for a decode
- *      step, more for a prompt).  Rows past the given number are neither read nor written.
+ *      operator is prepared once for up to `m` rows (0 .. 2^30) and enn_b200_op_execute_rows runs it on 0 .. m of them (1 for a
+ *      decode step, more for a prompt).  Rows past the given number are neither read nor written.
  *
  * Quantised rows ("byte rows"): row t is c int8 values q[t][i] in [-127, 127], enn_b200_token_pitch(c) bytes from row to
  * row, and a float scale s[t]; they stand for q * s.  Rows are quantised as s = max_i |y_i| / 127,
@@ -331,7 +331,7 @@ int32_t enn_b200_log_probs_prepare(enn_b200_context *ctx, const enn_b200_log_pro
 /* Bytes from row to row of byte rows of c channels: c rounded up to 16. */
 int64_t enn_b200_token_pitch(int32_t c);
 /* Runs a token operator on the first `rows` (0 .. m) rows of its inputs: enqueues on the context's stream, whatever device
- * is current, and can be captured.  The inputs and outputs the descriptor asks for, in its order, aligned to their element
+ * is current, and can be captured (the operator must then outlive the graph).  The inputs and outputs the descriptor asks for, in its order, aligned to their element
  * type (byte rows: q and out of token_fc are fast at 16-byte addresses; outputs of 16-byte alignment are written fastest). */
 int32_t enn_b200_op_execute_rows(enn_b200_op *op, int32_t rows, const void *const *ins_dev, int32_t n_in, void *const *outs_dev,
                                  int32_t n_out);

@@ -44,6 +44,8 @@ int main() {
     expect(!fc(1, 1, 1, ENN_B200_S8, 0) && !fc(1, 1, 1, 2, 0), "fc result type");
     expect(fc(1, 33, 1, ENN_B200_F32, 33) && !fc(1, 33, 1, ENN_B200_F32, 32) && !fc(1, 33, 1, ENN_B200_F32, -16), "fc pitch");
 
+    expect(fc(1 << 30, 1, 1, ENN_B200_F32, 0) && !fc((1 << 30) + 1, 1, 1, ENN_B200_F32, 0), "most rows");
+
     TokenCall n;
     expect(norm([](auto &) {}, &n) && n.n_in == 3 && n.n_out == 3 && n.in_bytes[2] == 2 * 40 * 2 && n.out_bytes[1] == 4 * 48 && n.in_place, "norm sizes");
     TokenCall n2;
