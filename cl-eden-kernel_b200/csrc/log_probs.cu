@@ -25,11 +25,12 @@ constexpr int kMaxSegments = 8;
 constexpr int kChunk = 4;               // 16-byte pieces a thread works on at a time
 constexpr int kDepth = 2;               // chunks a thread asks for ahead
 constexpr int kCandidates = 1024;
-// Threads of a CTA: kLong, or kShort for many short rows, whose time is that of the reductions and of the search, one step after the
-// other: more rows side by side.  And the CTAs an SM is to hold.
-constexpr int kLong = 256, kShort = 64;
-constexpr int kShortBytes = 16384;       // of a short row
-constexpr int blocks_of(int threads) { return threads == kLong ? 3 : 8; }
+// Threads of a CTA: kLong; kShort for many short rows, whose time is that of the reductions and of the search, one step after the other:
+// more rows side by side (4000x2000 bf16 42 us with kLong, 18 us so); kLongest where the stream is most of it (2048x65536 f32, 20
+// alternatives, 118 us with kLong, 108 us so; 4000x16000 bf16 64 and 93 us).  And the CTAs an SM is to hold.
+constexpr int kLongest = 512, kLong = 256, kShort = 64;
+constexpr int kShortBytes = 16 << 10, kLongestBytes = 192 << 10;       // rows of up to, segments of at least
+constexpr int blocks_of(int threads) { return threads == kLongest ? 2 : (threads == kLong ? 3 : 8); }
 constexpr int kLookers = 8;             // threads that look at one thread's logits again
 constexpr float kNothing = -1e4f;       // 2^-10000 is 0; keeps the products d 2^d away from infinity times 0
 constexpr float kSlack = 20.f;
@@ -557,6 +558,7 @@ cudaError_t launch_typed(const enn_b200_op *op, int32_t rows, const void *const 
         return cudaLaunchKernelEx(&cfg, kernel, p, rows, seg_size, static_cast<const T *>(ins[0]), ids, given, entropy, top_ids, top);
     };
     if (rows > blocks_of(kLong) * sms && p.vocab * static_cast<int64_t>(sizeof(T)) <= kShortBytes) return run(std::integral_constant<int, kShort>{});
+    if (seg_size * static_cast<int64_t>(sizeof(T)) >= kLongestBytes) return run(std::integral_constant<int, kLongest>{});
     return run(std::integral_constant<int, kLong>{});
 }
 
