@@ -425,7 +425,7 @@ __global__ void __launch_bounds__(kThreads, blocks_of(kThreads)) log_probs_kerne
             // after it (a vocabulary is ruled out all over).
             const uint64_t minus_m = pair(-a.m, -a.m), k2 = pair(k, k);
             const auto sum = [&](auto limit) {
-                uint64_t s2 = pair(a.s, 0.f), u2 = pair(a.u, 0.f);
+                uint64_t s2 = 0, u2 = 0;      // of the chunk: no long chain of additions
 #pragma unroll
                 for (int c = 0; c < kChunk; ++c) {
                     float x[E];
@@ -452,8 +452,8 @@ __global__ void __launch_bounds__(kThreads, blocks_of(kThreads)) log_probs_kerne
                     const float2 d = unpair(d2);
                     return pair(max_nan(d.x, kNothing), max_nan(d.y, kNothing));
                 });
-            a.s = su.x;
-            a.u = su.y;
+            a.s += su.x;
+            a.u += su.y;
         }
 
         // The statistics of the segment, the same in every thread.

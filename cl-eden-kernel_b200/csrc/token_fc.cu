@@ -57,8 +57,8 @@ __global__ void __launch_bounds__(kDirectThreads) token_fc_direct_kernel(TokenFc
 }
 
 // ---- tensor-core kernel: one tile of 128 channels x bn tokens per CTA, the reduction split over a cluster.
-// The channels are the rows of the matrix instruction (always 128), the tokens its columns (16 .. 256), so that a call of few tokens
-// wastes nothing but its 16th columns and is bound by reading the weights.  A cluster of `splits` CTAs shares a tile: each multiplies
+// The channels are the rows of the matrix instruction (always 128), the tokens its columns (16 .. 128), so that a call of few tokens
+// multiplies at most 15 columns for nothing and is bound by reading the weights.  A cluster of `splits` CTAs shares a tile: each multiplies
 // its part of k, and the exact 32-bit partial sums meet through distributed shared memory; no atomics, no workspace, the same result for
 // every split.
 //   warp 0, lane 0   copies the weight tiles.  Weights are constants of the operator, so their copies start before the kernel ahead in
@@ -570,6 +570,8 @@ cudaError_t launch_tc(enn_b200_op *op, int32_t rows, const void *const *ins, voi
                                f.map_w, map_q, c2, out);
     }
 
+    // (CTAs of clusters wait for one another, so that none may wait for tensor memory that a CTA of another cluster holds.  A split leaves two
+    // stages at least, 54 KB with more than 64 tokens: an SM holds four such CTAs at most, which have 128 of its 512 columns each.)
     // Two CTAs share an SM: while one waits for its first tiles or stores its results, the other keeps the SM busy.
     TcCall c{};
     c.rows = rows; c.n = f.n; c.kb_total = kb_total;

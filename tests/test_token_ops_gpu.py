@@ -650,6 +650,21 @@ def test_log_probs_clusters_of_large_values(enn, ctx):
         check_log_probs(logits, ids, 32, run_log_probs(enn, ctx, logits, ids, 32))
 
 
+@pytest.mark.parametrize("m,v,io,top", [(600, 3000, "bf16", 20), (500, 1001, "f16", 5), (450, 8000, "bf16", 32), (700, 37, "f32", 32), (3000, 500, "f32", 1),
+                                        (230, 49500, "f32", 20), (250, 100001, "bf16", 7), (500, 20000, "f16", 20)])
+def test_log_probs_many_rows(enn, ctx, m, v, io, top):
+    """Many rows of every length, among them rows of equal logits, rows with little left and rows with none."""
+    logits = (rand(m + v, m, v) * 3).to(TYPES[io])
+    logits[1] = 0
+    logits[2, 3:] = -math.inf
+    logits[3] = torch.finfo(TYPES[io]).min
+    logits[3, 5] = 1
+    logits[m - 1] = (rand(3, v) * 2).round().to(TYPES[io])
+    ids = torch.randint(0, v, (m, 1), device="cuda", dtype=torch.int32)
+    got = run_log_probs(enn, ctx, logits, ids, top)
+    check_log_probs(logits, ids, top, got)
+
+
 def test_log_probs_masked_vocabulary(enn, ctx):
     v = 3001
     logits = rand(8, 5, v) * 4
@@ -853,6 +868,38 @@ def test_a_block_captured_and_replayed(enn):
         ctx.sync()
         assert all(torch.equal(first[k], bufs[k]) for k in bufs)
     del graph
+    for op in ops.values():
+        op.release()
+    ctx.close()
+
+
+def test_two_graphs_of_the_same_operators_at_once(enn):
+    """Graphs of the same handles on other tensors, replayed on two streams at the same time: the operators share no memory."""
+    ctx = enn.Context(0)
+    m, c, f, v = 33, 512, 1400, 6000
+    ops, weights = block(enn, ctx, m, c, f, v)
+    stream = torch.cuda.ExternalStream(ctx.stream)
+    graphs, sets = [], []
+    for i in range(2):
+        bufs = block_buffers(enn, m, c, f, v)
+        bufs["x"] = (rand(40 + i, m, c) * 2).bfloat16()
+        bufs["ids"] = torch.randint(0, v, (m, 1), device="cuda", dtype=torch.int32)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            run_block(ops, bufs, m)
+        graphs.append(graph)
+        sets.append(bufs)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for graph, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                graph.replay()
+    torch.cuda.synchronize()
+    for bufs in sets:
+        check_block(bufs, weights, m, c, f)
+    del graph, graphs
     for op in ops.values():
         op.release()
     ctx.close()
