@@ -541,16 +541,17 @@ bool aligned(const void *p, size_t to) { return reinterpret_cast<uintptr_t>(p) %
 
 // Threads of a row and groups per thread for `n` channels.  `spread`: as many threads as there are groups (few rows: latency), else
 // four groups each (many rows: what a row costs whatever its length, reductions and addresses, is shared by more channels), up to
-// `most_by_four` threads.
+// `most_by_four` threads; `two`: two, where four are too many (the code for shifted groups then overflows the instruction cache: 2048x4097
+// 30 us, 27 us with two; the rows of 32-bit types in flight leave L1 nothing: 2048x8192 82 us, 72 us with two).
 struct Shape {
     int nt, nv, per_block;
 };
-Shape row_shape(int n, bool lines, bool spread, int most_by_four) {
+Shape row_shape(int n, bool lines, bool spread, bool two, int most_by_four) {
     const int groups = (n + (lines ? 0 : kGroup - 1) + kGroup - 1) / kGroup;      // one more where they are shifted
     auto threads = [&](int nv) { return ((groups + nv - 1) / nv + 31) / 32 * 32; };
     Shape s;
     if (groups <= 32 || (spread && groups <= 1024)) s.nv = 1;
-    else if (groups <= 64 || (!lines && groups <= 1024)) s.nv = 2;      // (the code for shifted groups is long: four of them overflow the instruction cache)
+    else if (groups <= 64 || (two && groups <= 1024)) s.nv = 2;
     else s.nv = groups <= 4 * most_by_four ? 4 : 8;
     s.nt = threads(s.nv);
     s.per_block = s.nt == 32 ? 8 : 1;
@@ -582,7 +583,7 @@ cudaError_t norm_typed(const enn_b200_op *op, int32_t rows, const void *const *i
     void *y = outs[o++];
     float *scale = t.out_dtype == ENN_B200_S8 ? static_cast<float *>(outs[o++]) : nullptr;
     const bool lines = p.c % kGroup == 0 && aligned(x, 16) && aligned(residual, 16) && aligned(gate, 16) && aligned(stream, 16) && aligned(y, scale ? 8 : 16);
-    const Shape s = row_shape(p.c, lines, rows <= 2 * op->token->sms, max_threads(4));
+    const Shape s = row_shape(p.c, lines, rows <= 2 * op->token->sms, !lines || sizeof(T) == 4, max_threads(4));
     // As many blocks as an SM holds, each taking rows in turn, and rings of up to four rows in what shared memory
     // that leaves them; the widest rows of 32-bit types do without.
     const int threads = s.nt * s.per_block;
@@ -616,7 +617,7 @@ cudaError_t gate_typed(const enn_b200_op *op, int32_t rows, const void *const *i
         while (segs < 8 && (p.c > (segs == 1 ? 16384 : 8192 * segs) || (static_cast<int64_t>(rows) * segs * 2 <= 2 * op->token->sms && p.c >= 2048 * segs))) segs *= 2;
     const int seg = segs == 1 ? p.c : ((p.c + segs - 1) / segs + kGroup - 1) / kGroup * kGroup;
     if (!bytes) segs = (p.c + seg - 1) / seg;
-    const Shape s = row_shape(seg, lines, static_cast<int64_t>(rows) * segs <= 2 * op->token->sms, gate_threads(4));
+    const Shape s = row_shape(seg, lines, static_cast<int64_t>(rows) * segs <= 2 * op->token->sms, !lines, gate_threads(4));
     const int per_block = segs > 1 && bytes ? 1 : s.per_block;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(static_cast<unsigned>((static_cast<int64_t>(rows) + per_block - 1) / per_block), static_cast<unsigned>(segs));
