@@ -8,6 +8,8 @@
 // bounds the n-th largest logit from below, so that what is above it lies with those threads, and their logits alone are looked at again.
 // A row is split over a cluster of up to eight CTAs where the rows alone do not occupy the device; the parts meet in the first CTA's
 // shared memory, without atomics or workspace.  All orders are total (value, then index), so that results do not depend on timing.
+// 2048x65536 f32 with one alternative 101 us (5.3 TB/s), 93 us without; 1x131072 8.1 us, half of it the search.  16-bit rows are bound by
+// instructions (8 a logit, one of them 2^x, of which an SM does 16 a cycle): 2048x65536 bf16 48 us without alternatives (5.6 TB/s).
 #include <math_constants.h>
 
 #include <algorithm>
