@@ -2,8 +2,8 @@
 //
 // Both are bound by memory: a row is read once, stays in registers as floats while its statistics are reduced, and is written once.
 // A row belongs to a warp (up to 1024 channels), a CTA, or for quantised gates a cluster; a thread holds up to eight groups of eight
-// neighbouring channels, 16 bytes of a 16-bit type.  Constant vectors come from L1, which they share with nothing: the rows are loaded
-// and stored past it.  Measured in queued passes: gates 8192x12288 bf16 92 us (6.6 TB/s), norms on both sides of a block with the stream
+// neighbouring channels, 16 bytes of a 16-bit type.  Constant vectors come from L1, which they share with nothing: rows are loaded and
+// stored past it (those of gates between lines, which have no such vectors, through it).  Measured in queued passes: gates 8192x12288 bf16 92 us (6.6 TB/s), norms on both sides of a block with the stream
 // 8192x5120 bf16 67 us (5.0 TB/s; half of the issue slots busy, 28 instructions a channel, the rest the latency of three reductions a row).
 #include <algorithm>
 #include <type_traits>
@@ -20,6 +20,19 @@ constexpr int kGroup = 8;           // channels a thread handles together
 __device__ __forceinline__ uint4 ld_stream(const void *p) {
     uint4 v;
     asm volatile("ld.global.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
+    return v;
+}
+// Zeros where `on` does not hold, without a branch that the loads after it would have to wait for.  It is for lines that two groups
+// share, so L1 keeps them (4096x4099, of gates and values: 26.2 us, 27.4 us where it does not).
+__device__ __forceinline__ uint4 ld_if(const void *p, bool on) {
+    uint4 v;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %5, 0;\n\t"
+        "mov.u32 %0, 0;\n\tmov.u32 %1, 0;\n\tmov.u32 %2, 0;\n\tmov.u32 %3, 0;\n\t"
+        "@p ld.global.v4.b32 {%0, %1, %2, %3}, [%4];\n\t}"
+        : "=&r"(v.x), "=&r"(v.y), "=&r"(v.z), "=&r"(v.w)
+        : "l"(p), "r"(static_cast<uint32_t>(on))
+        : "memory");
     return v;
 }
 // Eight channels as they lie in memory.
@@ -70,6 +83,8 @@ __device__ __forceinline__ uint32_t pack4_s8(const float *f, float inv) {
     return d;
 }
 
+// Lines that a group which begins inside one touches.
+template <typename T> constexpr int kLinesOf = static_cast<int>(sizeof(T)) / 2 + 1;
 // The part of a row that a group of `nt` threads holds: channels [0, n) of a segment in groups of eight neighbours, NV per thread.
 // LINES: every group is whole and lies on 16-byte lines (n, every address and every pitch allow it).  Else the groups are shifted
 // by `skip` channels, so that they lie on the lines of the tensor they were laid out for; the first and the last may reach over the
@@ -106,32 +121,63 @@ struct Row {
         high = n + static_cast<int>(min(static_cast<int64_t>(2 * kGroup), after));
     }
     // A group that lies across lines: put together from those, or channel by channel (0 outside) where they are not the tensor's.
-    template <typename T> __device__ __forceinline__ Raw<T> across(const T *p, int v) const {
-        constexpr int W = static_cast<int>(sizeof(T)) * 2, L = W / 4 + 1;      // words of a group, lines it touches
-        const int off = static_cast<int>(reinterpret_cast<uintptr_t>(p + at(v)) & 15), before = off / static_cast<int>(sizeof(T));
+    template <typename T> __device__ __forceinline__ int offset(const T *p, int v) const { return static_cast<int>(reinterpret_cast<uintptr_t>(p + at(v)) & 15); }
+    template <typename T> __device__ __forceinline__ bool lines_readable(int v, int off) const {
+        const int first = at(v) - off / static_cast<int>(sizeof(T));
+        return first >= low && first + kLinesOf<T> * 16 / static_cast<int>(sizeof(T)) <= high;
+    }
+    template <typename T> __device__ __forceinline__ Raw<T> join(const uint4 (&q)[kLinesOf<T>], int off) const {
+        constexpr int L = kLinesOf<T>, W = static_cast<int>(sizeof(T)) * 2;      // W: words of a group
+        uint32_t w[4 * L], out[W];
+#pragma unroll
+        for (int i = 0; i < L; ++i) { w[4 * i] = q[i].x; w[4 * i + 1] = q[i].y; w[4 * i + 2] = q[i].z; w[4 * i + 3] = q[i].w; }
+#pragma unroll
+        for (int i = 0; i < 4 * L - 2; ++i) w[i] = off & 8 ? w[i + 2] : w[i];
+#pragma unroll
+        for (int i = 0; i < 4 * L - 3; ++i) w[i] = off & 4 ? w[i + 1] : w[i];
+#pragma unroll
+        for (int i = 0; i < W; ++i) out[i] = sizeof(T) == 2 ? __funnelshift_r(w[i], w[i + 1], off & 2 ? 16 : 0) : w[i];
         Raw<T> r;
-        if (at(v) - before >= low && at(v) - before + L * 16 / static_cast<int>(sizeof(T)) <= high) {
-            uint32_t w[4 * L];
-#pragma unroll
-            for (int i = 0; i < L; ++i) {
-                const uint4 q = ld_stream(reinterpret_cast<const uint4 *>(p + at(v) - before) + i);
-                w[4 * i] = q.x; w[4 * i + 1] = q.y; w[4 * i + 2] = q.z; w[4 * i + 3] = q.w;
-            }
-#pragma unroll
-            for (int i = 0; i < 4 * L - 2; ++i) w[i] = off & 8 ? w[i + 2] : w[i];
-#pragma unroll
-            for (int i = 0; i < 4 * L - 3; ++i) w[i] = off & 4 ? w[i + 1] : w[i];
-            uint32_t out[W];
-#pragma unroll
-            for (int i = 0; i < W; ++i) out[i] = sizeof(T) == 2 ? __funnelshift_r(w[i], w[i + 1], off & 2 ? 16 : 0) : w[i];
-            __builtin_memcpy(&r, out, sizeof(out));
-        } else {
-            T e[kGroup];
-#pragma unroll
-            for (int j = 0; j < kGroup; ++j) e[j] = inside(v, j) ? p[at(v, j)] : from_float<T>(0.f);
-            __builtin_memcpy(&r, e, sizeof(e));
-        }
+        __builtin_memcpy(&r, out, sizeof(out));
         return r;
+    }
+    template <typename T> __device__ __forceinline__ Raw<T> gather(const T *p, int v) const {
+        T e[kGroup];
+#pragma unroll
+        for (int j = 0; j < kGroup; ++j) e[j] = inside(v, j) ? p[at(v, j)] : from_float<T>(0.f);
+        Raw<T> r;
+        __builtin_memcpy(&r, e, sizeof(e));
+        return r;
+    }
+    template <typename T> __device__ __forceinline__ Raw<T> across(const T *p, int v) const {
+        const int off = offset(p, v);
+        if (!lines_readable<T>(v, off)) return gather(p, v);
+        uint4 q[kLinesOf<T>];
+#pragma unroll
+        for (int i = 0; i < kLinesOf<T>; ++i) q[i] = ld_stream(reinterpret_cast<const uint4 *>(reinterpret_cast<const uint8_t *>(p + at(v)) - off) + i);
+        return join<T>(q, off);
+    }
+    // Two tensors whose groups lie across lines, all loads ahead of their first use (4096x4099, of gates and values: bf16 34.0 us group
+    // by group, 26.2 us so; f32 42.9 and 39.9 us).  Four groups of a 32-bit type and more would not fit the registers.
+    template <typename T> __device__ __forceinline__ void load_two(const T *a, const T *b, Raw<T> (&ra)[NV], Raw<T> (&rb)[NV]) const {
+        const int oa = offset(a, 0), ob = offset(b, 0);     // a group's length is a multiple of a line's
+        uint4 qa[NV][kLinesOf<T>], qb[NV][kLinesOf<T>];
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            const bool on_a = any(v) && lines_readable<T>(v, oa), on_b = any(v) && lines_readable<T>(v, ob);
+#pragma unroll
+            for (int i = 0; i < kLinesOf<T>; ++i) {
+                qa[v][i] = ld_if(reinterpret_cast<const uint4 *>(reinterpret_cast<const uint8_t *>(a + at(v)) - oa) + i, on_a);
+                qb[v][i] = ld_if(reinterpret_cast<const uint4 *>(reinterpret_cast<const uint8_t *>(b + at(v)) - ob) + i, on_b);
+            }
+        }
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            ra[v] = join<T>(qa[v], oa);
+            rb[v] = join<T>(qb[v], ob);
+            if (any(v) && !lines_readable<T>(v, oa)) ra[v] = gather(a, v);
+            if (any(v) && !lines_readable<T>(v, ob)) rb[v] = gather(b, v);
+        }
     }
     // Past the row's ends what lies there; nothing where the thread has no channels.
     template <typename T> __device__ __forceinline__ void load(const T *p, Raw<T> (&held)[NV]) const {
@@ -469,8 +515,12 @@ __device__ __forceinline__ float gate_act(float g) {
 template <typename T, int NV, bool LINES>
 __device__ __forceinline__ void gate_row(const Row<NV, LINES> &row, const T *gates, const T *values, int act, float (&f)[NV][8]) {
     Raw<T> rg[NV], ru[NV];
-    row.load(gates, rg);
-    row.load(values, ru);
+    if (!LINES && (sizeof(T) == 2 || (NV <= 2 && !(row.lined(gates) && row.lined(values))))) {
+        row.load_two(gates, values, rg, ru);
+    } else {
+        row.load(gates, rg);
+        row.load(values, ru);
+    }
     auto apply = [&](auto which) {
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
