@@ -346,10 +346,10 @@ __device__ __forceinline__ void norm_row(const Row<NV, LINES> &row, float (&f)[N
     if (largest) *largest = reduce.largest(largest_of(f));
 }
 
-// Threads a block has at most: what the registers of NV groups a thread allow.
-constexpr int max_threads(int nv) { return nv == 1 ? 1024 : (nv == 2 ? 512 : (nv == 4 ? 256 : 544)); }
-// Blocks of that size an SM is to hold: 64 registers a thread, 80 with four groups, 120 with eight.
-constexpr int min_blocks(int nv) { return nv == 4 ? 3 : (nv == 2 ? 2 : 1); }
+// Threads that the registers of NV groups a thread leave an SM: 64 registers each, 80 with four groups, 96 with eight.  One block may
+// have them all, so that eight groups, which spill, remain for rows above 24576 channels (2048x10240 bf16 with a stream: 46 us in eight
+// groups, 29 us in four; 33x10241: 12.9 us, 6.5 us in two).
+constexpr int norm_threads(int nv) { return nv <= 2 ? 1024 : (nv == 4 ? 768 : 544); }
 
 // A thread's own ring in shared memory: `depth` rows ahead, each with `streams` tensors, filled by asynchronous copies.  A thread reads
 // what it copied itself, so that no barrier is needed; the bytes in flight do not depend on how long a row's reductions take.
@@ -399,7 +399,7 @@ constexpr int kRingBytes = 216 * 1024;      // at most
 constexpr int kRingShare = 112 * 1024;      // of an SM: what they take, L1 lacks for the constant vectors (8192x5120: 65 us with all of it, 61 us so)
 
 template <typename T, int NV, bool LINES>
-__global__ void __launch_bounds__(max_threads(NV), min_blocks(NV)) token_norm_kernel(NormParams p, int32_t rows, int32_t out_dtype, int32_t depth, const T *x,
+__global__ void __launch_bounds__(norm_threads(NV)) token_norm_kernel(NormParams p, int32_t rows, int32_t out_dtype, int32_t depth, const T *x,
                                                                                        const T *residual, const T *gate, T *stream, void *out, float *scale) {
     extern __shared__ __align__(16) uint8_t ring[];
     __shared__ float2 scratch[2][32];
@@ -542,7 +542,7 @@ __device__ __forceinline__ void gate_row(const Row<NV, LINES> &row, const T *gat
     }
 }
 
-constexpr int gate_threads(int nv) { return nv == 4 ? 512 : max_threads(nv); }
+constexpr int gate_threads(int nv) { return nv == 1 ? 1024 : 512; }
 
 // Grid: rows x segments of `seg` channels.  Floats leave at once.  Bytes need the row's largest magnitude first: the
 // segments of a row are then the CTAs of a cluster, which tell each other theirs.
@@ -592,31 +592,32 @@ bool aligned(const void *p, size_t to) { return reinterpret_cast<uintptr_t>(p) %
 
 // Threads of a row and groups per thread for `n` channels.  `spread`: as many threads as there are groups (few rows: latency), else
 // four groups each (many rows: what a row costs whatever its length, reductions and addresses, is shared by more channels), up to
-// `most_by_four` threads; `two`: two, where four are too many (the code for shifted groups then overflows the instruction cache: 2048x4097
-// 30 us, 27 us with two; the rows of 32-bit types in flight leave L1 nothing: 2048x8192 82 us, 72 us with two).
+// `most(groups)` threads; `two`: two, where four are too many (the code for shifted groups then overflows the instruction cache: norms of
+// 2048x4097 30 us, 27 us with two, gates of 4096x4099 35 us, 26 us; the rows of 32-bit types in flight leave L1 nothing: norms of 2048x8192
+// 82 us, 72 us with two).
 struct Shape {
     int nt, nv, per_block;
 };
-Shape row_shape(int n, bool lines, bool spread, bool two, int most_by_four) {
+Shape row_shape(int n, bool lines, bool spread, bool two, int (*most)(int)) {
     const int groups = (n + (lines ? 0 : kGroup - 1) + kGroup - 1) / kGroup;      // one more where they are shifted
     auto threads = [&](int nv) { return ((groups + nv - 1) / nv + 31) / 32 * 32; };
     Shape s;
-    if (groups <= 32 || (spread && groups <= 1024)) s.nv = 1;
-    else if (groups <= 64 || (two && groups <= 1024)) s.nv = 2;
-    else s.nv = groups <= 4 * most_by_four ? 4 : 8;
+    if (groups <= 32 || (spread && groups <= most(1))) s.nv = 1;
+    else if (groups <= 64 || ((two || spread) && groups <= 2 * most(2))) s.nv = 2;
+    else s.nv = groups <= 4 * most(4) ? 4 : 8;
     s.nt = threads(s.nv);
     s.per_block = s.nt == 32 ? 8 : 1;
     return s;
 }
 
-template <typename F>
+template <int MOST, typename F>
 cudaError_t with_shape(int nv, bool lines, F f) {
     auto groups = [&](auto v) {
         switch (nv) {
             case 1: return f(std::integral_constant<int, 1>{}, v);
             case 2: return f(std::integral_constant<int, 2>{}, v);
             case 4: return f(std::integral_constant<int, 4>{}, v);
-            default: return f(std::integral_constant<int, 8>{}, v);
+            default: return f(std::integral_constant<int, MOST>{}, v);
         }
     };
     return lines ? groups(std::true_type{}) : groups(std::false_type{});
@@ -634,16 +635,16 @@ cudaError_t norm_typed(const enn_b200_op *op, int32_t rows, const void *const *i
     void *y = outs[o++];
     float *scale = t.out_dtype == ENN_B200_S8 ? static_cast<float *>(outs[o++]) : nullptr;
     const bool lines = p.c % kGroup == 0 && aligned(x, 16) && aligned(residual, 16) && aligned(gate, 16) && aligned(stream, 16) && aligned(y, scale ? 8 : 16);
-    const Shape s = row_shape(p.c, lines, rows <= 2 * op->token->sms, !lines || sizeof(T) == 4, max_threads(4));
+    const Shape s = row_shape(p.c, lines, rows <= 2 * op->token->sms, !lines || sizeof(T) == 4, norm_threads);
     // As many blocks as an SM holds, each taking rows in turn, and rings of up to four rows in what shared memory
     // that leaves them; the widest rows of 32-bit types do without.
     const int threads = s.nt * s.per_block;
-    const int blocks = std::max(1, max_threads(s.nv) * min_blocks(s.nv) / threads);
+    const int blocks = norm_threads(s.nv) / threads;
     const int ahead_bytes = threads * s.nv * kGroup * static_cast<int>(sizeof(T)) * (1 + (residual != nullptr) + (gate != nullptr));
     const int depth = ahead_bytes > kRingBytes ? 0 : std::min(kMaxDepth, std::max(1, kRingShare / blocks / ahead_bytes));
     const int64_t want = (static_cast<int64_t>(rows) + s.per_block - 1) / s.per_block, most = static_cast<int64_t>(t.sms) * blocks;
     const dim3 grid(static_cast<unsigned>(std::min(want, most))), block(static_cast<unsigned>(s.nt), static_cast<unsigned>(s.per_block));
-    return with_shape(s.nv, lines, [&](auto nv, auto v) {
+    return with_shape<8>(s.nv, lines, [&](auto nv, auto v) {
         constexpr auto kernel = token_norm_kernel<T, decltype(nv)::value, decltype(v)::value>;
         static PerDeviceInit once;
         const cudaError_t e = once.run(op->ctx->device, [&] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBytes); });
@@ -665,10 +666,10 @@ cudaError_t gate_typed(const enn_b200_op *op, int32_t rows, const void *const *i
     int segs = 1;
     if (!bytes) segs = (p.c + 8191) / 8192;
     else
-        while (segs < 8 && (p.c > (segs == 1 ? 16384 : 8192 * segs) || (static_cast<int64_t>(rows) * segs * 2 <= 2 * op->token->sms && p.c >= 2048 * segs))) segs *= 2;
+        while (segs < 8 && (p.c > (segs == 1 ? 16384 - (lines ? 0 : kGroup) : 8192 * segs) || (static_cast<int64_t>(rows) * segs * 2 <= 2 * op->token->sms && p.c >= 2048 * segs))) segs *= 2;
     const int seg = segs == 1 ? p.c : ((p.c + segs - 1) / segs + kGroup - 1) / kGroup * kGroup;
     if (!bytes) segs = (p.c + seg - 1) / seg;
-    const Shape s = row_shape(seg, lines, static_cast<int64_t>(rows) * segs <= 2 * op->token->sms, !lines, gate_threads(4));
+    const Shape s = row_shape(seg, lines, static_cast<int64_t>(rows) * segs <= 2 * op->token->sms, !lines, gate_threads);      // at most four groups: segments end before
     const int per_block = segs > 1 && bytes ? 1 : s.per_block;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(static_cast<unsigned>((static_cast<int64_t>(rows) + per_block - 1) / per_block), static_cast<unsigned>(segs));
@@ -682,7 +683,7 @@ cudaError_t gate_typed(const enn_b200_op *op, int32_t rows, const void *const *i
     attr[1].val.clusterDim.y = static_cast<unsigned>(segs);
     cfg.attrs = attr;
     cfg.numAttrs = bytes && segs > 1 ? 2 : 1;
-    return with_shape(s.nv, lines, [&](auto nv, auto v) {
+    return with_shape<4>(s.nv, lines, [&](auto nv, auto v) {
         return cudaLaunchKernelEx(&cfg, token_gate_kernel<T, decltype(nv)::value, decltype(v)::value>, p, rows, seg, t.out_dtype, g, u, outs[0],
                                   bytes ? static_cast<float *>(outs[1]) : nullptr);
     });

@@ -346,6 +346,13 @@ def test_token_norm_widest_rows(enn, ctx, c, out):
     run_norm(enn, ctx, norm_case(3, c, "f32", out, "layer", "none", False))
 
 
+@pytest.mark.parametrize("m", [2, 300])
+@pytest.mark.parametrize("c", [8185, 8192, 8193, 16376, 16377, 16384, 16385, 24569, 24576, 24577])
+def test_token_norm_widths_around_a_block_s(enn, ctx, m, c):
+    run_norm(enn, ctx, norm_case(m, c, "bf16", "s8", "rms", "none", True))
+    run_norm(enn, ctx, norm_case(m, c, "f32", "f32", "layer", "rms", True, 3))
+
+
 @pytest.mark.parametrize("rows", [0, 1, 16, 37])
 def test_token_norm_fewer_rows_than_prepared(enn, ctx, rows):
     for out in ("bf16", "s8"):
@@ -505,6 +512,14 @@ def test_token_gate_activations(enn, ctx, act, out, packed):
 @pytest.mark.parametrize("out", ["bf16", "s8"])
 def test_token_gate_widest_rows(enn, ctx, c, out):
     run_gate(enn, ctx, 2, c, "bf16", out, "silu", True)
+
+
+@pytest.mark.parametrize("m", [2, 300])
+@pytest.mark.parametrize("out", ["bf16", "s8"])
+@pytest.mark.parametrize("c", [8185, 8193, 16376, 16377, 16383, 16384, 16385])
+def test_token_gate_widths_around_a_segment_s(enn, ctx, m, c, out):
+    run_gate(enn, ctx, m, c, "bf16", out, "silu", True)
+    run_gate(enn, ctx, m, c, "f32", out, "relu", False)
 
 
 @pytest.mark.parametrize("out", ["bf16", "s8"])
