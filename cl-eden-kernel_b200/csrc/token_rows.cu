@@ -398,8 +398,10 @@ constexpr int kMaxDepth = 4;
 constexpr int kRingBytes = 216 * 1024;      // at most
 constexpr int kRingShare = 112 * 1024;      // of an SM: what they take, L1 lacks for the constant vectors (8192x5120: 65 us with all of it, 61 us so)
 
-template <typename T, int NV, bool LINES>
-__global__ void __launch_bounds__(norm_threads(NV)) token_norm_kernel(NormParams p, int32_t rows, int32_t out_dtype, int32_t depth, const T *x,
+// BYTES: the result is quantised.  A kernel of its own, since one for both overflows the instruction cache (2048x4097 bf16: 27.1 us, 25.1 us
+// so; 8192x1001: 20.7 and 18.4 us).
+template <typename T, int NV, bool LINES, bool BYTES>
+__global__ void __launch_bounds__(norm_threads(NV), 1) token_norm_kernel(NormParams p, int32_t rows, int32_t out_dtype, int32_t depth, const T *x,
                                                                                        const T *residual, const T *gate, T *stream, void *out, float *scale) {
     extern __shared__ __align__(16) uint8_t ring[];
     __shared__ float2 scratch[2][32];
@@ -470,7 +472,7 @@ __global__ void __launch_bounds__(norm_threads(NV)) token_norm_kernel(NormParams
         fetch(ahead.slot, t + depth * step);        // this row's memory has been read
         if (++ahead.slot >= depth) ahead.slot = 0;
         if (residual) row.store(stream + t * p.c, f);
-        if (out_dtype != ENN_B200_S8) {
+        if constexpr (!BYTES) {
             norm_row(row, f, p.c, p.norm, p.eps, p.weight, p.bias, p.stride, reduce, nullptr);
             row.store_as(out_dtype, out, t * p.c, f);
         } else {
@@ -645,11 +647,15 @@ cudaError_t norm_typed(const enn_b200_op *op, int32_t rows, const void *const *i
     const int64_t want = (static_cast<int64_t>(rows) + s.per_block - 1) / s.per_block, most = static_cast<int64_t>(t.sms) * blocks;
     const dim3 grid(static_cast<unsigned>(std::min(want, most))), block(static_cast<unsigned>(s.nt), static_cast<unsigned>(s.per_block));
     return with_shape<8>(s.nv, lines, [&](auto nv, auto v) {
-        constexpr auto kernel = token_norm_kernel<T, decltype(nv)::value, decltype(v)::value>;
-        static PerDeviceInit once;
-        const cudaError_t e = once.run(op->ctx->device, [&] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBytes); });
-        if (e != cudaSuccess) return e;
-        return launch_pdl(kernel, grid, block, static_cast<size_t>(depth) * ahead_bytes, op->ctx->stream, p, rows, t.out_dtype, depth, x, residual, gate, stream, y, scale);
+        auto launch = [&](auto kernel, PerDeviceInit &once) {
+            const cudaError_t e = once.run(op->ctx->device, [&] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBytes); });
+            if (e != cudaSuccess) return e;
+            return launch_pdl(kernel, grid, block, static_cast<size_t>(depth) * ahead_bytes, op->ctx->stream, p, rows, t.out_dtype, depth, x, residual, gate, stream, y, scale);
+        };
+        static PerDeviceInit bytes, floats;
+        constexpr int NV = decltype(nv)::value;
+        constexpr bool LINES = decltype(v)::value;
+        return scale ? launch(token_norm_kernel<T, NV, LINES, true>, bytes) : launch(token_norm_kernel<T, NV, LINES, false>, floats);
     });
 }
 
