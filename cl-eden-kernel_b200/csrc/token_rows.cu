@@ -3,8 +3,9 @@
 // Both are bound by memory: a row is read once, stays in registers as floats while its statistics are reduced, and is written once.
 // A row belongs to a warp (up to 1024 channels), a CTA, or for quantised gates a cluster; a thread holds up to eight groups of eight
 // neighbouring channels, 16 bytes of a 16-bit type.  Constant vectors come from L1, which they share with nothing: rows are loaded and
-// stored past it (those of gates between lines, which have no such vectors, through it).  Measured in queued passes: gates 8192x12288 bf16 92 us (6.6 TB/s), norms on both sides of a block with the stream
-// 8192x5120 bf16 67 us (5.0 TB/s; half of the issue slots busy, 28 instructions a channel, the rest the latency of three reductions a row).
+// stored past it (those of gates between lines, which have no such vectors, through it).  Measured in queued passes: gates 8192x12288
+// bf16 92 us (6.6 TB/s), norms on both sides of a block with the stream 8192x5120 bf16 66 us (5.1 TB/s; half of the issue slots busy, 28
+// instructions a channel, the rest the latency of three reductions a row).
 #include <algorithm>
 #include <type_traits>
 
