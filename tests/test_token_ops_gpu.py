@@ -530,6 +530,29 @@ def test_token_gate_odd_widths_many_rows(enn, ctx, m, c, packed, out):
     run_gate(enn, ctx, min(m, 100), c, "f32", out, "gelu_tanh", packed)
 
 
+@pytest.mark.parametrize("g_off,u_off,y_off", [(1, 0, 0), (0, 3, 0), (0, 0, 1), (5, 5, 5), (2, 6, 3), (4, 0, 4)])
+def test_token_gate_tensors_on_different_lines(enn, ctx, g_off, u_off, y_off):
+    """Gates, values and results at addresses of their own, NaN before and behind what is read."""
+    def place(t, off):
+        flat = torch.full((t.numel() + 16,), float("nan"), dtype=t.dtype, device="cuda")
+        flat[off:off + t.numel()] = t.reshape(-1)
+        return flat[off:off + t.numel()].view(t.shape)
+    for m, c, io, out in ((400, 515, "bf16", "bf16"), (400, 516, "f32", "f32"), (30, 1024, "f16", "s8"), (310, 4096, "f32", "s8"), (310, 4099, "bf16", "f32"), (1, 7, "f16", "f16"), (3, 20000, "f32", "bf16")):
+        g, u = place((rand(1, m, c) * 3).to(TYPES[io]), g_off), place(rand(2, m, c).to(TYPES[io]), u_off)
+        op = enn.token_gate(ctx, enn.TokenGateDesc(m=m, c=c, act=enn.GATE_SILU, packed=0, in_dtype=code(enn, io), out_dtype=code(enn, out)))
+        outs = [guarded(m, enn.token_pitch(c), torch.int8, y_off), guarded(m, 1, torch.float32)] if out == "s8" else [guarded(m, c, TYPES[out], y_off)]
+        execute(op, m, [g, u], outs)
+        op.release()
+        a, err = act64(g.double(), "silu")
+        want = a * u.double()
+        err = err * u.double().abs() + U * want.abs()
+        assert torch.equal(outs[0][m:], guarded(m, outs[0].shape[1], outs[0].dtype, y_off)[m:])
+        if out == "s8":
+            check_bytes(outs[0][:m], outs[1][:m, 0], want, err, c)
+        else:
+            check_close(outs[0][:m], want, err, out)
+
+
 def test_token_gate_many_rows(enn, ctx):
     run_gate(enn, ctx, 4000, 200, "bf16", "s8", "silu", True)
     run_gate(enn, ctx, 700, 4000, "f16", "s8", "gelu_tanh", False)
