@@ -160,6 +160,8 @@ def _byte_weights(gen, n, k):
 
 
 def prepare(case, seed):
+    if own:
+        _use_the_operators_stream()
     gen = _generator(seed)
     m, op = case["m"], case["op"]
     s = _State(case=case)
@@ -287,7 +289,17 @@ def _plain(s):
 @functools.lru_cache(maxsize=None)
 def _library():
     enn = importlib.import_module("cl-eden-kernel_b200")
-    return enn, enn.Context(torch.cuda.current_device())
+    ctx = enn.Context(torch.cuda.current_device())
+    return enn, ctx, torch.cuda.ExternalStream(ctx.stream)
+
+
+def _use_the_operators_stream():
+    """The program's torch work runs on the stream of the operators, so that inputs, calls, what reads their results, and memory that is
+    given back and used again are in order without events or waits."""
+    _, ctx, stream = _library()
+    if torch.cuda.current_stream().cuda_stream != ctx.stream:
+        torch.cuda.synchronize()
+        torch.cuda.set_stream(stream)
 
 
 class _Op:
@@ -302,11 +314,10 @@ class _Op:
 
 def _prepare_own(s):
     """Prepares the operators on their weights and allocates their results, as a program does before its first call."""
-    enn, ctx = _library()
+    enn, ctx, _ = _library()
     types = {"f32": enn.F32, "f16": enn.F16, "bf16": enn.BF16}
     norms = {"none": enn.NORM_NONE, "rms": enn.NORM_RMS, "layer": enn.NORM_LAYER}
     acts = {"silu": enn.GATE_SILU, "gelu": enn.GATE_GELU, "gelu_tanh": enn.GATE_GELU_TANH, "relu": enn.GATE_RELU, "sigmoid": enn.GATE_SIGMOID}
-    torch.cuda.synchronize()      # the operators run on the context's stream
     case = s.case
     m, op = case["m"], case["op"]
 
