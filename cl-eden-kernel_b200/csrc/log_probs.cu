@@ -1,6 +1,6 @@
 // log_probs: log probabilities of given ids, entropy and the largest alternatives of rows of logits.
 //
-// Bound by reading the logits, which happens once: with k = scale * log2(e), m near the running maximum and d = k (l - m), a thread keeps
+// Bound by reading the logits, which happens once: with k = scale * log2(e), m the running maximum and d = k (l - m), a thread keeps
 //   S = sum 2^d   and   U = sum d 2^d,
 // rescaled whenever m grows (S' = c S, U' = c (U + d S) with d = k (m - m'), c = 2^d).  Then
 //   log p = scale (l - m) - ln S,   entropy = ln S - ln 2 U / S.
@@ -35,7 +35,6 @@ constexpr int kShortBytes = 16 << 10, kLongestBytes = 192 << 10;       // rows o
 constexpr int blocks_of(int threads) { return threads == kLongest ? 2 : (threads == kLong ? 3 : 8); }
 constexpr int kLookers = 8;             // threads that look at one thread's logits again
 constexpr float kNothing = -1e4f;       // 2^-10000 is 0; keeps the products d 2^d away from infinity times 0
-constexpr float kSlack = 20.f;
 constexpr float kLowest = -3.402823466e38f;
 
 // Order of the logits as unsigned integers: NaN above +inf, -0 equal to +0; the lower index first among equals.  0 is below all keys.
@@ -421,8 +420,9 @@ __global__ void __launch_bounds__(kThreads, blocks_of(kThreads)) log_probs_kerne
             at = at == mine0 + (kDepth - 1) * kSlot ? mine0 : at + kSlot;
             const float largest = largest_of(raw, T{});
             best = fmaxf(best, largest);
-            // m stays while nothing exceeds it by more than a factor of 2^kSlack: the sums have room for that.
-            if ((largest - a.m) * k > kSlack) a.rescale(fmaxf(largest, kLowest), k);
+            // m is the maximum, and not a value near it: the largest logit then counts as exactly 1 and 0, and log p and the entropy of a row
+            // that is all but certain are not what is left of two larger numbers.  (Moving m only by factors of 2^20 was no quicker.)
+            if (largest > a.m) a.rescale(largest, k);
             // Two at a time.  What is ruled out makes 0 times -inf of d 2^d, seen in U: the chunk is then done again with care, as are those
             // after it (a vocabulary is ruled out all over).
             const uint64_t minus_m = pair(-a.m, -a.m), k2 = pair(k, k);
