@@ -141,7 +141,7 @@ int32_t enn_b200_token_fc_prepare(enn_b200_context *ctx, const enn_b200_token_fc
     if (e != cudaSuccess) return cfail(ctx, e);
     if (tc_available(ctx) && (e = token_fc_plan(b.op)) != cudaSuccess) return cfail(ctx, e);
     b.op->impl = b.op->info.impl = t.fc.err_dev ? ENN_B200_IMPL_TCGEN05 : ENN_B200_IMPL_DIRECT;
-    b.op->info.macs = static_cast<int64_t>(d->m) * d->k * d->n;
+    b.op->info.macs = token_macs(d->m, d->k, d->n);
     b.op->info.algorithmic_bytes += static_cast<int64_t>(d->n) * d->k;
     b.op->info.out_c = d->n;
     return b.finish(out);

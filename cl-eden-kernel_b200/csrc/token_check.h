@@ -34,6 +34,17 @@ inline int32_t float_size(int32_t dtype) {
     return dtype == ENN_B200_F32 ? 4 : (dtype == ENN_B200_F16 || dtype == ENN_B200_BF16 ? 2 : 0);
 }
 
+// Most bytes a tensor may span: far above any device's memory, and far enough below 2^63 for the sums over an operator's tensors.
+constexpr int64_t kMostBytes = int64_t{1} << 60;
+// Rows of `row` bytes, `stride` bytes from one to the next.
+inline bool rows_fit(int32_t m, int64_t stride, int64_t row) { return m <= 1 || stride <= (kMostBytes - row) / (m - 1); }
+
+// Multiply-accumulates of a product, the largest number where they are more.
+inline int64_t token_macs(int32_t m, int32_t k, int32_t n) {
+    const int64_t mn = static_cast<int64_t>(m) * n;
+    return mn > INT64_MAX / k ? INT64_MAX : mn * k;
+}
+
 inline int64_t token_pitch(int32_t c) { return (static_cast<int64_t>(c) + 15) & ~int64_t{15}; }
 
 // The check_* return null and fill `call`, or what is wrong with the descriptor.
@@ -45,6 +56,7 @@ inline const char *check_token_fc(const enn_b200_token_fc_desc &d, TokenCall *ca
     if (d.in_pitch != 0 && d.in_pitch < d.k) return "token_fc: rows overlap (in_pitch < k)";
     if (d.in_pitch > (int64_t{1} << 38)) return "token_fc: in_pitch is too large";
     const int64_t pitch = d.in_pitch ? d.in_pitch : token_pitch(d.k);
+    if (!rows_fit(d.m, pitch, d.k)) return "token_fc: rows span more than 2^60 bytes";
     call->m = d.m;
     call->add_in(d.m ? (d.m - 1) * pitch + d.k : 0, 1);
     call->add_in(int64_t{4} * d.m, 4);
@@ -106,6 +118,7 @@ inline const char *check_log_probs(const enn_b200_log_probs_desc &d, TokenCall *
     if (d.in_pitch != 0 && d.in_pitch < d.vocab) return "log_probs: rows overlap (in_pitch < vocab)";
     if (d.in_pitch > (int64_t{1} << 38)) return "log_probs: in_pitch is too large";
     const int64_t pitch = d.in_pitch ? d.in_pitch : d.vocab;
+    if (!rows_fit(d.m, pitch * e, int64_t{e} * d.vocab)) return "log_probs: rows span more than 2^60 bytes";
     call->m = d.m;
     call->add_in(d.m ? ((d.m - 1) * pitch + d.vocab) * e : 0, e);
     if (d.given) call->add_in(int64_t{4} * d.m * d.given, 4);

@@ -167,6 +167,7 @@ typedef struct enn_b200_resize_desc {
  *      the blocks of a language model served in 8-bit integers.  No counterpart in the reference.  A row is a token; an
  *      operator is prepared once for up to `m` rows (0 .. 2^30) and enn_b200_op_execute_rows runs it on 0 .. m of them (1 for a
  *      decode step, more for a prompt).  Rows past the given number are neither read nor written.
+ *      The m rows of a tensor span at most 2^60 bytes.
  *
  * Quantised rows ("byte rows"): row t is c int8 values q[t][i] in [-127, 127], enn_b200_token_pitch(c) bytes from row to
  * row, and a float scale s[t]; they stand for q * s.  Rows are quantised as s = max_i |y_i| / 127,
