@@ -215,6 +215,7 @@ int32_t enn_b200_op_execute_rows(enn_b200_op *op, int32_t rows, const void *cons
     if (!op->token) return tfail(ctx, ENN_B200_INVALID_PARAMS, "not a token operator");
     const TokenState &t = *op->token;
     if (const char *wrong = check_rows_call(t.call, rows, ins, n_in, outs, n_out)) return tfail(ctx, ENN_B200_INVALID_PARAMS, wrong);
+    if (const char *wrong = check_rows_memory(t.call, rows, ins, outs)) return tfail(ctx, ENN_B200_INVALID_PARAMS, wrong);
     if (rows == 0) return ENN_B200_SUCCESS;
     OnDevice dev(ctx->device);
     if (!dev.ok()) return tfail(ctx, ENN_B200_CUDA_FAILURE, "the context's device cannot be selected");

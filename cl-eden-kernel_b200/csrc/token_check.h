@@ -9,22 +9,45 @@
 
 namespace enn_b200 {
 
+// Rows in memory: `row` bytes each, `stride` bytes from one to the next; `group` tokens share a row.
+struct RowLayout {
+    int64_t row = 0, stride = 0;
+    int32_t group = 1;
+    int64_t span(int32_t tokens) const {
+        const int64_t rows = tokens / group + (tokens % group ? 1 : 0);
+        return rows ? (rows - 1) * stride + row : 0;
+    }
+    // Whether `bytes` > 0 bytes at `other` reach into the rows of the tokens; what lies between rows is not theirs.
+    bool reached_by(const void *at, int32_t tokens, const void *other, int64_t bytes) const {
+        const uintptr_t a = reinterpret_cast<uintptr_t>(at), o = reinterpret_cast<uintptr_t>(other);
+        if (o < a) return static_cast<uint64_t>(bytes) > a - o;
+        if (o - a >= static_cast<uint64_t>(span(tokens))) return false;
+        const int64_t within = static_cast<int64_t>((o - a) % static_cast<uint64_t>(stride));
+        return within < row || within + bytes > stride;
+    }
+};
+
 // What a call of a prepared token operator is checked against.
 struct TokenCall {
     static constexpr int kMaxIns = 3, kMaxOuts = 4;
     int32_t m = 0;
     int32_t n_in = 0, n_out = 0;
+    RowLayout in[kMaxIns], out[kMaxOuts];
     int64_t in_bytes[kMaxIns] = {}, out_bytes[kMaxOuts] = {};      // of all m rows
     int32_t in_align[kMaxIns] = {}, out_align[kMaxOuts] = {};      // element sizes
     bool in_place = false;                                          // out 0 may be the memory of in 1 (token_norm's stream)
 
-    void add_in(int64_t bytes, int32_t align) {
+    void add_in(int64_t row, int64_t stride, int32_t align, int32_t group = 1) {
+        in[n_in] = RowLayout{row, stride, group};
         in_align[n_in] = align;
-        in_bytes[n_in++] = bytes;
+        in_bytes[n_in] = in[n_in].span(m);
+        ++n_in;
     }
-    void add_out(int64_t bytes, int32_t align) {
+    void add_out(int64_t row, int32_t align) {
+        out[n_out] = RowLayout{row, row, 1};
         out_align[n_out] = align;
-        out_bytes[n_out++] = bytes;
+        out_bytes[n_out] = out[n_out].span(m);
+        ++n_out;
     }
 };
 
@@ -58,20 +81,20 @@ inline const char *check_token_fc(const enn_b200_token_fc_desc &d, TokenCall *ca
     const int64_t pitch = d.in_pitch ? d.in_pitch : token_pitch(d.k);
     if (!rows_fit(d.m, pitch, d.k)) return "token_fc: rows span more than 2^60 bytes";
     call->m = d.m;
-    call->add_in(d.m ? (d.m - 1) * pitch + d.k : 0, 1);
-    call->add_in(int64_t{4} * d.m, 4);
-    call->add_out(static_cast<int64_t>(d.m) * d.n * e, e);
+    call->add_in(d.k, pitch, 1);
+    call->add_in(4, 4, 4);
+    call->add_out(static_cast<int64_t>(d.n) * e, e);
     return nullptr;
 }
 
-inline bool token_out(TokenCall *call, int32_t m, int32_t c, int32_t dtype) {
+inline bool token_out(TokenCall *call, int32_t c, int32_t dtype) {
     if (dtype == ENN_B200_S8) {
-        call->add_out(m * token_pitch(c), 1);
-        call->add_out(int64_t{4} * m, 4);
+        call->add_out(token_pitch(c), 1);
+        call->add_out(4, 4);
         return true;
     }
     const int32_t e = float_size(dtype);
-    call->add_out(static_cast<int64_t>(m) * c * e, e);
+    call->add_out(static_cast<int64_t>(c) * e, e);
     return e != 0;
 }
 
@@ -87,12 +110,12 @@ inline const char *check_token_norm(const enn_b200_token_norm_desc &d, TokenCall
     if (!std::isfinite(d.residual_scale)) return "token_norm: residual_scale must be finite";
     const int64_t row = static_cast<int64_t>(d.c) * e;
     call->m = d.m;
-    call->add_in(d.m * row, e);
-    if (d.residual) call->add_in(d.m * row, e);
-    if (d.gate_tokens) call->add_in((d.m / d.gate_tokens + (d.m % d.gate_tokens ? 1 : 0)) * row, e);
-    if (d.residual) call->add_out(d.m * row, e);
+    call->add_in(row, row, e);
+    if (d.residual) call->add_in(row, row, e);
+    if (d.gate_tokens) call->add_in(row, row, e, d.gate_tokens);
+    if (d.residual) call->add_out(row, e);
     call->in_place = d.residual != 0;
-    return token_out(call, d.m, d.c, d.out_dtype) ? nullptr : "token_norm: out_dtype must be F32, F16, BF16 or S8";
+    return token_out(call, d.c, d.out_dtype) ? nullptr : "token_norm: out_dtype must be F32, F16, BF16 or S8";
 }
 
 inline const char *check_token_gate(const enn_b200_token_gate_desc &d, TokenCall *call) {
@@ -103,9 +126,9 @@ inline const char *check_token_gate(const enn_b200_token_gate_desc &d, TokenCall
     if (!e) return "token_gate: in_dtype must be F32, F16 or BF16";
     const int64_t row = static_cast<int64_t>(d.c) * e;
     call->m = d.m;
-    call->add_in(d.m * row * (d.packed ? 2 : 1), e);
-    if (!d.packed) call->add_in(d.m * row, e);
-    return token_out(call, d.m, d.c, d.out_dtype) ? nullptr : "token_gate: out_dtype must be F32, F16, BF16 or S8";
+    call->add_in(row * (d.packed ? 2 : 1), row * (d.packed ? 2 : 1), e);
+    if (!d.packed) call->add_in(row, row, e);
+    return token_out(call, d.c, d.out_dtype) ? nullptr : "token_gate: out_dtype must be F32, F16, BF16 or S8";
 }
 
 inline const char *check_log_probs(const enn_b200_log_probs_desc &d, TokenCall *call) {
@@ -120,13 +143,13 @@ inline const char *check_log_probs(const enn_b200_log_probs_desc &d, TokenCall *
     const int64_t pitch = d.in_pitch ? d.in_pitch : d.vocab;
     if (!rows_fit(d.m, pitch * e, int64_t{e} * d.vocab)) return "log_probs: rows span more than 2^60 bytes";
     call->m = d.m;
-    call->add_in(d.m ? ((d.m - 1) * pitch + d.vocab) * e : 0, e);
-    if (d.given) call->add_in(int64_t{4} * d.m * d.given, 4);
-    if (d.given) call->add_out(int64_t{4} * d.m * d.given, 4);
-    call->add_out(int64_t{4} * d.m, 4);
+    call->add_in(int64_t{e} * d.vocab, pitch * e, e);
+    if (d.given) call->add_in(int64_t{4} * d.given, int64_t{4} * d.given, 4);
+    if (d.given) call->add_out(int64_t{4} * d.given, 4);
+    call->add_out(4, 4);
     if (d.top) {
-        call->add_out(int64_t{4} * d.m * d.top, 4);
-        call->add_out(int64_t{4} * d.m * d.top, 4);
+        call->add_out(int64_t{4} * d.top, 4);
+        call->add_out(int64_t{4} * d.top, 4);
     }
     return nullptr;
 }
@@ -147,6 +170,19 @@ inline const char *check_rows_call(const TokenCall &c, int32_t rows, const void 
             if (outs[o] == ins[i] && !(c.in_place && o == 0 && i == 1)) return "an output must not be an input's memory";
         for (int p = 0; p < o; ++p)
             if (outs[o] == outs[p]) return "two outputs must not be the same memory";
+    }
+    return nullptr;
+}
+
+// The memory of a call that check_rows_call has passed: null, or what is wrong with it.
+inline const char *check_rows_memory(const TokenCall &c, int32_t rows, const void *const *ins, void *const *outs) {
+    for (int o = 0; o < c.n_out && rows > 0; ++o) {
+        const int64_t bytes = c.out[o].span(rows);
+        for (int i = 0; i < c.n_in; ++i)
+            if (c.in[i].reached_by(ins[i], rows, outs[o], bytes) && !(c.in_place && o == 0 && i == 1 && outs[o] == ins[i]))
+                return "an output must not share memory with an input";
+        for (int p = 0; p < o; ++p)
+            if (c.out[p].reached_by(outs[p], rows, outs[o], bytes)) return "two outputs must not share memory";
     }
     return nullptr;
 }

@@ -333,7 +333,8 @@ int32_t enn_b200_log_probs_prepare(enn_b200_context *ctx, const enn_b200_log_pro
 int64_t enn_b200_token_pitch(int32_t c);
 /* Runs a token operator on the first `rows` (0 .. m) rows of its inputs: enqueues on the context's stream, whatever device
  * is current, and can be captured (the operator must then outlive the graph).  The inputs and outputs the descriptor asks for, in its order, aligned to their element
- * type (byte rows: q and out of token_fc are fast at 16-byte addresses; outputs of 16-byte alignment are written fastest). */
+ * type (byte rows: q and out of token_fc are fast at 16-byte addresses; outputs of 16-byte alignment are written fastest).
+ * Outputs that share memory with an input or with each other are refused, but for a stream written over itself. */
 int32_t enn_b200_op_execute_rows(enn_b200_op *op, int32_t rows, const void *const *ins_dev, int32_t n_in, void *const *outs_dev,
                                  int32_t n_out);
 

@@ -4,7 +4,7 @@ import math
 import pytest
 import torch
 
-from test_token_ops_gpu import TYPES, U, run_log_probs
+from test_token_ops_gpu import TYPES, U, execute, refused, run_log_probs
 
 pytestmark = pytest.mark.gpu
 
@@ -35,3 +35,21 @@ def test_log_probs_of_rows_that_are_all_but_certain(enn, ctx, m, v, io, early, l
     assert bool(((given[:, 0].double() - (want - d)).abs() <= (12 + 2 * d) * U).all())
     assert bool(((entropy.double() - want_entropy).abs() <= 24 * U).all()), float((entropy.double() - want_entropy).abs().max() / U)
     assert torch.equal(top_ids[d > 0][:, 0], torch.full_like(top_ids[d > 0][:, 0], late))
+
+
+# ---- calls ------------------------------------------------------------------------------------------------------------
+
+def test_outputs_that_share_memory_are_refused(enn, ctx):
+    """A stream that is shifted against itself, results inside an input or another result; next to each other they pass."""
+    m, c = 16, 40
+    flat = torch.zeros(8, m * c + 64, dtype=torch.bfloat16, device="cuda")
+    x, r, h, y = (flat[i].data_ptr() for i in range(4))
+    size = m * c * 2
+    op = enn.token_norm(ctx, enn.TokenNormDesc(m=m, c=c, norm=enn.NORM_RMS, residual=1, io_dtype=enn.BF16, out_dtype=enn.BF16, eps=1e-6, residual_scale=1.0))
+    torch.cuda.synchronize()
+    for outs in ([r + 2, y], [r + size - 2, y], [r - 2, y], [x + 16, y], [h, r + 80], [h, h + 16], [r, r + 16]):
+        refused(enn, op.execute_rows, m, [x, r], outs)
+    op.execute_rows(m, [x, r], [r, y])
+    op.execute_rows(m // 2, [x, r], [r, r + size // 2])
+    ctx.sync()
+    op.release()
