@@ -107,6 +107,10 @@ int32_t tc_test_starve_next(enn_b200_op *op);
 int32_t tc_fuse_add(enn_b200_op *op, const AddParams &add, bool conv_is_second);
 void tc_set_residual(enn_b200_op *op, const void *res);
 void tc_clear_error(enn_b200_op *op);
+
+bool op_gave_up(const enn_b200_op *op) {
+    return (op->impl == ENN_B200_IMPL_TCGEN05 && tc_gave_up(op)) || (op->impl == ENN_B200_IMPL_DEPTHWISE && dw_ring_gave_up(op)) || (op->token && op->token->fc.gave_up());
+}
 }  // namespace enn_b200
 
 extern "C" {

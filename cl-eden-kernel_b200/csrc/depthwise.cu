@@ -799,6 +799,11 @@ void dw_ring_clear_error(enn_b200_op *op) {
     if (pl && pl->err_host) *pl->err_host = 0;
 }
 
+bool dw_ring_gave_up(const enn_b200_op *op) {
+    const DwRingPlan *pl = static_cast<const DwRingPlan *>(op->dw_ring);
+    return pl && pl->err_host && *static_cast<volatile const int32_t *>(pl->err_host) != 0;
+}
+
 // Returns cudaErrorNotSupported when the plan cannot serve this call (pointers not aligned for the bulk copies and the
 // 32-bit stores), cudaErrorLaunchFailure when an earlier launch gave up on a barrier wait.
 cudaError_t dw_ring_launch(enn_b200_op *op, const void *in, void *out) {

@@ -1883,6 +1883,11 @@ void tc_clear_error(enn_b200_op *op) {
     if (plan && plan->err_host) *plan->err_host = 0;
 }
 
+bool tc_gave_up(const enn_b200_op *op) {
+    const TcPlan *plan = static_cast<const TcPlan *>(op->tc);
+    return plan && plan->err_host && *static_cast<volatile const int32_t *>(plan->err_host) != 0;
+}
+
 void tc_release(enn_b200_op *op) {
     free_plan(static_cast<TcPlan *>(op->tc));
     op->tc = nullptr;

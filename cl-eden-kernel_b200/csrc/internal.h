@@ -143,6 +143,9 @@ bool dw_ring_plan(enn_b200_op *op);
 cudaError_t dw_ring_launch(enn_b200_op *op, const void *in, void *out);
 void dw_ring_release(enn_b200_op *op);
 void dw_ring_clear_error(enn_b200_op *op);
+bool dw_ring_gave_up(const enn_b200_op *op);
+bool tc_gave_up(const enn_b200_op *op);            // gemm_tc.cu
+bool op_gave_up(const enn_b200_op *op);            // abi.cu: a kernel of the operator gave up on a wait and nobody has cleared that
 cudaError_t add_kernel_init();
 cudaError_t launch_add(const AddParams &p, int64_t count, const void *a, const void *b, void *out, int sm_count,
                        cudaStream_t s);

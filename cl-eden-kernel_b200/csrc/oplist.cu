@@ -76,6 +76,13 @@ int32_t run_node(const enn_b200_oplist::Node &n, F ptr) {
     for (int t : n.more_outs) outs[n_out++] = ptr(t);
     return enn_b200_op_execute_rows(n.op, n.op->token->call.m, ins, n_in, outs, n_out);
 }
+// A kernel of the list that gave up on a wait leaves its results unwritten: known once the work is complete, and until the operator's
+// error is cleared.
+int32_t check_waits(enn_b200_oplist *l) {
+    for (auto &n : l->nodes)
+        if (enn_b200::op_gave_up(n.op)) return lfail(l, ENN_B200_CUDA_FAILURE, "oplist: a kernel gave up on a barrier wait");
+    return ENN_B200_SUCCESS;
+}
 int32_t run_nodes(enn_b200_oplist *l, int slot = 0) {
     auto ptr = [&](int t) {
         auto &T = l->tensors[t];
@@ -297,6 +304,7 @@ int32_t enn_b200_oplist_finalize(enn_b200_oplist *l) {
     int32_t st = run_nodes(l);
     if (st != ENN_B200_SUCCESS) return st;
     if (cudaStreamSynchronize(ctx->stream) != cudaSuccess) return lfail(l, ENN_B200_CUDA_FAILURE, "oplist: warm-up pass failed");
+    if ((st = check_waits(l)) != ENN_B200_SUCCESS) return st;
     if (n_nodes > 0) {
         if (cudaStreamBeginCapture(ctx->stream, cudaStreamCaptureModeThreadLocal) != cudaSuccess)
             return lfail(l, ENN_B200_CUDA_FAILURE, "oplist: stream capture could not start");
@@ -315,6 +323,7 @@ int32_t enn_b200_oplist_finalize(enn_b200_oplist *l) {
         st = run_nodes(l, 1);      // eager pass on the alternate pointers (operators cache per-pointer state)
         if (st != ENN_B200_SUCCESS) return st;
         if (cudaStreamSynchronize(ctx->stream) != cudaSuccess) return lfail(l, ENN_B200_CUDA_FAILURE, "oplist: warm-up pass failed");
+        if ((st = check_waits(l)) != ENN_B200_SUCCESS) return st;
         if (cudaStreamBeginCapture(ctx->stream, cudaStreamCaptureModeThreadLocal) != cudaSuccess)
             return lfail(l, ENN_B200_CUDA_FAILURE, "oplist: stream capture could not start");
         st = run_nodes(l, 1);
@@ -338,6 +347,8 @@ int32_t enn_b200_oplist_finalize(enn_b200_oplist *l) {
 int32_t enn_b200_oplist_execute_device(enn_b200_oplist *l) {
     if (!l || !l->finalized) return lfail(l, ENN_B200_INVALID_PARAMS, "oplist not finalized");
     if (!l->exec) return ENN_B200_SUCCESS;
+    const int32_t st = check_waits(l);
+    if (st != ENN_B200_SUCCESS) return st;
     if (cudaGraphLaunch(l->exec, l->ctx->stream) != cudaSuccess) return lfail(l, ENN_B200_CUDA_FAILURE, "oplist: graph launch failed");
     return ENN_B200_SUCCESS;
 }
@@ -361,7 +372,7 @@ int32_t enn_b200_oplist_execute(enn_b200_oplist *l, const void *const *host_inpu
             return lfail(l, ENN_B200_CUDA_FAILURE, "oplist_execute: output copy failed");
     }
     if (cudaStreamSynchronize(s) != cudaSuccess) return lfail(l, ENN_B200_CUDA_FAILURE, "oplist_execute: stream synchronisation failed");
-    return ENN_B200_SUCCESS;
+    return check_waits(l);
 }
 
 // Pipelined ExecuteSubGraph: returns as soon as the work is queued.  The host-to-device copy of this submission runs
@@ -422,7 +433,8 @@ int32_t enn_b200_oplist_submit(enn_b200_oplist *l, const void *const *host_input
     if ((!l->inputs.empty() && !host_inputs) || (!l->outputs.empty() && !host_outputs)) return lfail(l, ENN_B200_INVALID_PARAMS, "oplist_submit: null buffer table");
     if (!l->exec || !l->exec_alt) return enn_b200_oplist_execute(l, host_inputs, host_outputs);
     const int slot = static_cast<int>(l->seq & 1);
-    int32_t st = submit_inputs(l, host_inputs, slot);
+    int32_t st = check_waits(l);
+    if (st == ENN_B200_SUCCESS) st = submit_inputs(l, host_inputs, slot);
     if (st == ENN_B200_SUCCESS) st = submit_run(l, host_outputs, slot, nullptr, 0);
     if (st != ENN_B200_SUCCESS) return st;
     l->slot_used[slot] = true;
@@ -448,6 +460,10 @@ int32_t enn_b200_oplist_submit_round(enn_b200_oplist *const *lists, int32_t n, c
             if (lists[j] == l) return lfail(l, ENN_B200_INVALID_PARAMS, "oplist_submit_round: a list named twice");
     }
     for (int32_t k = 0; k < n; ++k) {
+        const int32_t st = check_waits(lists[k]);
+        if (st != ENN_B200_SUCCESS) return st;
+    }
+    for (int32_t k = 0; k < n; ++k) {
         const int32_t st = submit_inputs(lists[k], host_inputs[k], static_cast<int>(lists[k]->seq & 1), lists, n);
         if (st != ENN_B200_SUCCESS) return st;
     }
@@ -467,7 +483,7 @@ int32_t enn_b200_oplist_wait(enn_b200_oplist *l) {
     if (l->copy_stream && cudaStreamSynchronize(l->copy_stream) != cudaSuccess) return lfail(l, ENN_B200_CUDA_FAILURE, "oplist_wait: copy stream failed");
     if (cudaStreamSynchronize(l->ctx->stream) != cudaSuccess) return lfail(l, ENN_B200_CUDA_FAILURE, "oplist_wait: stream synchronisation failed");
     if (l->out_stream && cudaStreamSynchronize(l->out_stream) != cudaSuccess) return lfail(l, ENN_B200_CUDA_FAILURE, "oplist_wait: output stream failed");
-    return ENN_B200_SUCCESS;
+    return check_waits(l);
 }
 
 int32_t enn_b200_oplist_tensor_ptr(enn_b200_oplist *l, int32_t tensor_id, void **dev_ptr) {
@@ -524,6 +540,7 @@ int32_t enn_b200_oplist_profile(enn_b200_oplist *l, int32_t repeats, float *node
             cudaEventRecord(ev[i + 1], ctx->stream);
         }
         if (st == ENN_B200_SUCCESS && cudaStreamSynchronize(ctx->stream) != cudaSuccess) st = lfail(l, ENN_B200_CUDA_FAILURE, "oplist_profile: execution failed");
+        if (st == ENN_B200_SUCCESS) st = check_waits(l);
         for (int i = 0; i < n && st == ENN_B200_SUCCESS && rep >= 0; ++i) {
             float ms = 0.f;
             cudaEventElapsedTime(&ms, ev[i], ev[i + 1]);

@@ -216,6 +216,7 @@ int32_t enn_b200_op_execute_rows(enn_b200_op *op, int32_t rows, const void *cons
     const TokenState &t = *op->token;
     if (const char *wrong = check_rows_call(t.call, rows, ins, n_in, outs, n_out)) return tfail(ctx, ENN_B200_INVALID_PARAMS, wrong);
     if (const char *wrong = check_rows_memory(t.call, rows, ins, outs)) return tfail(ctx, ENN_B200_INVALID_PARAMS, wrong);
+    if (t.fc.gave_up()) return tfail(ctx, ENN_B200_CUDA_FAILURE, "token_fc: the kernel gave up on a barrier wait earlier");
     if (rows == 0) return ENN_B200_SUCCESS;
     OnDevice dev(ctx->device);
     if (!dev.ok()) return tfail(ctx, ENN_B200_CUDA_FAILURE, "the context's device cannot be selected");
@@ -226,7 +227,6 @@ int32_t enn_b200_op_execute_rows(enn_b200_op *op, int32_t rows, const void *cons
         case OP_TOKEN_GATE: e = token_gate_launch(op, rows, ins, outs); break;
         case OP_LOG_PROBS: e = log_probs_launch(op, rows, ins, outs); break;
     }
-    if (e == cudaErrorLaunchFailure && t.fc.err_host && *t.fc.err_host) return tfail(ctx, ENN_B200_CUDA_FAILURE, "token_fc: the kernel gave up on a barrier wait earlier");
     return e == cudaSuccess ? ENN_B200_SUCCESS : cfail(ctx, e);
 }
 

@@ -638,8 +638,6 @@ cudaError_t token_fc_plan(enn_b200_op *op) {
 }
 
 cudaError_t token_fc_launch(enn_b200_op *op, int32_t rows, const void *const *ins, void *const *outs) {
-    const TokenFcParams &f = op->token->fc;
-    if (f.err_host && *reinterpret_cast<volatile int32_t *>(f.err_host) != 0) return cudaErrorLaunchFailure;
     switch (op->token->out_dtype) {
         case ENN_B200_F32: return launch_typed<float>(op, rows, ins, outs);
         case ENN_B200_F16: return launch_typed<__half>(op, rows, ins, outs);

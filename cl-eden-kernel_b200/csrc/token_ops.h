@@ -45,6 +45,7 @@ struct TokenFcParams {
     CUtensorMap map_w;
     int32_t *err_host, *err_dev;      // pinned word in which a kernel that gave up on a wait leaves a code
     bool starve_next;                 // the next call is a self-test of that
+    bool gave_up() const { return err_host && *static_cast<volatile const int32_t *>(err_host) != 0; }
     TokenFcDirect direct() const { return {k, n, in_pitch, w_pitch, w, channel_scale, bias}; }
 };
 

@@ -1,10 +1,13 @@
 """Token operators: calls that earlier tests do not make.  Tolerances count roundings, u = 2^-24."""
+import ctypes as C
 import math
 
+import numpy as np
 import pytest
 import torch
 
-from test_token_ops_gpu import TYPES, U, execute, refused, run_log_probs
+import cases
+from test_token_ops_gpu import TYPES, U, fc_check, fc_inputs, guarded, refused, run_log_probs
 
 pytestmark = pytest.mark.gpu
 
@@ -53,3 +56,102 @@ def test_outputs_that_share_memory_are_refused(enn, ctx):
     op.execute_rows(m // 2, [x, r], [r, r + size // 2])
     ctx.sync()
     op.release()
+
+
+# ---- kernels that give up on a wait -----------------------------------------------------------------------------------
+
+def gave_up(enn, f, *args):
+    with pytest.raises(enn.EnnError) as e:
+        f(*args)
+    assert e.value.status == enn.CUDA_FAILURE and "gave up" in str(e.value)
+
+
+@pytest.mark.parametrize("m,k,n", [(3, 1024, 512), (2000, 512, 4096)])
+def test_a_replayed_product_that_gives_up_is_known_to_a_call_of_no_rows(enn, m, k, n):
+    ctx = enn.Context(0)
+    q, w, s, sw, _ = fc_inputs(21, m, k, n)
+    op = enn.token_fc(ctx, enn.TokenFcDesc(m=m, k=k, n=n, out_dtype=enn.F32), w.data_ptr(), sw.data_ptr())
+    y = guarded(m, n, torch.float32)
+    stream = torch.cuda.ExternalStream(ctx.stream)
+    graphs = []
+    for starve in (True, False):
+        if starve:
+            op.test_starve_next()
+        graph = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph, stream=stream):
+            op.execute_rows(m, [q.data_ptr(), s.data_ptr()], [y.data_ptr()])
+        graphs.append(graph)
+    op.execute_rows(0, [None, None], [None])
+    for graph, works in zip(graphs, (False, True)):
+        with torch.cuda.stream(stream):
+            graph.replay()
+        ctx.sync()
+        if works:
+            op.execute_rows(0, [None, None], [None])
+        else:
+            gave_up(enn, op.execute_rows, 0, [None, None], [None])
+            gave_up(enn, op.execute_rows, m, [q.data_ptr(), s.data_ptr()], [y.data_ptr()])
+            op.clear_error()
+    fc_check(y[:m], q, w, s, sw, None, "f32", k)
+    del graph, graphs
+    op.release()
+    ctx.close()
+
+
+@pytest.mark.parametrize("kind", ["token_fc", "conv"])
+def test_lists_report_kernels_that_gave_up(enn, ctx, kind):
+    """The word that a kernel left is seen by every way of running the list, and nothing else of it changes."""
+    ol = enn.OpList(ctx)
+    if kind == "token_fc":
+        m, k, n = 16, 512, 256
+        rng = np.random.default_rng(5)
+        host = [rng.integers(-100, 100, (m, k), dtype=np.int8), np.linspace(0.01, 0.02, m, dtype=np.float32)]
+        op = enn.token_fc(ctx, enn.TokenFcDesc(m=m, k=k, n=n, out_dtype=enn.F32), rng.integers(-100, 100, (n, k), dtype=np.int8), np.full(n, 0.01, np.float32))
+    else:
+        d, x, w, b, sc = cases.conv_case(seed=5, n=2, h=16, w=16, cin=64, cout=64, k=1, per_channel=True, out_scale=0.3)
+        op = enn.conv2d(ctx, d, w, b, sc)
+        host = [np.ascontiguousarray(x)]
+    assert op.info.impl == enn.IMPL_TCGEN05
+    size = op.info.out_bytes
+    ids = [ol.tensor(a.nbytes) for a in host]
+    out = ol.tensor(size)
+    handle = C.c_void_p(op.h.value)
+    if kind == "token_fc":
+        ol.add_n(op, ids, [out])
+    else:
+        ol.add(op, ids, out)
+    ol.set_io(ids, [out], [size])
+    ol.finalize()
+    ins = [a.ctypes.data for a in host]
+
+    def run(how):
+        got = np.zeros(size, np.uint8)
+        if how == "execute":
+            ol.execute_host_ptrs(ins, [got.ctypes.data])
+        else:
+            ol.submit_host_ptrs(ins, [got.ctypes.data])
+            ol.wait()
+        return got
+
+    want = run("execute")
+    assert want.any() and np.array_equal(want, run("submit"))
+    devs = [ctx.to_device(a) for a in host] + [ctx.malloc(size)]
+    ctx.check(enn.lib.enn_b200_op_test_starve_next(handle))
+    if kind == "token_fc":
+        addresses = (C.c_void_p * 2)(devs[0].value, devs[1].value)
+        ctx.check(enn.lib.enn_b200_op_execute_rows(handle, 16, addresses, 2, (C.c_void_p * 1)(devs[2].value), 1))
+    else:
+        ctx.check(enn.lib.enn_b200_op_execute(handle, devs[0], devs[1]))
+    ctx.sync()
+    gave_up(enn, run, "execute")
+    gave_up(enn, run, "submit")
+    gave_up(enn, ol.wait)
+    gave_up(enn, ol.profile, 1)
+    gave_up(enn, ol.execute_device)
+    ctx.check(enn.lib.enn_b200_op_clear_error(handle))
+    for how in ("execute", "submit", "submit", "execute"):
+        assert np.array_equal(want, run(how))
+    ol.destroy()
+    for d in devs:
+        ctx.free(d)
