@@ -587,7 +587,7 @@ int32_t enn_b200_fc_prepare(enn_b200_context *ctx, const enn_b200_fc_desc *d, co
 int32_t enn_b200_add_prepare(enn_b200_context *ctx, const enn_b200_add_desc *d, enn_b200_op **out) {
     if (!ctx || !d || !out) return fail(ctx, ENN_B200_INVALID_PARAMS, "null argument");
     *out = nullptr;
-    if (d->count < 0 || d->act_dtype >= ENN_B200_F32 || !(d->in0_scale > 0.f) || !(d->in1_scale > 0.f) || !(d->out_scale > 0.f))
+    if (d->count < 0 || is_float_dtype(d->act_dtype) || !(d->in0_scale > 0.f) || !(d->in1_scale > 0.f) || !(d->out_scale > 0.f))
         return fail(ctx, ENN_B200_INVALID_PARAMS, "bad add descriptor");
     enn_b200_op *op = new (std::nothrow) enn_b200_op();
     if (!op) return fail(ctx, ENN_B200_FAILURE, "out of host memory");
@@ -663,7 +663,7 @@ int32_t enn_b200_avgpool_prepare(enn_b200_context *ctx, const enn_b200_pool_desc
     if (!ctx || !d || !out) return fail(ctx, ENN_B200_INVALID_PARAMS, "null argument");
     *out = nullptr;
     if (d->n < 0 || d->h <= 0 || d->w <= 0 || d->c <= 0 || d->kh <= 0 || d->kw <= 0 || d->stride_h <= 0 || d->stride_w <= 0 ||
-        d->out_h <= 0 || d->out_w <= 0 || d->pad_t < 0 || d->pad_l < 0 || d->act_dtype >= ENN_B200_F32 || !(d->out_scale > 0.f))
+        d->out_h <= 0 || d->out_w <= 0 || d->pad_t < 0 || d->pad_l < 0 || is_float_dtype(d->act_dtype) || !(d->out_scale > 0.f))
         return fail(ctx, ENN_B200_INVALID_PARAMS, "bad pool descriptor");
     enn_b200_op *op = new (std::nothrow) enn_b200_op();
     if (!op) return fail(ctx, ENN_B200_FAILURE, "out of host memory");

@@ -286,7 +286,7 @@ int32_t enn_b200_maxpool_prepare(enn_b200_context *ctx, const enn_b200_pool_desc
     if (!ctx || !d || !out) return gfail(ctx, ENN_B200_INVALID_PARAMS, "null argument");
     *out = nullptr;
     if (d->n < 0 || d->h <= 0 || d->w <= 0 || d->c <= 0 || d->kh <= 0 || d->kw <= 0 || d->stride_h <= 0 || d->stride_w <= 0 ||
-        d->out_h <= 0 || d->out_w <= 0 || d->pad_t < 0 || d->pad_l < 0 || d->act_dtype >= ENN_B200_F32 || !(d->out_scale > 0.f))
+        d->out_h <= 0 || d->out_w <= 0 || d->pad_t < 0 || d->pad_l < 0 || is_float_dtype(d->act_dtype) || !(d->out_scale > 0.f))
         return gfail(ctx, ENN_B200_INVALID_PARAMS, "bad pool descriptor");
     enn_b200_op *op = new (std::nothrow) enn_b200_op();
     if (!op) return gfail(ctx, ENN_B200_FAILURE, "out of host memory");
@@ -319,7 +319,7 @@ int32_t enn_b200_mean_prepare(enn_b200_context *ctx, const enn_b200_mean_desc *d
         if (d->axis_mask & (1 << a)) count *= d->dims[a];
         else out_elems *= d->dims[a];
     }
-    if ((d->axis_mask & ~15) || count > (1 << 23) || d->act_dtype >= ENN_B200_F32) return gfail(ctx, ENN_B200_INVALID_PARAMS, "mean: bad axis mask or too many elements per output");
+    if ((d->axis_mask & ~15) || count > (1 << 23) || is_float_dtype(d->act_dtype)) return gfail(ctx, ENN_B200_INVALID_PARAMS, "mean: bad axis mask or too many elements per output");
     enn_b200_op *op = new_graph_op(ctx, OP_MEAN);
     if (!op) return gfail(ctx, ENN_B200_FAILURE, "out of host memory");
     MeanGeom &g = static_cast<GraphOpState *>(op->graph_state)->mean;
@@ -341,7 +341,7 @@ int32_t enn_b200_mean_prepare(enn_b200_context *ctx, const enn_b200_mean_desc *d
 int32_t enn_b200_concat_prepare(enn_b200_context *ctx, const enn_b200_concat_desc *d, enn_b200_op **out) {
     if (!ctx || !d || !out) return gfail(ctx, ENN_B200_INVALID_PARAMS, "null argument");
     *out = nullptr;
-    if (d->n_inputs < 1 || d->n_inputs > ENN_B200_CONCAT_MAX_INPUTS || d->outer < 0 || d->act_dtype >= ENN_B200_F32 || !(d->out_scale > 0.f))
+    if (d->n_inputs < 1 || d->n_inputs > ENN_B200_CONCAT_MAX_INPUTS || d->outer < 0 || is_float_dtype(d->act_dtype) || !(d->out_scale > 0.f))
         return gfail(ctx, ENN_B200_INVALID_PARAMS, "bad concat descriptor");
     enn_b200_op *op = new_graph_op(ctx, OP_CONCAT);
     if (!op) return gfail(ctx, ENN_B200_FAILURE, "out of host memory");
@@ -378,7 +378,7 @@ int32_t enn_b200_concat_prepare(enn_b200_context *ctx, const enn_b200_concat_des
 int32_t enn_b200_softmax_prepare(enn_b200_context *ctx, const enn_b200_softmax_desc *d, enn_b200_op **out) {
     if (!ctx || !d || !out) return gfail(ctx, ENN_B200_INVALID_PARAMS, "null argument");
     *out = nullptr;
-    if (d->outer < 0 || d->channels <= 0 || d->inner <= 0 || d->act_dtype >= ENN_B200_F32 || !(d->in_scale > 0.f) || !(d->out_scale > 0.f))
+    if (d->outer < 0 || d->channels <= 0 || d->inner <= 0 || is_float_dtype(d->act_dtype) || !(d->in_scale > 0.f) || !(d->out_scale > 0.f))
         return gfail(ctx, ENN_B200_INVALID_PARAMS, "bad softmax descriptor");
     enn_b200_op *op = new_graph_op(ctx, OP_SOFTMAX);
     if (!op) return gfail(ctx, ENN_B200_FAILURE, "out of host memory");
@@ -405,7 +405,7 @@ int32_t enn_b200_softmax_prepare(enn_b200_context *ctx, const enn_b200_softmax_d
 int32_t enn_b200_resize_bilinear_prepare(enn_b200_context *ctx, const enn_b200_resize_desc *d, enn_b200_op **out) {
     if (!ctx || !d || !out) return gfail(ctx, ENN_B200_INVALID_PARAMS, "null argument");
     *out = nullptr;
-    if (d->n < 0 || d->h <= 0 || d->w <= 0 || d->c <= 0 || d->out_h <= 0 || d->out_w <= 0 || d->act_dtype >= ENN_B200_F32)
+    if (d->n < 0 || d->h <= 0 || d->w <= 0 || d->c <= 0 || d->out_h <= 0 || d->out_w <= 0 || is_float_dtype(d->act_dtype))
         return gfail(ctx, ENN_B200_INVALID_PARAMS, "bad resize descriptor");
     enn_b200_op *op = new_graph_op(ctx, OP_RESIZE);
     if (!op) return gfail(ctx, ENN_B200_FAILURE, "out of host memory");

@@ -82,6 +82,9 @@ __host__ __device__ inline uint32_t add_lut2_index(uint32_t a, uint32_t b) {
 
 struct TokenState;     // token_ops.h
 
+// Element types that the byte operators refuse; every other value but ENN_B200_S8 means unsigned bytes to those that do not check it.
+inline bool is_float_dtype(int32_t dtype) { return dtype == ENN_B200_F32 || dtype == ENN_B200_F16 || dtype == ENN_B200_BF16; }
+
 struct PoolGeom {
     int32_t n, h, w, c, kh, kw, sh, sw, pt, pl, oh, ow;
     int32_t act_min, act_max, is_signed;

@@ -155,3 +155,45 @@ def test_lists_report_kernels_that_gave_up(enn, ctx, kind):
     ol.destroy()
     for d in devs:
         ctx.free(d)
+
+
+# ---- byte operators and float types -----------------------------------------------------------------------------------
+
+def byte_operators(enn):
+    """Each operator that takes a type for its bytes: how it is prepared, a descriptor, and its inputs."""
+    rng = np.random.default_rng(9)
+    x = rng.integers(0, 256, (1, 6, 6, 8), dtype=np.uint8)
+    pool = dict(n=1, h=6, w=6, c=8, kh=2, kw=2, stride_h=2, stride_w=2, out_h=3, out_w=3, out_scale=0.1, out_zp=3)
+    q = dict(in_scale=0.1, in_zp=3, out_scale=1 / 256)
+    concat = enn.ConcatDesc(n_inputs=2, outer=36, out_scale=0.2, out_zp=4)
+    for i in range(2):
+        concat.inner[i], concat.in_scale[i], concat.in_zp[i] = 8, 0.1 + 0.1 * i, 3
+    return [(enn.add, enn.AddDesc(count=288, in0_scale=0.1, in0_zp=3, in1_scale=0.2, in1_zp=5, out_scale=0.3, out_zp=7), [x, x[:, ::-1]], 288),
+            (enn.avgpool, enn.PoolDesc(**pool), [x], 72), (enn.maxpool, enn.PoolDesc(**pool), [x], 72), (enn.mean, enn.mean_desc((1, 6, 6, 8), (1, 2)), [x], 8),
+            (enn.concat, concat, [x, x[:, ::-1]], 576), (enn.softmax, enn.SoftmaxDesc(outer=36, channels=8, inner=1, beta=1.0, **q), [x], 288),
+            (enn.resize_bilinear, enn.ResizeDesc(n=1, h=6, w=6, c=8, out_h=9, out_w=5), [x], 360)]
+
+
+@pytest.mark.parametrize("which", range(7))
+def test_byte_operators_refuse_the_float_types_and_no_other_value(enn, ctx, which):
+    prepare, desc, ins, size = byte_operators(enn)[which]
+    devs = [ctx.to_device(a) for a in ins]
+    out = ctx.malloc(size)
+
+    def run():
+        op = prepare(ctx, desc)
+        op.execute_n(devs, out)
+        got = ctx.download(out, (size,))
+        op.release()
+        return got
+
+    desc.act_dtype = enn.U8
+    want = run()
+    for other in (2, 15, 19, 64, 1 << 20, -1, -16):
+        desc.act_dtype = other
+        assert np.array_equal(run(), want), other
+    for floating in (enn.F32, enn.F16, enn.BF16):
+        desc.act_dtype = floating
+        refused(enn, prepare, ctx, desc)
+    for d in devs + [out]:
+        ctx.free(d)
