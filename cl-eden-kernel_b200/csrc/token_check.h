@@ -137,7 +137,7 @@ inline const char *check_log_probs(const enn_b200_log_probs_desc &d, TokenCall *
     if (!e) return "log_probs: in_dtype must be F32, F16 or BF16";
     if (d.given < 0 || d.given > 1024) return "log_probs: given must be within 0 .. 1024";
     if (d.top < 0 || d.top > ENN_B200_LOG_PROBS_MAX_TOP || d.top > d.vocab) return "log_probs: top must be within 0 .. min(vocab, 32)";
-    if (!(d.scale > 0.f) || std::isinf(d.scale)) return "log_probs: scale must be positive and finite";
+    if (!(d.scale > 0.f) || d.scale > 0x1p127f) return "log_probs: scale must be positive and at most 2^127";      // scale * log2(e) is a float
     if (d.in_pitch != 0 && d.in_pitch < d.vocab) return "log_probs: rows overlap (in_pitch < vocab)";
     if (d.in_pitch > (int64_t{1} << 38)) return "log_probs: in_pitch is too large";
     const int64_t pitch = d.in_pitch ? d.in_pitch : d.vocab;

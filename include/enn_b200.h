@@ -218,7 +218,7 @@ typedef struct enn_b200_token_gate_desc {
  *   given[t][j] = log p[ids[t][j]]  (a negative id gives 0, one past the vocabulary NaN)
  *   entropy[t]  = - sum_i p_i log p_i, where p_i = 0 adds nothing
  *   top_ids[t], top[t]: the `top` largest logits in descending order, the lower index first among equals, and their log p.
- * -inf rules a logit out.  A row that is ruled out as a whole, or holds +inf or a NaN, has no distribution: NaN in place of
+ * -inf rules a logit out, and so does lying further below the row's largest than a float reaches.  A row that is ruled out as a whole, or holds +inf or a NaN, has no distribution: NaN in place of
  * its numbers; top_ids are then still in order, NaN above all.
  * Inputs {logits [m][vocab], int32 ids [m][given] if given}, outputs {given if given, entropy, int32 top_ids and top if top};
  * results are float. */
@@ -228,7 +228,7 @@ typedef struct enn_b200_log_probs_desc {
     int32_t in_dtype;               /* ENN_B200_F32 | F16 | BF16 */
     int32_t given;                  /* ids per row, 0 .. 1024 */
     int32_t top;                    /* alternatives per row, 0 .. min(vocab, ENN_B200_LOG_PROBS_MAX_TOP) */
-    float scale;                    /* 1 / temperature, > 0 */
+    float scale;                    /* 1 / temperature, > 0 .. 2^127 */
     int64_t in_pitch;               /* logits from row to row; 0: vocab */
 } enn_b200_log_probs_desc;
 

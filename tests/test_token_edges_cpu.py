@@ -16,7 +16,7 @@ def checks(tmp_path_factory):
     return exe
 
 
-@pytest.mark.parametrize("which", ["sizes", "overlaps", "calls"])
+@pytest.mark.parametrize("which", ["sizes", "overlaps", "calls", "scales"])
 def test_checks(checks, which):
     r = subprocess.run([checks, which], capture_output=True, text=True)
     assert r.returncode == 0, r.stdout + r.stderr

@@ -40,6 +40,27 @@ def test_log_probs_of_rows_that_are_all_but_certain(enn, ctx, m, v, io, early, l
     assert torch.equal(top_ids[d > 0][:, 0], torch.full_like(top_ids[d > 0][:, 0], late))
 
 
+@pytest.mark.parametrize("scale", [2.0 ** 127, 2.0 ** 64, 2.0 ** -126, 1e-45])
+def test_log_probs_with_scales_at_the_limits(enn, ctx, scale):
+    """A temperature of nearly nothing leaves the largest logits alone, one beyond all logits leaves equal shares: exact but for
+    the logarithm: an ulp and a rounding of ln 3 (3 u), of ln 8192 (16 u and 8 u)."""
+    v = 8192
+    logits = torch.arange(v, dtype=torch.float32, device="cuda").flip(0).repeat(3, 1)
+    logits[1, 100:103] = 1e6
+    logits[2, 50:] = torch.finfo(torch.float32).min
+    ids = torch.tensor([[0, 1], [101, 0], [0, 60]], dtype=torch.int32, device="cuda")
+    given, entropy, top_ids, top = run_log_probs(enn, ctx, logits, ids, 2, scale=scale)
+    assert top_ids.tolist() == [[0, 1], [100, 101], [0, 1]]
+    if scale > 1:
+        ln = torch.tensor([0.0, math.log(3), 0.0], device="cuda")
+        assert bool(((entropy - ln).abs() <= 3 * U).all()) and bool(((given[:, 0] + ln).abs() <= 3 * U).all())
+        far = given[:, 1] if scale > 2.0 ** 100 else given[2:, 1]
+        assert bool((far < -1e18).all()) and not bool(torch.isnan(given).any()) and not bool(torch.isnan(top).any())
+    else:      # z differs by 2^-126 * 1e6 at most, but for the lowest value: z = -4 there with the scale 2^-126
+        shares = torch.tensor([v, v], dtype=torch.float64, device="cuda")
+        assert bool(((entropy[:2].double() - torch.log(shares)).abs() <= 24 * U).all()) and bool(((given[:2].double() + torch.log(shares)[:, None]).abs() <= 24 * U).all())
+
+
 # ---- calls ------------------------------------------------------------------------------------------------------------
 
 def test_outputs_that_share_memory_are_refused(enn, ctx):

@@ -1,6 +1,7 @@
 // Sizes and calls of the token operators at their limits (csrc/token_check.h), without a device.
 #include "token_check.h"
 
+#include <cmath>
 #include <cstdio>
 #include <cstring>
 #include <initializer_list>
@@ -100,11 +101,23 @@ static void calls() {
     expect(fc(100, far, far + 400) && !fc(100, far, far + 396) && !fc(100, far, far - 2796) && fc(100, far, far - 2800) && !fc(100, far, x + 3296) && fc(100, far, x + 3300), "fc");
 }
 
+static void scales() {
+    for (float scale : {1e-45f, 1.f, 0x1p126f, 0x1p127f}) {
+        TokenCall c;
+        expect(!check_log_probs({2, 100, ENN_B200_F32, 1, 5, scale, 0}, &c), "a scale whose product with log2(e) is a float");
+    }
+    for (float scale : {std::nextafterf(0x1p127f, INFINITY), 3.402823466e38f, INFINITY, -1.f, -0.f}) {
+        TokenCall c;
+        expect(check_log_probs({2, 100, ENN_B200_F32, 1, 5, scale, 0}, &c), "a scale whose product with log2(e) is none");
+    }
+}
+
 int main(int argc, char **argv) {
     const char *which = argc > 1 ? argv[1] : "";
     if (!std::strcmp(which, "sizes")) sizes();
     else if (!std::strcmp(which, "overlaps")) overlaps();
     else if (!std::strcmp(which, "calls")) calls();
+    else if (!std::strcmp(which, "scales")) scales();
     else expect(false, "which test?");
     return failures ? 1 : 0;
 }
