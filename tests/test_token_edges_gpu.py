@@ -7,9 +7,85 @@ import pytest
 import torch
 
 import cases
-from test_token_ops_gpu import TYPES, U, fc_check, fc_inputs, guarded, refused, run_log_probs
+from test_token_ops_gpu import (TYPES, U, check_bytes, check_close, check_log_probs, code, execute, fc_check, fc_inputs, guarded, norm_case, norm_reference,
+                                rand, refused, run_log_probs)
 
 pytestmark = pytest.mark.gpu
+
+
+def kept(buf, rows, offset=0):
+    """Everything in a guarded() buffer outside its first `rows` rows is the pattern, what lies before them too."""
+    flat = torch.empty(0, dtype=buf.dtype, device="cuda").set_(buf.untyped_storage())
+    want = (torch.arange(flat.numel(), device="cuda") % 97).to(buf.dtype)
+    end = offset + rows * buf.shape[1]
+    return torch.equal(flat[:offset], want[:offset]) and torch.equal(flat[end:], want[end:])
+
+
+# ---- addresses --------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("m", [1, 20, 150, 700])
+@pytest.mark.parametrize("q_offset,pitch,out_offset", [(0, 101, 0), (1, 112, 0), (0, 208, 1), (3, 150, 3), (16, 112, 8), (0, 112, 4)])
+@pytest.mark.parametrize("out", ["f32", "f16"])
+def test_token_fc_writes_its_rows_alone(enn, ctx, m, q_offset, pitch, out_offset, out):
+    k, n = 100, 9001 if m == 700 else 72
+    q, w, s, sw, _ = fc_inputs(9, m, k, n, pitch)
+    flat = torch.zeros(q.numel() + 64, dtype=torch.int8, device="cuda")
+    moved = flat[q_offset:q_offset + q.numel()].view(q.shape)
+    moved.copy_(q)
+    op = enn.token_fc(ctx, enn.TokenFcDesc(m=m, k=k, n=n, out_dtype=code(enn, out), in_pitch=pitch), w.data_ptr(), sw.data_ptr())
+    for rows in (m, max(1, m - 3)):
+        y = guarded(m, n, TYPES[out], out_offset)
+        execute(op, rows, [moved, s], [y])
+        fc_check(y[:rows], q[:rows], w, s[:rows], sw, None, out, k)
+        assert kept(y, rows, out_offset)
+    op.release()
+
+
+@pytest.mark.parametrize("out_off,y_off", [(0, 0), (1, 3), (4, 1), (7, 5)])
+@pytest.mark.parametrize("m,c,io,out", [(400, 515, "bf16", "bf16"), (30, 1024, "f16", "s8"), (310, 4097, "bf16", "s8"), (5, 1001, "f32", "f16"), (700, 67, "f16", "f32"),
+                                        (3, 32767, "bf16", "s8"), (1, 7, "bf16", "bf16")])
+def test_token_norm_writes_its_rows_alone(enn, ctx, m, c, io, out, out_off, y_off):
+    """What lies before the first row and behind the last, in both results and in the scales, stays as it was."""
+    x, r = rand(1, m, c).to(TYPES[io]), rand(2, m, c).to(TYPES[io])
+    op = enn.token_norm(ctx, enn.TokenNormDesc(m=m, c=c, norm=enn.NORM_RMS, residual=1, io_dtype=code(enn, io), out_dtype=code(enn, out), eps=1e-6, residual_scale=0.5))
+    for rows in {m, max(1, m - 2)}:
+        h, y, s = guarded(m, c, TYPES[io], out_off), guarded(m, enn.token_pitch(c) if out == "s8" else c, TYPES.get(out, torch.int8), y_off), guarded(m, 1, torch.float32, 1)
+        execute(op, rows, [x, r], [h, y] + ([s] if out == "s8" else []))
+        stream, (want, err) = norm_reference(norm_case(m, c, io, out), x[:rows], r[:rows], None, (None,) * 4, 0.5, float(np.float32(1e-6)))
+        check_close(h[:rows], *stream, io)
+        if out == "s8":
+            check_bytes(y[:rows], s[:rows, 0], want, err, c)
+        else:
+            check_close(y[:rows], want, err, out)
+        assert kept(h, rows, out_off) and kept(y, rows, y_off) and kept(s, rows if out == "s8" else 0, 1)
+    op.release()
+
+
+@pytest.mark.parametrize("io,out", [("bf16", "bf16"), ("f16", "s8"), ("f32", "s8"), ("bf16", "f32")])
+@pytest.mark.parametrize("m,c", [(3000, 67), (2000, 1001), (1500, 4097), (400, 12301), (900, 264), (5000, 9), (2, 32765)])
+@pytest.mark.parametrize("x_off,r_off", [(0, 0), (3, 0), (0, 5), (1, 1)])
+def test_token_norm_stream_in_place_between_lines(enn, ctx, m, c, io, out, x_off, r_off):
+    """Rows that share lines with their neighbours, written over the stream they were read from: the bits of a run into memory of its own."""
+    def place(t, off):
+        flat = torch.zeros(t.numel() + 16, dtype=t.dtype, device="cuda")
+        return flat[off:off + t.numel()].view(t.shape).copy_(t)
+    e = TYPES[io]
+    x, r, gate = place(rand(1, m, c).to(e), x_off), place(rand(2, m, c).to(e), r_off), rand(3, -(-m // 50), c).to(e)
+    weight = 1 + 0.3 * rand(4, c)
+    torch.cuda.synchronize()
+    op = enn.token_norm(ctx, enn.TokenNormDesc(m=m, c=c, norm=enn.NORM_RMS, post_norm=enn.NORM_LAYER, residual=1, gate_tokens=50, io_dtype=code(enn, io), out_dtype=code(enn, out),
+                                               eps=1e-6, post_eps=1e-6, residual_scale=0.7), weight.data_ptr())
+    results = []
+    for in_place in (False, True, True):
+        stream = place(r, r_off)
+        h = stream if in_place else torch.zeros_like(r)
+        y = torch.zeros(m, enn.token_pitch(c) if out == "s8" else c, dtype=TYPES.get(out, torch.int8), device="cuda")
+        s = torch.zeros(m, device="cuda")
+        execute(op, m, [x, stream, gate], [h, y] + ([s] if out == "s8" else []))
+        results.append((h.clone(), y, s))
+    for again in results[1:]:
+        assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(results[0], again))
+    op.release()
 
 
 # ---- log_probs --------------------------------------------------------------------------------------------------------
@@ -38,6 +114,27 @@ def test_log_probs_of_rows_that_are_all_but_certain(enn, ctx, m, v, io, early, l
     assert bool(((given[:, 0].double() - (want - d)).abs() <= (12 + 2 * d) * U).all())
     assert bool(((entropy.double() - want_entropy).abs() <= 24 * U).all()), float((entropy.double() - want_entropy).abs().max() / U)
     assert torch.equal(top_ids[d > 0][:, 0], torch.full_like(top_ids[d > 0][:, 0], late))
+
+
+@pytest.mark.parametrize("m,v,io,top", [(600, 3000, "bf16", 20), (500, 1001, "f16", 5), (700, 37, "f32", 32), (3000, 500, "f32", 1), (230, 49500, "f32", 20), (500, 20000, "f16", 0)])
+def test_log_probs_of_rows_without_a_distribution_among_others(enn, ctx, m, v, io, top):
+    """A CTA that takes several rows meets rows of -inf, NaN and +inf between ordinary ones, and rows with little left: each keeps to itself."""
+    logits = (rand(m + v, m, v) * 3).to(TYPES[io])
+    bad = torch.zeros(m, dtype=torch.bool, device="cuda")
+    logits[0::7] = -math.inf
+    logits[2::7, v // 2] = math.nan
+    logits[4::7, v - 1] = math.inf
+    bad[0::7], bad[2::7], bad[4::7] = True, True, True
+    logits[1::7, v // 3:] = -math.inf
+    logits[3::7, :] = logits[3::7, :].clamp(max=-1)
+    logits[3::7, v - 1] = 5
+    ids = torch.randint(0, v, (m, 1), device="cuda", dtype=torch.int32)
+    given, entropy, top_ids, top_lp = run_log_probs(enn, ctx, logits, ids, top)
+    assert bool(torch.isnan(given[bad]).all()) and bool(torch.isnan(entropy[bad]).all()) and (not top or bool(torch.isnan(top_lp[bad]).all()))
+    if top:
+        assert torch.equal(top_ids[0].long(), torch.arange(top, device="cuda")) and bool((top_ids[2::7, 0] == v // 2).all()) and bool((top_ids[4::7, 0] == v - 1).all())
+    ok = ~bad
+    check_log_probs(logits[ok], ids[ok], top, (given[ok], entropy[ok], top_ids[ok] if top else None, top_lp[ok] if top else None))
 
 
 @pytest.mark.parametrize("scale", [2.0 ** 127, 2.0 ** 64, 2.0 ** -126, 1e-45])
