@@ -211,7 +211,7 @@ __global__ void __launch_bounds__(kTcThreads) token_fc_kernel(const __grid_const
         pdl_wait();
         const int per = p.splits * (kTcThreads / 32);
 #pragma unroll 2
-        for (int j = split + p.splits * warp; j < tokens; j += per) {
+        for (int j = split + p.splits * warp; j < tokens && n < p.n; j += per) {
             const float ts = scales[j];
             const uint32_t at = ring + j * (kChannels * 4) + lane * 16;
             int4 a = make_int4(0, 0, 0, 0);
@@ -225,16 +225,18 @@ __global__ void __launch_bounds__(kTcThreads) token_fc_kernel(const __grid_const
             }
             const float v[4] = {scaled(a.x, ts, cs[0], b[0]), scaled(a.y, ts, cs[1], b[1]), scaled(a.z, ts, cs[2], b[2]), scaled(a.w, ts, cs[3], b[3])};
             O *o = out + (m0 + j) * p.n + n;
-            if (p.vec && n < p.n) {
+            if (p.vec) {
                 store4(o, v);
-            } else if (!p.vec) {
+            } else {
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
                     if (n + i < p.n) o[i] = from_float<O>(v[i]);
             }
         }
     }
-    // Nobody leaves while its sums are still read; the results' stores need not be waited for.
+    // Nobody leaves while its sums are still read.  The arrival is relaxed, so that it does not wait for the results' stores; it has no need to order
+    // memory: a lane reads sums of other CTAs only where it stores what it makes of them, and its loads have returned by then.
+    __syncwarp();
     if (p.splits > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
     else __syncthreads();
     if (warp == 2) {
