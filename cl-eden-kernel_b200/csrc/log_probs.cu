@@ -8,7 +8,7 @@
 // bounds the n-th largest logit from below, so that what is above it lies with those threads, and their logits alone are looked at again.
 // A row is split over a cluster of up to eight CTAs where the rows alone do not occupy the device; the parts meet in the first CTA's
 // shared memory, without atomics or workspace.  All orders are total (value, then index), so that results do not depend on timing.
-// 2048x65536 f32 with one alternative 101 us (5.3 TB/s), 93 us without; 1x131072 8.1 us, half of it the search.  16-bit rows are bound by
+// 2048x65536 f32 with one id and one alternative 106 us (5.1 TB/s), 93 us without both; 1x131072 8.1 us, half of it the search.  16-bit rows are bound by
 // instructions (8 a logit, one of them 2^x, of which an SM does 16 a cycle): 2048x65536 bf16 48 us without alternatives (5.6 TB/s).
 #include <math_constants.h>
 
@@ -27,9 +27,12 @@ constexpr int kMaxSegments = 8;
 constexpr int kChunk = 4;               // 16-byte pieces a thread works on at a time
 constexpr int kDepth = 2;               // chunks a thread asks for ahead
 constexpr int kCandidates = 1024;
-// Threads of a CTA: kLong; kShort for many short rows, whose time is that of the reductions and of the search, one step after the other:
-// more rows side by side (4000x2000 bf16 42 us with kLong, 18 us so); kLongest where the stream is most of it (2048x65536 f32, 20
-// alternatives, 118 us with kLong, 108 us so; 4000x16000 bf16 64 and 93 us).  And the CTAs an SM is to hold.
+// Threads of a CTA, and the CTAs an SM is to hold.  kLong; kShort for short rows that are more than the device holds CTAs of kLong, whose time is that of
+// the reductions and of the search, one step after the other: more rows side by side (bf16 with five alternatives: 450x2000 9.0 us with kLong,
+// 6.1 us so, 4000x2000 42 and 18 us, with 20: 450x8000 10.2 and 11.7 us, 1000x8000 16.4 and 14.3 us; below, 440x2000 6.9 us with kLong, 6.2 us with kShort,
+// 440x8000 7.4 and 11.3 us).  kLongest where the stream is most of it (f32 with 20 alternatives, kLong and kLongest: 1000x24576 28.3 and 34.0 us,
+// 800x40000 33.6 and 37.8 us, 600x49152 34.6 and 31.6 us, 2048x65536 118 and 109 us).  16-bit rows of these bytes have twice the logits and gain
+// nothing (1000x98304 bf16 54 and 60 us, 2048x131072 bf16 126 and 128 us).
 constexpr int kLongest = 512, kLong = 256, kShort = 64;
 constexpr int kShortBytes = 16 << 10, kLongestBytes = 192 << 10;       // rows of up to, segments of at least
 constexpr int blocks_of(int threads) { return threads == kLongest ? 2 : (threads == kLong ? 3 : 8); }
@@ -292,7 +295,7 @@ __device__ __forceinline__ uint64_t reached_by(uint64_t mine, int top, Shared<kT
         }
     }
     __syncthreads();
-    if (static_cast<int>(threadIdx.x) < n) {      // at most 36 keys
+    if (static_cast<int>(threadIdx.x) < n) {      // at most 64 keys, and never more than threads
         const uint64_t k = sh.firsts[threadIdx.x];
         int place = 0;
         for (int j = 0; j < n; ++j) {

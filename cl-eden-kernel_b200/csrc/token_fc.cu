@@ -251,17 +251,23 @@ __global__ void __launch_bounds__(kTcThreads) token_fc_kernel(const __grid_const
 // into while the other is scaled and stored, 32 channels x 32 tokens at a time by a warp of the epilogue.  16-bit results are transposed
 // on their way through shared memory and leave in 16-byte pieces, 64 bytes of a token; others (n not a multiple of eight, 32-bit
 // results) leave straight from the accumulators' layout, where a thread has one channel: 32 neighbouring channels of a token per instruction.
-// 8192 x 4096 -> 8192: 178 us in a short run (3.1 POPS, tensor pipe 78 % busy), 210 us under the power limit of a long one.  The width of the
-// token tiles follows the rounds (512 x 4096 -> 4096: 14.6 us in 64 tiles of 128, 20 us on single CTAs); below kPairRows tokens
-// single CTAs with a split reduction read the weights faster (200 x 4096 -> 4096 15.0 against 16.4 us).
-//   warp 0, 1        as above, of both CTAs; warp 1 is the issuer in the first CTA and allocates in both
+// 8192 x 4096 -> 8192: 178 us in a short run (3.1 POPS, tensor pipe 78 % busy), 207 us under the power limit of a long one.  The width of the
+// token tiles follows the rounds (512 x 4096 -> 4096: 13.0 us in 64 tiles of 128, 14.8 us on single CTAs).  Below kPairRows tokens
+// single CTAs with a split reduction are quicker where the weights are few, and about as quick where they are many (pairs in parentheses):
+// 160 x 4096 -> 4096 10.2 us (12.4), 64 x 8192 -> 16384 26.4 us (27.5), 128 x 8192 -> 16384 29.2 us (28.3).  From there pairs lose less than
+// they gain: 200 x 4096 -> 4096 11.2 us (12.2), 256 x 4096 -> 4096 12.1 us (12.3), 200 x 8192 -> 16384 38.6 us (30.4), 300 x 1024 -> 4096 9.6 us (7.2).
+//   warp 0           copies the weight tiles, of both CTAs
+//   warp 1           issues the matrix instructions in the first CTA; allocates in both
 //   warps 2 .. 9     epilogue: lane quarter warp & 3, every other group of 32 tokens
 //   warp 10          copies the token tiles
 constexpr int kPairStages = 6;
 constexpr int kPairEpiWarps = 8;
 constexpr int kPairThreads = (kPairEpiWarps + 3) * 32;
 constexpr int kPairStageBytes = (kBM + kMaxBN / 2) * kBK;
-constexpr int kPairRows = 192, kTileCost = 48;
+constexpr int kPairRows = 192;
+// What a tile costs beside its columns, in columns; found by trying.  Less takes tiles that are too narrow (512 x 4096 -> 4096 13.0 us, 17.0 with 0, 14.9 with
+// 24; 2048 x 4096 -> 6144 38 us, 99 with 0), more some that are too wide (256 x 4096 -> 4096 12.3 us, 15.9 with 96; 8192 x 512 -> 4096 23.4, 24.1).
+constexpr int kTileCost = 48;
 constexpr int kPairOutBytes = 32 * 32 * 2;      // results of a warp on their way out
 
 struct PairCall {
@@ -304,7 +310,9 @@ __device__ __forceinline__ void pair_tile(const PairCall &p, int tile, int &tc, 
     tc = b * p.band + (r - tt * width);
 }
 
-// The accumulators have been read into registers: that needs no order with the results' stores, for which a release would wait.
+// Gives an accumulator back without a release, which would wait for the results' stores as well.  What has to be over is the reading of
+// tensor memory alone, and it is: tcgen05.wait::ld has brought the values of every load into registers, and the tcgen05 fence before the arrival
+// with the one that the issuer takes after its wait orders these loads before the next matrix instructions.  Nothing else passes from here to the issuer.
 __device__ __forceinline__ void arrive_relaxed(uint32_t cluster_addr) {
     asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }

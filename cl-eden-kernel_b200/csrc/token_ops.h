@@ -53,7 +53,8 @@ struct TokenFcParams {
 struct TokenState {
     TokenCall call;
     int32_t in_dtype = 0, out_dtype = 0;
-    int32_t sms = 0;        // SMs a launch may occupy (option grid_cap when the operator was prepared)
+    int32_t sms = 0;        // what launches are sized for (option grid_cap when the operator was prepared, else all): the persistent kernels,
+                            // pairs of token_fc, norms and log_probs of many rows, keep to as many CTAs as they hold; the others have a CTA per tile
     bool residual = false, packed = false;
     NormParams norm{};
     GateParams gate{};

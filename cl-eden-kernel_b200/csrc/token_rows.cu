@@ -4,7 +4,7 @@
 // A row belongs to a warp (up to 1024 channels), a CTA, or for quantised gates a cluster; a thread holds up to eight groups of eight
 // neighbouring channels, 16 bytes of a 16-bit type.  Constant vectors come from L1, which they share with nothing: rows are loaded and
 // stored past it (those of gates between lines, which have no such vectors, through it).  Measured in queued passes: gates 8192x12288
-// bf16 92 us (6.6 TB/s), norms on both sides of a block with the stream 8192x5120 bf16 66 us (5.1 TB/s; half of the issue slots busy, 28
+// bf16 92 us (6.6 TB/s), norms on both sides of a block with the stream 8192x5120 bf16 65 us (5.2 TB/s; half of the issue slots busy, 28
 // instructions a channel, the rest the latency of three reductions a row).
 #include <algorithm>
 #include <type_traits>
@@ -349,7 +349,7 @@ __device__ __forceinline__ void norm_row(const Row<NV, LINES> &row, float (&f)[N
 
 // Threads that the registers of NV groups a thread leave an SM: 64 registers each, 80 with four groups, 96 with eight.  One block may
 // have them all, so that eight groups, which spill, remain for rows above 24576 channels (2048x10240 bf16 with a stream: 46 us in eight
-// groups, 29 us in four; 33x10241: 12.9 us, 6.5 us in two).
+// groups, 29 us in four; 33x10241 bf16 to bytes with a stream: 12.9 us, 6.5 us in two).
 constexpr int norm_threads(int nv) { return nv <= 2 ? 1024 : (nv == 4 ? 768 : 544); }
 
 // A thread's own ring in shared memory: `depth` rows ahead, each with `streams` tensors, filled by asynchronous copies.  A thread reads
@@ -397,10 +397,12 @@ __device__ __forceinline__ void ahead_wait(int pending) {
 }
 constexpr int kMaxDepth = 4;
 constexpr int kRingBytes = 216 * 1024;      // at most
-constexpr int kRingShare = 112 * 1024;      // of an SM: what they take, L1 lacks for the constant vectors (8192x5120: 65 us with all of it, 61 us so)
+// Of an SM: what they take, L1 lacks for the constant vectors (the same tensors pass after pass: 8192x5120 bf16, both norms and a stream, 67 us with
+// all of it, 61 us so; 2048x12289 bf16 to bytes with a stream 88 and 83 us; 2048x8192 f32, both norms and a stream, 72 us either way).
+constexpr int kRingShare = 112 * 1024;
 
-// BYTES: the result is quantised.  A kernel of its own, since one for both overflows the instruction cache (2048x4097 bf16: 27.1 us, 25.1 us
-// so; 8192x1001: 20.7 and 18.4 us).
+// BYTES: the result is quantised.  A kernel of its own, since one for both overflows the instruction cache (with a stream: 2048x4097 bf16 to bytes
+// 27.1 us, 25.1 us so; 8192x1001 bf16 20.7 and 18.4 us).
 template <typename T, int NV, bool LINES, bool BYTES>
 __global__ void __launch_bounds__(norm_threads(NV), 1) token_norm_kernel(NormParams p, int32_t rows, int32_t out_dtype, int32_t depth, const T *x,
                                                                                        const T *residual, const T *gate, T *stream, void *out, float *scale) {
@@ -595,9 +597,9 @@ bool aligned(const void *p, size_t to) { return reinterpret_cast<uintptr_t>(p) %
 
 // Threads of a row and groups per thread for `n` channels.  `spread`: as many threads as there are groups (few rows: latency), else
 // four groups each (many rows: what a row costs whatever its length, reductions and addresses, is shared by more channels), up to
-// `most(groups)` threads; `two`: two, where four are too many (the code for shifted groups then overflows the instruction cache: norms of
-// 2048x4097 30 us, 27 us with two, gates of 4096x4099 35 us, 26 us; the rows of 32-bit types in flight leave L1 nothing: norms of 2048x8192
-// 82 us, 72 us with two).
+// `most(groups)` threads; `two`: two, where four are too many (the code for shifted groups then overflows the instruction cache: 2048x4097 bf16 to
+// bytes with a stream 30 us, 27 us with two, gates of 4096x4099 bf16 35 us, 26 us; the rows of 32-bit types in flight leave L1 nothing:
+// 2048x8192 f32, both norms and a stream, 82 us, 72 us with two).
 struct Shape {
     int nt, nv, per_block;
 };

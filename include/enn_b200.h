@@ -277,7 +277,8 @@ void *enn_b200_stream(enn_b200_context *ctx);
  * pack_wide, no_bres, no_bres_k1, tc_bn (>= 96), tc_pair, tc_raster, dw_legacy, dw_rows, no_fuse, fuse_all, no_out_stream, no_narrow_n, no_gconv,
  * gc_per_sm (1 or 2); no_wide_store, no_implicit, no_fan_out and epi_g are accepted and change nothing.
  * grid_cap = G: operators prepared afterwards launch at most G CTAs of their persistent tensor-core kernels (GEMM and gather
- * convolution) and as many of the row-ring depthwise kernel as G SMs hold.  Meant for several contexts that share one GPU, each
+ * convolution, large token_fc products) and as many of the row-ring depthwise, token_norm and log_probs kernels as G SMs hold; kernels with
+ * a CTA for every tile (token_gate, small token_fc products and others) are not limited.  Meant for several contexts that share one GPU, each
  * running its own operator list: with G = SMs / 4 their kernels run side by side in four shares instead of taking
  * the whole GPU in turn, which hides the latency of the small layers (MobileNetV2-u8, 256 images: 1.25 ms per step
  * with eight lists of 37 SMs against 1.43 ms with three uncapped lists; 32 images: 0.22 against 0.34 ms).
