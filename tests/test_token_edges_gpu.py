@@ -32,6 +32,7 @@ def test_token_fc_writes_its_rows_alone(enn, ctx, m, q_offset, pitch, out_offset
     flat = torch.zeros(q.numel() + 64, dtype=torch.int8, device="cuda")
     moved = flat[q_offset:q_offset + q.numel()].view(q.shape)
     moved.copy_(q)
+    torch.cuda.synchronize()
     op = enn.token_fc(ctx, enn.TokenFcDesc(m=m, k=k, n=n, out_dtype=code(enn, out), in_pitch=pitch), w.data_ptr(), sw.data_ptr())
     for rows in (m, max(1, m - 3)):
         y = guarded(m, n, TYPES[out], out_offset)
@@ -188,6 +189,7 @@ def gave_up(enn, f, *args):
 def test_a_replayed_product_that_gives_up_is_known_to_a_call_of_no_rows(enn, m, k, n):
     ctx = enn.Context(0)
     q, w, s, sw, _ = fc_inputs(21, m, k, n)
+    torch.cuda.synchronize()
     op = enn.token_fc(ctx, enn.TokenFcDesc(m=m, k=k, n=n, out_dtype=enn.F32), w.data_ptr(), sw.data_ptr())
     y = guarded(m, n, torch.float32)
     stream = torch.cuda.ExternalStream(ctx.stream)
