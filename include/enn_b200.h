@@ -382,7 +382,8 @@ int32_t enn_b200_op_info(const enn_b200_op *op, enn_b200_op_info_t *info);
  * bounded barrier wait ran out leaves a code in host-visible memory and every later execute of that operator returns
  * CUDA_FAILURE until enn_b200_op_clear_error; enn_b200_op_execute_rows does with 0 rows too, which asks for the code and no
  * more (after a captured graph was replayed and waited for).  An operator list that holds such an operator reports it where the
- * list's work is waited for (execute, wait, profile) and runs no more until then.  enn_b200_op_test_starve_next arms a self-test of exactly that path for
+ * list's work is waited for (execute, wait, profile) and runs no more until the handle, which stays valid in the list, is cleared
+ * (a model is opened again).  enn_b200_op_test_starve_next arms a self-test of exactly that path for
  * a tensor-core operator: its next execute issues no operand copy and uses a wait limit of under a millisecond, so the
  * kernel gives up with nothing in flight, releases its tensor memory and returns; outputs of that execute are
  * undefined. */
