@@ -65,7 +65,7 @@ static void calls() {
     static char buf[16384];
     TokenCall n;      // 4 rows of 40 16-bit channels, a row of gates for 3 tokens, to bytes (48 a row) and scales
     expect(!check_token_norm({4, 40, ENN_B200_NORM_RMS, ENN_B200_NORM_NONE, 1, 3, ENN_B200_BF16, ENN_B200_S8, 1e-6f, 0.f, 1.f}, &n), "a norm");
-    char *x = buf, *r = buf + 640, *g = buf + 1280, *h = buf + 2048, *q = buf + 3072, *s = buf + 4096;
+    char *x = buf, *r = buf + 640, *g = buf + 1280, *h = buf + 2048, *q = buf + 2560, *s = buf + 4096;
     const auto norm = [&](int32_t rows, char *ho, char *qo, char *so) {
         const void *ins[] = {x, r, g};
         void *outs[] = {ho, qo, so};
